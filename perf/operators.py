@@ -1,0 +1,440 @@
+"""Performance cases of the operators that stand next to the MoC layers in a block:
+the short causal convolution (``moc.causal_conv``), the selective state space scan
+(``moc.selective_scan``) and layer norm (``moc.layer_norm``).
+
+``listed()`` names the cases, ``draw(rng)`` gives more of the same ranges,
+``prepare(case, seed)`` makes the inputs on the GPU, ``run(state)`` is one pass
+through one operator: the framework's where ``own`` is true, elementary torch
+operations in 32 bits (running sums of decays in 64) otherwise.  ``exact(case,
+seed)`` is the operator's definition in 64 bits, one token after the other.
+
+A case has an ``op`` (conv, scan, norm) and a ``kind``:
+
+  step     one decode token per sequence, the cache updated in place
+  forward  without gradients, the final state returned (conv, scan)
+  chunk    the same, continuing from a cache
+  train    forward and the gradients of every input
+
+``tokens`` > 0 packs sequences of uneven lengths behind ``cu_seqlens``; otherwise
+the batch is ``batch`` x ``time``.
+"""
+from __future__ import annotations
+
+import math
+import random
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+_DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
+_Q = 64  # tokens of a chunk of the plain scan
+
+
+def _moc():
+    pkg = str(Path(__file__).resolve().parents[1] / "mixture-of-convolutions_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import moc
+    return moc
+
+
+def _case(name, op, kind, batch=0, time=0, tokens=0, shortest=0, longest=0, dtype="bf16",
+          dim=0, s=0, act="", heads=0, p=0, n=0, groups=1):
+    c = {"op": op, "kind": kind, "batch": batch, "time": time, "tokens": tokens,
+         "shortest": shortest, "longest": longest, "dtype": dtype, "dim": dim, "s": s, "act": act,
+         "heads": heads, "p": p, "n": n, "groups": groups}
+    if name:
+        c["name"] = name
+    return c
+
+
+def listed():
+    return [
+        # a few users' token-by-token generation: the smallest call, all latency
+        _case("conv_step", "conv", "step", 8, 1, dim=2048, s=4, act="silu"),
+        # the convolution of the benchmark layer's shape, as a training step
+        _case("conv_train", "conv", "train", 4, 4096, dim=2048, s=4, act="silu"),
+        # packed ragged sequences, fp32, channel count off every vector width
+        _case("conv_packed_fp32", "conv", "train", tokens=6007, shortest=1, longest=1500,
+              dtype="fp32", dim=1130, s=3),
+        # decode of a serving batch: each sequence's state read and written
+        _case("scan_step", "scan", "step", 256, 1, heads=32, p=64, n=128),
+        # decode of a small fp32 model, a handful of sequences: latency
+        _case("scan_step_fp32", "scan", "step", 5, 1, dtype="fp32", heads=12, p=48, n=16, groups=2),
+        # a training step at the benchmark layer's tokens and channels
+        _case("scan_train", "scan", "train", 4, 4096, heads=32, p=64, n=128),
+        # packed ragged sequences in fp32, sizes off every tile, two groups
+        _case("scan_train_packed_fp32", "scan", "train", tokens=5003, shortest=1, longest=1900,
+              dtype="fp32", heads=10, p=40, n=24, groups=2),
+        # one long prompt of one user
+        _case("scan_prompt", "scan", "forward", 1, 16381, heads=32, p=64, n=128),
+        # a short piece of several prompts, continuing from their states
+        _case("scan_chunk", "scan", "chunk", 8, 777, heads=24, p=64, n=64),
+        # the norm before a decode step's projections: latency
+        _case("norm_tokens", "norm", "forward", 8, 1, dim=2048),
+        # the norm of a training step at the benchmark layer's shape
+        _case("norm_train", "norm", "train", 4, 4096, dim=2048),
+        # fp32, odd row length
+        _case("norm_train_fp32", "norm", "train", 3, 1667, dtype="fp32", dim=1131),
+    ]
+
+
+def _spread(rng, lo, hi):
+    """A whole number between lo and hi, spread over its logarithm."""
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    dtype = rng.choice(["bf16", "fp32"])
+    op = rng.choice(["conv", "scan", "scan", "norm"])
+    if op == "norm":
+        rows, dim = _spread(rng, 1, 16384), _spread(rng, 64, 8192)
+        rows = max(1, min(rows, 16384 * 2048 // dim))
+        return _case("", "norm", rng.choice(["forward", "train"]), 1, rows, dtype=dtype, dim=dim)
+    if op == "conv":
+        dim = rng.choice([_spread(rng, 64, 4096), 8 * _spread(rng, 8, 512)])
+        s, act = rng.randint(2, 8), rng.choice(["", "silu"])
+        kind = rng.choice(["step", "chunk", "train", "train"])
+        most = max(64, 16384 * 2048 // dim // (2 if s > 4 else 1))
+        if kind == "train" and rng.random() < 0.5:
+            tokens = _spread(rng, 50, min(most, 16384))
+            return _case("", "conv", "train", tokens=tokens, shortest=1,
+                         longest=_spread(rng, 40, 4096), dtype=dtype, dim=dim, s=s, act=act)
+        batch = _spread(rng, 1, 256 if kind == "step" else 8)
+        time = 1 if kind == "step" else _spread(rng, 2, min(8192, max(2, most // batch)))
+        return _case("", "conv", kind, batch, time, dtype=dtype, dim=dim, s=s, act=act)
+    groups = rng.choice([1, 1, 2, 4])
+    heads = groups * rng.choice([1, 2, 4, 5, 8])
+    p, n = rng.choice([16, 32, 40, 64, 64, 80]), rng.choice([16, 24, 64, 100, 128, 128])
+    kind = rng.choice(["step", "forward", "chunk", "train", "train"])
+    if kind == "step":
+        return _case("", "scan", "step", _spread(rng, 1, 256), 1, dtype=dtype, heads=heads, p=p,
+                     n=n, groups=groups)
+    most = min(16384, max(256, 16384 * 32 * 64 * 128 // (heads * p * n)))
+    if kind == "train" and rng.random() < 0.5:
+        return _case("", "scan", "train", tokens=_spread(rng, 80, most // 2), shortest=1,
+                     longest=_spread(rng, 60, 4096), dtype=dtype, heads=heads, p=p, n=n, groups=groups)
+    batch = _spread(rng, 1, 8)
+    time = _spread(rng, 2, max(2, min(4096, most // (2 * batch))))
+    return _case("", "scan", kind, batch, time, dtype=dtype, heads=heads, p=p, n=n, groups=groups)
+
+
+def _lengths(c):
+    """The packed sequences' lengths, the same for every seed."""
+    rng, left, got = random.Random(c["tokens"]), c["tokens"], []
+    while left > 0:
+        got.append(min(left, _spread(rng, max(1, c["shortest"]), max(1, c["longest"]))))
+        left -= got[-1]
+    return got
+
+
+def prepare(case, seed):
+    c = dict(case)
+    dev, dt = torch.device("cuda:0"), _DTYPES[c["dtype"]]
+    g = torch.Generator(device=dev).manual_seed(int(seed))
+
+    def normal(*shape, scale=1.0, mean=0.0):
+        return (torch.randn(*shape, device=dev, generator=g) * scale + mean).to(dt)
+
+    def uniform(*shape, lo=0.0, hi=1.0):
+        return torch.rand(*shape, device=dev, generator=g) * (hi - lo) + lo
+
+    st = {"case": c, "cu": None, "max_seqlen": None, "cache": None}
+    lead = (c["batch"], c["time"])
+    if c["tokens"]:
+        lens = _lengths(c)
+        lead = (c["tokens"],)
+        st["cu"] = torch.tensor([0] + lens, device=dev).cumsum(0).to(torch.int32)
+        st["max_seqlen"] = max(lens)
+    train = c["kind"] == "train"
+    if c["op"] == "norm":
+        st["inputs"] = [normal(*lead, c["dim"], scale=1.5, mean=0.3), normal(c["dim"], scale=0.1, mean=1.0),
+                        normal(c["dim"], scale=0.1)]
+    elif c["op"] == "conv":
+        bound = 1.0 / math.sqrt(c["s"])
+        st["inputs"] = [normal(*lead, c["dim"]), uniform(c["s"], c["dim"], lo=-bound, hi=bound).to(dt),
+                        uniform(c["dim"], lo=-bound, hi=bound).to(dt)]
+        if c["kind"] in ("step", "chunk"):
+            st["cache"] = normal(c["batch"], c["dim"], c["s"])
+    else:
+        H, P, N, G = c["heads"], c["p"], c["n"], c["groups"]
+        # step lengths from 0.001 to 0.1 before the token's own part, decay rates 1 to 16
+        u = torch.exp(uniform(H, lo=math.log(1e-3), hi=math.log(0.1)))
+        st["inputs"] = [normal(*lead, H, P), normal(*lead, H, scale=0.5), (-uniform(H, lo=1.0, hi=16.0)).to(dt),
+                        normal(*lead, G, N), normal(*lead, G, N), uniform(H, lo=0.5, hi=1.5).to(dt),
+                        (u + torch.log(-torch.expm1(-u))).to(dt)]
+        if c["kind"] in ("step", "chunk"):
+            st["cache"] = torch.randn(c["batch"], H, P, N, device=dev, generator=g) * 0.3
+    if train:
+        st["dy"] = normal(*st["inputs"][0].shape)
+        for t in st["inputs"]:
+            t.requires_grad_()
+    return st
+
+
+def _activate(v, act):
+    return v * torch.sigmoid(v) if act == "silu" else v
+
+
+def _sequence_of(st):
+    """The sequence that each token of the flat token axis belongs to."""
+    x, c = st["inputs"][0], st["case"]
+    if st["cu"] is None:
+        return torch.arange(c["batch"], device=x.device).repeat_interleave(c["time"])
+    at = torch.arange(c["tokens"], device=x.device)
+    return (at[:, None] >= st["cu"][None, 1:]).sum(1)
+
+
+# ---------------------------------------------------------------------------
+# the plain forms
+
+def _plain_norm(st):
+    x, w, b = [t.float() for t in st["inputs"]]
+    d = x - x.mean(-1, keepdim=True)
+    y = d * torch.rsqrt((d * d).mean(-1, keepdim=True) + 1e-5) * w + b
+    return y.to(st["inputs"][0].dtype)
+
+
+def _plain_conv(st):
+    """(y, final state or None)."""
+    x0, (x, w, b), c = st["inputs"][0], [t.float() for t in st["inputs"]], st["case"]
+    S, D = w.shape
+    cache = st["cache"]
+    if c["kind"] == "step":
+        window = torch.cat((cache[:, :, 1:], x0.transpose(1, 2)), 2)
+        y = _activate((window.float() * w.t()).sum(-1) + b, c["act"])
+        cache.copy_(window)
+        return y[:, None].to(x0.dtype), cache
+    if c["kind"] == "chunk":
+        every = torch.cat((cache, x0.transpose(1, 2)), 2)  # [B, D, S + T]
+        y = (every[:, :, 1:].float().unfold(2, S, 1) * w.t()[None, :, None]).sum(-1)
+        y = _activate(y + b[:, None], c["act"]).transpose(1, 2)
+        return y.to(x0.dtype).contiguous(), every[:, :, -S:].contiguous()
+    flat = torch.cat((x.new_zeros(S - 1, D), x.reshape(-1, D)), 0)
+    seq = _sequence_of(st)
+    before = torch.cat((seq.new_full((S - 1,), -1), seq), 0).unfold(0, S, 1)  # [N, S]
+    window = flat.unfold(0, S, 1) * (before == seq[:, None])[:, None].float()  # [N, D, S]
+    y = _activate((window * w.t()).sum(-1) + b, c["act"])
+    return y.to(x0.dtype).reshape(x0.shape), None
+
+
+def _softplus(v):
+    return torch.clamp(v, min=0) + torch.log1p(torch.exp(-torch.abs(v)))
+
+
+def _plain_scan(st):
+    """(y, final state or None)."""
+    c, x0 = st["case"], st["inputs"][0]
+    x, dt, A, B, C, D, bias = [t.float() for t in st["inputs"]]
+    H, P, N, G = c["heads"], c["p"], c["n"], c["groups"]
+    cache = st["cache"]
+    u = _softplus(dt + bias)
+    if c["kind"] == "step":
+        Bh, Ch = (t[:, 0].repeat_interleave(H // G, 1)[:, :, None] for t in (B, C))
+        x1, u1 = x[:, 0, :, :, None], u[:, 0, :, None, None]
+        h = torch.exp(u1 * A[:, None, None]) * cache + u1 * x1 * Bh
+        cache.copy_(h)
+        y = (h * Ch).sum(-1) + D[:, None] * x[:, 0]
+        return y[:, None].to(x0.dtype), cache
+    n_tok = x.numel() // (H * P)
+    pad = -n_tok % _Q
+
+    def chunks(t, width):  # [chunks, Q, ...]
+        t = t.reshape(n_tok, *width)
+        return torch.cat((t, t.new_zeros(pad, *width)), 0).reshape(-1, _Q, *width)
+
+    seq = _sequence_of(st)
+    sq = torch.cat((seq, seq.new_full((pad,), -1)), 0).reshape(-1, _Q)
+    uc, xc = chunks(u, (H,)), chunks(x, (H, P)).transpose(1, 2)  # xc [chunks, H, Q, P]
+    Bc, Cc = (chunks(t, (G, N)).repeat_interleave(H // G, 2).transpose(1, 2) for t in (B, C))
+    cs = (uc.double() * A.double()).cumsum(1).transpose(1, 2)  # [chunks, H, Q], in 64 bits
+    uh = uc.transpose(1, 2)
+    at = torch.arange(_Q, device=x.device)
+    same = (sq[:, :, None] == sq[:, None]) & (at[:, None] >= at[None])  # [chunks, i, j]
+    gap = (cs[..., :, None] - cs[..., None, :]).masked_fill(~same[:, None], -math.inf)
+    weights = torch.matmul(Cc, Bc.transpose(2, 3)) * torch.exp(gap.float()) * uh[:, :, None]
+    y = torch.matmul(weights, xc)
+    # the state that each chunk's last sequence leaves, and what reaches a later chunk of it
+    to_end = torch.exp((cs[..., -1:] - cs).masked_fill((sq != sq[:, -1:])[:, None], -math.inf).float())
+    left = torch.matmul((xc * (uh * to_end)[..., None]).transpose(2, 3), Bc)  # [chunks, H, P, N]
+    total = cs[..., -1].t().cumsum(1)  # [H, chunks]
+    before = total - cs[..., -1].t()
+    k = torch.arange(sq.shape[0], device=x.device)
+    reach = (k[:, None] > k[None]) & (sq[:, 0][:, None] == sq[:, -1][None])
+    carry = torch.exp((before[:, :, None] - total[:, None]).masked_fill(~reach, -math.inf).float())
+    entering = torch.matmul(carry, left.transpose(0, 1).reshape(H, -1, P * N)).reshape(H, -1, P, N).transpose(0, 1)
+    from_start = torch.exp(cs.masked_fill((sq != sq[:, :1])[:, None], -math.inf).float())
+    y = y + from_start[..., None] * torch.matmul(Cc, entering.transpose(2, 3))
+    y = y.transpose(1, 2).reshape(-1, H, P)[:n_tok].reshape(x.shape) + D[:, None] * x
+    if c["kind"] == "train":
+        return y.to(x0.dtype), None
+    cs = (u.double() * A.double()).cumsum(1)  # [B, T, H]
+    Bh, Ch = (t.repeat_interleave(H // G, 2).transpose(1, 2) for t in (B, C))
+    last = (u * torch.exp((cs[:, -1:] - cs).float()))[..., None] * x  # [B, T, H, P]
+    state = torch.matmul(last.permute(0, 2, 3, 1), Bh)
+    if cache is not None:
+        decay = torch.exp(cs.float())
+        y = y + decay[..., None] * torch.matmul(Ch, cache.transpose(2, 3)).transpose(1, 2)
+        state = state + decay[:, -1, :, None, None] * cache
+    return y.to(x0.dtype), state
+
+
+# ---------------------------------------------------------------------------
+
+def _own(st):
+    """(y, final state or None) by the framework's operators."""
+    moc, c, ins = _moc(), st["case"], st["inputs"]
+    if c["op"] == "norm":
+        return moc.layer_norm(*ins, eps=1e-5), None
+    more = {"cu_seqlens": st["cu"], "max_seqlen": st["max_seqlen"], "cache": st["cache"],
+            "output_final_state": c["kind"] != "train"}
+    if c["op"] == "conv":
+        return moc.causal_conv(*ins, activation=c["act"] or None, **more)
+    return moc.selective_scan(*ins, **more)
+
+
+def run(state):
+    c = state["case"]
+    if own:
+        y, final = _own(state)
+    elif c["op"] == "norm":
+        y, final = _plain_norm(state), None
+    else:
+        y, final = (_plain_conv if c["op"] == "conv" else _plain_scan)(state)
+    if c["kind"] == "train":
+        return (y.detach(), *torch.autograd.grad(y, state["inputs"], state["dy"]))
+    return y if final is None else (y, final)
+
+
+def work(case):
+    c = case
+    e = 2 if c["dtype"] == "bf16" else 4
+    tok = c["tokens"] or c["batch"] * c["time"]
+    train = c["kind"] == "train"
+    if c["op"] == "norm":
+        return {"bytes": tok * c["dim"] * e * (4 if train else 2) + c["dim"] * e * (4 if train else 2),
+                "flops": tok * c["dim"] * (20 if train else 8)}
+    states = {"step": 2, "chunk": 2, "forward": 1, "train": 0}[c["kind"]]
+    if c["op"] == "conv":
+        return {"bytes": tok * c["dim"] * e * (4 if train else 2) + states * c["batch"] * c["dim"] * c["s"] * e
+                + (c["s"] + 1) * c["dim"] * e * (2 if train else 1),
+                "flops": tok * c["dim"] * c["s"] * (8 if train else 2)}
+    H, P, N, G = c["heads"], c["p"], c["n"], c["groups"]
+    per = 2 * H * P + 2 * G * N + H  # x, y, B, C, dt; the same again for gradients
+    return {"bytes": tok * per * e * (2 if train else 1) + states * c["batch"] * H * P * N * 4,
+            "flops": tok * H * P * N * (17 if train else 5)}
+
+
+# ---------------------------------------------------------------------------
+# the definitions in 64 bits, one token after the other
+
+def _rows(st, t):
+    """t as [sequences, longest, ...], padded with zeros, and the way back."""
+    if st["cu"] is None:
+        return t, lambda v: v
+    cu = st["cu"].tolist()
+    spans = list(zip(cu[:-1], cu[1:]))
+    out = t.new_zeros(len(spans), st["max_seqlen"], *t.shape[1:])
+    for i, (a, b) in enumerate(spans):
+        out[i, :b - a] = t[a:b]
+    return out, lambda v: torch.cat([v[i, :b - a] for i, (a, b) in enumerate(spans)], 0)
+
+
+def _exact_norm(st):
+    x, w, b = [t.detach().double() for t in st["inputs"]]
+    mean = x.mean(-1, keepdim=True)
+    rstd = 1.0 / torch.sqrt(((x - mean) ** 2).mean(-1, keepdim=True) + 1e-5)
+    xh = (x - mean) * rstd
+    y = xh * w + b
+    if st["case"]["kind"] != "train":
+        return y
+    dy = st["dy"].double()
+    g = dy * w
+    dx = rstd * (g - g.mean(-1, keepdim=True) - xh * (g * xh).mean(-1, keepdim=True))
+    lead = tuple(range(x.dim() - 1))
+    return y, dx, (dy * xh).sum(lead), dy.sum(lead)
+
+
+def _exact_conv(st):
+    c = st["case"]
+    x, w, b = [t.detach().double() for t in st["inputs"]]
+    S = c["s"]
+    if st["cache"] is not None:
+        every = torch.cat((st["cache"].double().transpose(1, 2), x), 1)  # [B, S + T, D]
+        T = x.shape[1]
+        p = b + sum(w[s] * every[:, s + 1:s + 1 + T] for s in range(S))
+        y = p / (1 + torch.exp(-p)) if c["act"] else p
+        return y, every[:, -S:].transpose(1, 2)
+    x, back = _rows(st, x)
+    T = x.shape[1]
+    p = b.expand_as(x).clone()
+    for s in range(S):
+        k = S - 1 - s
+        p[:, k:] += w[s] * x[:, :T - k]
+    sg = 1 / (1 + torch.exp(-p))
+    y = p * sg if c["act"] else p
+    g, _ = _rows(st, st["dy"].double())
+    g = g * (sg * (1 + p * (1 - sg))) if c["act"] else g
+    dx, dw = torch.zeros_like(x), torch.zeros_like(w)
+    for s in range(S):
+        k = S - 1 - s
+        dx[:, :T - k] += w[s] * g[:, k:]
+        dw[s] = (g[:, k:] * x[:, :T - k]).sum((0, 1))
+    return back(y), back(dx), dw, g.sum((0, 1))
+
+
+def _exact_scan_rows(c, x, dt, A, B, C, D, bias, h, dy):
+    """Sequences of one length, [n, T, ...]: (y, final state), or with dy (y, gradients of the seven inputs)."""
+    H, G, T = c["heads"], c["groups"], x.shape[1]
+    Bh, Ch = (t.repeat_interleave(H // G, 2) for t in (B, C))
+    raw = dt + bias
+    u = torch.log1p(torch.exp(-raw.abs())) + raw.clamp(min=0)
+    a = torch.exp(u * A)
+    ux = u[..., None] * x
+    kept, ys = [h], []
+    for t in range(T):
+        h = a[:, t, :, None, None] * h + ux[:, t, :, :, None] * Bh[:, t, :, None]
+        ys.append((h * Ch[:, t, :, None]).sum(-1))
+        if dy is not None:
+            kept.append(h)
+    y = torch.stack(ys, 1) + D[:, None] * x
+    if dy is None:
+        return y, h
+    dx, du, da = D[:, None] * dy, torch.zeros_like(u), torch.zeros_like(u)
+    dB, dC, dh = [None] * T, [None] * T, torch.zeros_like(h)
+    for t in range(T - 1, -1, -1):
+        dh = dh + dy[:, t, :, :, None] * Ch[:, t, :, None]
+        dC[t] = (dy[:, t, :, :, None] * kept.pop()).sum(2)
+        dB[t] = (ux[:, t, :, :, None] * dh).sum(2)
+        hb = (dh * Bh[:, t, :, None]).sum(-1)
+        dx[:, t] += u[:, t, :, None] * hb
+        du[:, t] = (x[:, t] * hb).sum(-1)
+        dh = dh * a[:, t, :, None, None]
+        da[:, t] = (dh * kept[-1]).sum((-1, -2))
+    draw_ = (du + A * da) / (1 + torch.exp(-raw))
+    dB, dC = (torch.stack(t, 1).unflatten(2, (G, H // G)).sum(3) for t in (dB, dC))
+    return y, dx, draw_, (u * da).sum((0, 1)), dB, dC, (dy * x).sum((0, 1, 3)), draw_.sum((0, 1))
+
+
+def _exact_scan(st):
+    c = st["case"]
+    x, dt, A, B, C, D, bias = [t.detach().double() for t in st["inputs"]]
+    dy = st["dy"].double() if c["kind"] == "train" else None
+    n = x.shape[0] if st["cu"] is None else 1
+    h = x.new_zeros(n, c["heads"], c["p"], c["n"]) if st["cache"] is None else st["cache"].double()
+    if st["cu"] is None:
+        return _exact_scan_rows(c, x, dt, A, B, C, D, bias, h, dy)
+    cu = st["cu"].tolist()
+    got = [_exact_scan_rows(c, *(t[None, i:j] if t.dim() > 1 else t for t in (x, dt, A, B, C, D, bias)), h,
+                            dy[None, i:j]) for i, j in zip(cu[:-1], cu[1:])]
+    summed = (3, 6, 7)  # A, D and dt_bias belong to every sequence
+    return tuple(sum(g[k] for g in got) if k in summed else torch.cat([g[k][0] for g in got], 0) for k in range(8))
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    with torch.no_grad():
+        return {"norm": _exact_norm, "conv": _exact_conv, "scan": _exact_scan}[case["op"]](st)
