@@ -397,6 +397,124 @@ int moc_router_f32_backward(const void* z, const void* router, const void* dlogi
  */
 int moc_profile_events(void* start_event, void* stop_event);
 
+/*
+ * Operators that stand next to the MoC layers in a block.  They have no counterpart
+ * in the reference; conventions (pointers, streams, workspaces, errors, sequences) are
+ * those above.
+ */
+
+/*
+ * Layer norm over the last axis of x [rows, dim] (bf16 or f32):
+ *   mean = sum x / dim, rstd = 1 / sqrt(sum (x - mean)^2 / dim + eps),
+ *   y = (x - mean) rstd weight + bias.
+ * weight, bias [dim] in any dtype, or NULL (1 and 0).  mean, rstd [rows] f32: what the
+ * backward reads; both NULL: not kept.
+ */
+int moc_norm_forward(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                     int64_t rows, int64_t dim, int x_dtype, int weight_dtype, int bias_dtype, float eps,
+                     void* stream);
+
+/* Workspace bytes of moc_norm_backward with dweight or dbias (0 without them). */
+size_t moc_norm_backward_workspace_bytes(int64_t rows, int64_t dim);
+
+/* dx in the x dtype, dweight and dbias in their tensors' dtypes, summed over the rows in
+ * a fixed order; each may be NULL. */
+int moc_norm_backward(const void* x, const void* weight, const void* dy, const float* mean, const float* rstd,
+                      void* dx, void* dweight, void* dbias, int64_t rows, int64_t dim, int x_dtype, int weight_dtype,
+                      int bias_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Causal convolution with one kernel per channel for every token:
+ *   P[n,d] = bias[d] + sum_s weight[s,d] x[n-(S-1-s), d], y = silu(P) or P
+ * weight [kernel_size, dim], 1 <= kernel_size <= 16, bias [dim] or NULL, any dtypes.
+ * Fixed length only: cache [n_seqs, dim, kernel_size] in the x dtype (newest slot last) or
+ * NULL (zeros before a sequence), final_state the same or NULL: the last kernel_size
+ * inputs.  Tokens outside every [cu_seqlens[j], cu_seqlens[j+1]) start their own history.
+ */
+int moc_conv_forward(const void* x, const void* weight, const void* bias, const void* cache, void* y,
+                     void* final_state, const void* cu_seqlens, int cu_seqlens_i64, int64_t n_seqs, int64_t n_tokens,
+                     int64_t seq_len, int64_t dim, int64_t kernel_size, int x_dtype, int weight_dtype, int bias_dtype,
+                     int activation, void* stream);
+
+/* Workspace bytes of moc_conv_backward with dweight or dbias. */
+size_t moc_conv_backward_workspace_bytes(int64_t n_tokens, int64_t dim, int64_t kernel_size);
+
+/* Gradients of moc_conv_forward without a cache for dy [n_tokens, dim]; dx, dweight,
+ * dbias may each be NULL.  Sums over tokens are formed in a fixed order. */
+int moc_conv_backward(const void* x, const void* weight, const void* bias, const void* dy, void* dx, void* dweight,
+                      void* dbias, const void* cu_seqlens, int cu_seqlens_i64, int64_t n_seqs, int64_t n_tokens,
+                      int64_t seq_len, int64_t dim, int64_t kernel_size, int x_dtype, int weight_dtype,
+                      int bias_dtype, int activation, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token per sequence, in place on the cache (element strides; no two slots may
+ * share memory): the slots move down by one, the last takes x, y is formed from them. */
+int moc_conv_update(const void* x, const void* weight, const void* bias, void* cache, int64_t cache_stride_b,
+                    int64_t cache_stride_d, int64_t cache_stride_s, void* y, int64_t batch, int64_t dim,
+                    int64_t kernel_size, int x_dtype, int weight_dtype, int bias_dtype, int activation, void* stream);
+
+/*
+ * Selective scan: per head of head_dim channels with a [head_dim, state_dim] state h,
+ *   u = softplus(dt + dt_bias) (or dt + dt_bias), h_t = exp(u_t a) h_{t-1} + u_t x_t (x) b_t,
+ *   y_t = h_t c_t + d x_t.
+ * x [n_tokens, heads, head_dim], dt [n_tokens, heads], b and c [n_tokens, groups,
+ * state_dim] in x_dtype (bf16 or f32), tokens *_stride elements apart, a token's own
+ * values contiguous; heads h of group h / (heads / groups) share b and c.  a, d (or NULL),
+ * dt_bias (or NULL) [heads] in any dtype.  head_dim <= 128, state_dim <= 256.  States
+ * [n_seqs, heads, head_dim, state_dim] f32, fixed length only.
+ */
+typedef struct MocScan {
+  const void* x;
+  const void* dt;
+  const void* a;
+  const void* b;
+  const void* c;
+  const void* d;
+  const void* dt_bias;
+  int64_t x_stride, dt_stride, b_stride, c_stride;
+  const void* cu_seqlens; /* as for moc_forward */
+  int64_t n_seqs, n_tokens, seq_len;
+  int64_t heads, head_dim, groups, state_dim;
+  int cu_seqlens_i64;
+  int x_dtype, a_dtype, d_dtype, bias_dtype;
+  int dt_softplus;
+} MocScan;
+
+/* Gradients, contiguous, in their tensors' dtypes (dinitial_state: f32); dd, ddt_bias,
+ * dinitial_state may be NULL. */
+typedef struct MocScanGrads {
+  void* dx;
+  void* ddt;
+  void* da;
+  void* db;
+  void* dc;
+  void* dd;
+  void* ddt_bias;
+  float* dinitial_state;
+} MocScanGrads;
+
+/* Bytes of `saved` (0: the problem is not one the entry takes). */
+size_t moc_scan_saved_bytes(const MocScan* scan);
+
+/* Workspace bytes of moc_scan_forward with or without `saved`. */
+size_t moc_scan_forward_workspace_bytes(const MocScan* scan, int with_saved);
+
+/* y [n_tokens, heads, head_dim] in the x dtype.  initial_state, final_state may be NULL;
+ * they may not be the same tensor.  saved: what moc_scan_backward reads, or NULL. */
+int moc_scan_forward(const MocScan* scan, void* y, const float* initial_state, float* final_state, void* saved,
+                     size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t moc_scan_backward_workspace_bytes(const MocScan* scan);
+
+/* Gradients for dy (contiguous, x dtype) and dfinal_state (or NULL) on the inputs and the
+ * `saved` of moc_scan_forward; has_initial_state: whether that call had one.  Sums over
+ * tokens and heads are formed in a fixed order. */
+int moc_scan_backward(const MocScan* scan, const void* dy, int has_initial_state, const float* dfinal_state,
+                      const void* saved, size_t saved_bytes, const MocScanGrads* grads, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* One token per sequence (seq_len 1), in place on the contiguous state. */
+int moc_scan_update(const MocScan* scan, float* state, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -172,6 +172,20 @@ int hip_status(const char* what) {
 
 }  // namespace
 
+namespace moc {
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+void clear_error() { g_err[0] = '\0'; }
+
+}  // namespace moc
+
 extern "C" {
 
 int moc_abi_version(void) { return 5; }

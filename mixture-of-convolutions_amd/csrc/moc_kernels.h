@@ -185,4 +185,62 @@ void router_f32_forward(const void* z, const void* r, void* out, int64_t N, int6
 void router_f32_backward(const void* z, const void* r, const void* dl, void* dz, void* dr,
                          int64_t N, int64_t Z, int64_t K, void* workspace, hipStream_t st);
 
+// layer norm over rows of D (moc_norm.hip): x, y in dt; w, b in any dtype or null;
+// mean / rstd [rows] fp32 (null: not kept)
+size_t norm_backward_workspace(int64_t rows, int64_t D);
+void norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows,
+                  int64_t D, int dt, int w_dt, int b_dt, float eps, hipStream_t st);
+// dx, dw, db (each may be null), dw in w_dt and db in b_dt
+void norm_backward(const void* x, const void* w, const void* dy, const float* mean, const float* rstd, void* dx,
+                   void* dw, void* db, int64_t rows, int64_t D, int dt, int w_dt, int b_dt, void* workspace,
+                   hipStream_t st);
+
+// causal convolution with one kernel per channel (moc_conv.hip), 1 <= S <= 16
+constexpr int kConvMaxS = 16;
+struct Conv {
+  SeqLayout seq;
+  int64_t D, S;
+  int x_dt, w_dt, b_dt;
+  int activation;
+};
+size_t conv_backward_workspace(const Conv& p);
+// cache / fin [n_seqs, D, S] in the x dtype or null (fixed length only)
+void conv_forward(const Conv& p, const void* x, const void* w, const void* bias, const void* cache, void* y, void* fin,
+                  hipStream_t st);
+// dx, dw, dbias may each be null
+void conv_backward(const Conv& p, const void* x, const void* w, const void* bias, const void* dy, void* dx, void* dw,
+                   void* dbias, void* workspace, hipStream_t st);
+void conv_update(const void* x, const void* w, const void* bias, void* cache, int64_t cb, int64_t cd, int64_t cs,
+                 void* y, int64_t B, int64_t D, int64_t S, int x_dt, int w_dt, int b_dt, int act, hipStream_t st);
+
+// selective scan (moc_scan.hip, moc_scan_bwd.hip): P <= 128, N <= 256
+constexpr int kScanMaxP = 128, kScanMaxN = 256;
+struct Scan {
+  SeqLayout seq;
+  int64_t H, P, G, N;
+  const void *x, *dt, *A, *B, *C, *D, *bias;  // D, bias may be null
+  int64_t x_stride, dt_stride, b_stride, c_stride;  // elements between tokens
+  int x_dt, a_dt, d_dt, bias_dt;  // x, dt, B, C have x_dt
+  int softplus;
+};
+size_t scan_saved_bytes(const Scan& p);
+size_t scan_forward_workspace(const Scan& p, bool saved);
+// init / final [n_seqs, H, P, N] fp32 or null (fixed length only); saved: what the
+// backward reads, or null
+void scan_forward(const Scan& p, void* y, const float* init, float* fin, void* saved, void* workspace, hipStream_t st);
+struct ScanGrads {
+  void *dx, *ddt, *dA, *dB, *dC, *dD, *dbias;  // contiguous; dD, dbias may be null
+  float* dinit;                                // or null
+};
+size_t scan_backward_workspace(const Scan& p);
+// has_init: the forward had an initial state; dfin: gradient of the final state or null
+void scan_backward(const Scan& p, const void* dy, bool has_init, const float* dfin, const void* saved,
+                   const ScanGrads& g, void* workspace, hipStream_t st);
+// one token per sequence, in place on the state [n_seqs, H, P, N]
+void scan_update(const Scan& p, float* state, void* y, int64_t n_seqs, hipStream_t st);
+
+// error text of this thread's failed call (moc_capi.hip); returns code
+int fail(int code, const char* fmt, ...);
+void clear_error();
+
 }  // namespace moc

@@ -57,9 +57,17 @@ EXPORTED_SYMBOLS = (
     "moc_router_f32_supported", "moc_router_f32_forward",
     "moc_router_f32_backward_workspace_bytes", "moc_router_f32_backward",
     "moc_router_backward",
+    "moc_norm_forward", "moc_norm_backward_workspace_bytes", "moc_norm_backward",
+    "moc_conv_forward", "moc_conv_backward_workspace_bytes", "moc_conv_backward",
+    "moc_conv_update",
+    "moc_scan_saved_bytes", "moc_scan_forward_workspace_bytes", "moc_scan_forward",
+    "moc_scan_backward_workspace_bytes", "moc_scan_backward", "moc_scan_update",
 )
 
 MAX_LAYERS = 4
+# largest sizes of the causal convolution and the selective scan
+CONV_MAX_KERNEL = 16
+SCAN_MAX_HEAD_DIM, SCAN_MAX_STATE_DIM = 128, 256
 
 
 class MocLayer(ctypes.Structure):
@@ -71,6 +79,23 @@ class MocLayer(ctypes.Structure):
         ("dim", ctypes.c_int64), ("routing", ctypes.c_int), ("alpha_dtype", ctypes.c_int),
         ("basis_dtype", ctypes.c_int), ("activation", ctypes.c_int), ("k", ctypes.c_int64),
     ]
+
+
+class MocScan(ctypes.Structure):
+    """struct MocScan of include/moc_hip.h: a selective scan's inputs."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "dt", "a", "b", "c", "d", "dt_bias")]
+                + [(n, ctypes.c_int64) for n in ("x_stride", "dt_stride", "b_stride", "c_stride")]
+                + [("cu_seqlens", ctypes.c_void_p)]
+                + [(n, ctypes.c_int64) for n in ("n_seqs", "n_tokens", "seq_len", "heads",
+                                                 "head_dim", "groups", "state_dim")]
+                + [(n, ctypes.c_int) for n in ("cu_seqlens_i64", "x_dtype", "a_dtype", "d_dtype",
+                                               "bias_dtype", "dt_softplus")])
+
+
+class MocScanGrads(ctypes.Structure):
+    """struct MocScanGrads of include/moc_hip.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dx", "ddt", "da", "db", "dc", "dd", "ddt_bias",
+                                               "dinitial_state")]
 
 
 _lock = threading.Lock()
@@ -185,6 +210,28 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.moc_router_f32_backward_workspace_bytes.restype = _z
     lib.moc_router_f32_backward.argtypes = [_p, _p, _p, _p, _p, _l, _l, _l, _p, _z, _p]
     lib.moc_router_f32_backward.restype = _i
+    lib.moc_norm_forward.argtypes = [_p, _p, _p, _p, _p, _p, _l, _l, _i, _i, _i, ctypes.c_float, _p]
+    lib.moc_norm_backward_workspace_bytes.argtypes = [_l, _l]
+    lib.moc_norm_backward_workspace_bytes.restype = _z
+    lib.moc_norm_backward.argtypes = [_p] * 8 + [_l, _l, _i, _i, _i, _p, _z, _p]
+    seq = [_p, _i, _l, _l, _l]         # cu_seqlens, cu_seqlens_i64, n_seqs, n_tokens, seq_len
+    conv = [_l, _l, _i, _i, _i, _i]    # dim, kernel_size, dtypes, activation
+    lib.moc_conv_forward.argtypes = [_p] * 6 + seq + conv + [_p]
+    lib.moc_conv_backward_workspace_bytes.argtypes = [_l, _l, _l]
+    lib.moc_conv_backward_workspace_bytes.restype = _z
+    lib.moc_conv_backward.argtypes = [_p] * 7 + seq + conv + [_p, _z, _p]
+    lib.moc_conv_update.argtypes = [_p, _p, _p, _p, _l, _l, _l, _p, _l] + conv + [_p]
+    for name in ("moc_scan_saved_bytes", "moc_scan_backward_workspace_bytes"):
+        getattr(lib, name).argtypes = [_p]
+        getattr(lib, name).restype = _z
+    lib.moc_scan_forward_workspace_bytes.argtypes = [_p, _i]
+    lib.moc_scan_forward_workspace_bytes.restype = _z
+    lib.moc_scan_forward.argtypes = [_p, _p, _p, _p, _p, _z, _p, _z, _p]
+    lib.moc_scan_backward.argtypes = [_p, _p, _i, _p, _p, _z, _p, _p, _z, _p]
+    lib.moc_scan_update.argtypes = [_p, _p, _p, _p]
+    for name in ("moc_norm_forward", "moc_norm_backward", "moc_conv_forward", "moc_conv_backward",
+                 "moc_conv_update", "moc_scan_forward", "moc_scan_backward", "moc_scan_update"):
+        getattr(lib, name).restype = _i
 
 
 def lib() -> ctypes.CDLL:

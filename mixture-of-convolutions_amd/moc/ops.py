@@ -12,6 +12,8 @@ boundaries from ``cu_seqlens`` directly and do not need them.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 import torch.nn.functional as F
 
@@ -656,3 +658,213 @@ def launch_decode_step(x: torch.Tensor, z: torch.Tensor, router: torch.Tensor,
                                int(activation_flag), int(routing), _lib.stream_ptr(x.device))
     _lib.check(rc, "moc_decode_step")
     return out
+
+
+# ---------------------------------------------------------------------------
+# the operators of moc/blocks.py
+
+def _param(t: torch.Tensor | None):
+    """(pointer or None, dtype code) of a contiguous parameter or None."""
+    return (None, 0) if t is None else (t.data_ptr(), _lib.dtype_code(t.dtype))
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def launch_norm_forward(x, weight, bias, eps: float, keep: bool):
+    """(y, mean, rstd) of layer norm over the last axis of a contiguous x; mean and
+    rstd are None unless ``keep``."""
+    D = x.shape[-1]
+    rows = x.numel() // D
+    y = torch.empty_like(x)
+    mean = rstd = None
+    if keep:
+        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device).unbind(0)
+    (wp, wd), (bp, bd) = _param(weight), _param(bias)
+    with _lib.device_guard(x.device):
+        rc = _lib.lib().moc_norm_forward(x.data_ptr(), wp, bp, y.data_ptr(), _ptr(mean), _ptr(rstd),
+                                         rows, D, _lib.dtype_code(x.dtype), wd, bd, eps,
+                                         _lib.stream_ptr(x.device))
+    _lib.check(rc, "moc_norm_forward")
+    return y, mean, rstd
+
+
+def launch_norm_backward(x, weight, bias, dy, mean, rstd, need_x, need_w, need_b):
+    """(dx, dweight, dbias), each None where not needed."""
+    L = _lib.lib()
+    D = x.shape[-1]
+    rows = x.numel() // D
+    dy = dy.to(x.dtype).contiguous()
+    dx = torch.empty_like(x) if need_x else None
+    dw = torch.empty_like(weight) if need_w else None
+    db = torch.empty_like(bias) if need_b else None
+    (wp, wd), (_, bd) = _param(weight), _param(bias)
+    with _lib.device_guard(x.device):
+        n = L.moc_norm_backward_workspace_bytes(rows, D) if need_w or need_b else 0
+        ws = _workspace(n, x.device)
+        rc = L.moc_norm_backward(x.data_ptr(), wp, dy.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                 _ptr(dx), _ptr(dw), _ptr(db), rows, D, _lib.dtype_code(x.dtype),
+                                 wd, bd, ws.data_ptr(), ws.numel(), _lib.stream_ptr(x.device))
+    _lib.check(rc, "moc_norm_backward")
+    return dx, dw, db
+
+
+def launch_conv_forward(x, weight, bias, cache, *, activation_flag: int, cu_seqlens=None,
+                        final_state: bool = False):
+    """(y, final state or None) of the causal convolution of a contiguous [B, T, D] x
+    (continuing from ``cache`` [B, D, S], or from zeros) or a packed [N, D] x."""
+    S, D = weight.shape
+    cu_ptr, cu64, n_seqs, n_tokens, seq_len, _ = _seq_args(x, cu_seqlens)
+    y = torch.empty_like(x)
+    fin = x.new_empty(x.shape[0], D, S) if final_state else None
+    (wp, wd), (bp, bd) = _param(weight), _param(bias)
+    with _lib.device_guard(x.device):
+        rc = _lib.lib().moc_conv_forward(
+            x.data_ptr(), wp, bp, _ptr(cache), y.data_ptr(), _ptr(fin), cu_ptr, cu64, n_seqs,
+            n_tokens, seq_len, D, S, _lib.dtype_code(x.dtype), wd, bd, int(activation_flag),
+            _lib.stream_ptr(x.device))
+    _lib.check(rc, "moc_conv_forward")
+    return y, fin
+
+
+def launch_conv_backward(x, weight, bias, dy, *, activation_flag: int, need_x, need_w, need_b,
+                         cu_seqlens=None):
+    """(dx, dweight, dbias) of launch_conv_forward without a cache, each None where
+    not needed."""
+    L = _lib.lib()
+    S, D = weight.shape
+    cu_ptr, cu64, n_seqs, n_tokens, seq_len, _ = _seq_args(x, cu_seqlens)
+    dy = dy.to(x.dtype).contiguous()
+    dx = torch.empty_like(x) if need_x else None
+    dw = torch.empty_like(weight) if need_w else None
+    db = torch.empty_like(bias) if need_b else None
+    (wp, wd), (bp, bd) = _param(weight), _param(bias)
+    with _lib.device_guard(x.device):
+        n = L.moc_conv_backward_workspace_bytes(n_tokens, D, S) if need_w or need_b else 0
+        ws = _workspace(n, x.device)
+        rc = L.moc_conv_backward(
+            x.data_ptr(), wp, bp, dy.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), cu_ptr, cu64, n_seqs,
+            n_tokens, seq_len, D, S, _lib.dtype_code(x.dtype), wd, bd, int(activation_flag),
+            ws.data_ptr(), ws.numel(), _lib.stream_ptr(x.device))
+    _lib.check(rc, "moc_conv_backward")
+    return dx, dw, db
+
+
+def launch_conv_update(x, weight, bias, cache, *, activation_flag: int) -> torch.Tensor:
+    """One token per sequence (x [B, D], contiguous), in place on ``cache``
+    [B, D, S] (any strides)."""
+    S, D = weight.shape
+    y = torch.empty_like(x)
+    (wp, wd), (bp, bd) = _param(weight), _param(bias)
+    with _lib.device_guard(x.device):
+        rc = _lib.lib().moc_conv_update(
+            x.data_ptr(), wp, bp, cache.data_ptr(), *cache.stride(), y.data_ptr(), x.shape[0], D, S,
+            _lib.dtype_code(x.dtype), wd, bd, int(activation_flag), _lib.stream_ptr(x.device))
+    _lib.check(rc, "moc_conv_update")
+    return y
+
+
+def token_rows(t: torch.Tensor, inner: int) -> tuple[torch.Tensor, int]:
+    """(tensor, elements between tokens) of a tensor whose last ``inner`` dimensions
+    are a token's values and whose leading ones ([B, T] or [N]) are tokens: as it
+    is where a token's values are contiguous and tokens evenly apart (a slice of a
+    wider projection), a contiguous copy otherwise."""
+    lead, n = t.shape[:t.ndim - inner], 1
+    dense = True
+    for size, stride in zip(reversed(t.shape[t.ndim - inner:]),
+                            reversed(t.stride()[t.ndim - inner:])):
+        dense = dense and (size == 1 or stride == n)
+        n *= size
+    strides = [st for size, st in zip(lead, t.stride()) if size > 1]
+    if dense and len(strides) == 2:
+        dense = strides[0] == lead[1] * strides[1]
+    step = strides[-1] if strides else n
+    if not dense or step < n:
+        return t.contiguous(), n
+    return t, step
+
+
+def _scan_table(x, dt, A, B, C, D, dt_bias, softplus, cu_seqlens):
+    """(struct MocScan, the tensors it points to)."""
+    H, P = x.shape[-2:]
+    G, N = B.shape[-2:]
+    (x, xs), (dt, ds), (B, bs), (C, cs) = (token_rows(x, 2), token_rows(dt, 1), token_rows(B, 2),
+                                           token_rows(C, 2))
+    (ap, ad), (dp, dd), (bp, bd) = _param(A), _param(D), _param(dt_bias)
+    if cu_seqlens is None:
+        cu, cu64, n_seqs, T, n = None, 0, 0, x.shape[1], x.shape[0] * x.shape[1]
+    else:
+        cu, cu64 = cu_seqlens.data_ptr(), int(cu_seqlens.dtype == torch.int64)
+        n_seqs, T, n = cu_seqlens.numel() - 1, 0, x.shape[0]
+    table = _lib.MocScan(x.data_ptr(), dt.data_ptr(), ap, B.data_ptr(), C.data_ptr(), dp, bp, xs, ds,
+                         bs, cs, cu, n_seqs, n, T, H, P, G, N, cu64, _lib.dtype_code(x.dtype), ad, dd,
+                         bd, int(softplus))
+    return table, (x, dt, B, C)
+
+
+def _query(n: int, what: str) -> int:
+    """A size that the library gave; 0 with an error set: it does not take the problem."""
+    if n == 0:
+        msg = _lib.lib().moc_last_error().decode(errors="replace")
+        if msg:
+            raise RuntimeError(f"{what}: {msg}")
+    return n
+
+
+def launch_scan_forward(x, dt, A, B, C, D, dt_bias, init, *, softplus: bool, final_state: bool,
+                        keep: bool, cu_seqlens=None):
+    """(y, final state or None, saved or None) of the selective scan; ``keep``: also
+    what launch_scan_backward reads."""
+    L = _lib.lib()
+    table, held = _scan_table(x, dt, A, B, C, D, dt_bias, softplus, cu_seqlens)
+    ref = ctypes.byref(table)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    H, P, N = x.shape[-2], x.shape[-1], B.shape[-1]
+    fin = torch.empty(x.shape[0], H, P, N, dtype=torch.float32, device=x.device) if final_state else None
+    with _lib.device_guard(x.device):
+        saved = _workspace(_query(L.moc_scan_saved_bytes(ref), "moc_scan_forward"), x.device) if keep else None
+        ws = _workspace(_query(L.moc_scan_forward_workspace_bytes(ref, int(keep)), "moc_scan_forward"),
+                        x.device)
+        rc = L.moc_scan_forward(ref, y.data_ptr(), _ptr(init), _ptr(fin), _ptr(saved),
+                                0 if saved is None else saved.numel(), ws.data_ptr(), ws.numel(),
+                                _lib.stream_ptr(x.device))
+    _lib.check(rc, "moc_scan_forward")
+    del held
+    return y, fin, saved
+
+
+def launch_scan_backward(x, dt, A, B, C, D, dt_bias, dy, dfinal, saved, *, softplus: bool,
+                         has_init: bool, need_init: bool, cu_seqlens=None):
+    """(dx, ddt, dA, dB, dC, dD or None, ddt_bias or None, dinitial or None)."""
+    L = _lib.lib()
+    table, held = _scan_table(x, dt, A, B, C, D, dt_bias, softplus, cu_seqlens)
+    ref = ctypes.byref(table)
+    dy = dy.to(x.dtype).contiguous()
+    like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+    outs = [like(t) for t in (x, dt, A, B, C, D, dt_bias)]
+    dinit = None
+    if need_init:
+        dinit = torch.empty(x.shape[0], *x.shape[-2:], B.shape[-1], dtype=torch.float32, device=x.device)
+    grads = _lib.MocScanGrads(*[_ptr(t) for t in (*outs, dinit)])
+    with _lib.device_guard(x.device):
+        ws = _workspace(_query(L.moc_scan_backward_workspace_bytes(ref), "moc_scan_backward"), x.device)
+        rc = L.moc_scan_backward(ref, dy.data_ptr(), int(has_init), _ptr(dfinal), saved.data_ptr(),
+                                 saved.numel(), ctypes.byref(grads), ws.data_ptr(), ws.numel(),
+                                 _lib.stream_ptr(x.device))
+    _lib.check(rc, "moc_scan_backward")
+    del held
+    return (*outs, dinit)
+
+
+def launch_scan_update(x, dt, A, B, C, D, dt_bias, state, *, softplus: bool) -> torch.Tensor:
+    """One token per sequence ([B, 1, ..] inputs), in place on the contiguous fp32
+    ``state``."""
+    table, held = _scan_table(x, dt, A, B, C, D, dt_bias, softplus, None)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _lib.device_guard(x.device):
+        rc = _lib.lib().moc_scan_update(ctypes.byref(table), state.data_ptr(), y.data_ptr(),
+                                        _lib.stream_ptr(x.device))
+    _lib.check(rc, "moc_scan_update")
+    del held
+    return y
