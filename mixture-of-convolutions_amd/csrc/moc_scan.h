@@ -28,7 +28,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kQ = 64;        // tokens of a chunk
 constexpr int kTile = 64;     // channels of a head (P) and states (N) of a tile
-constexpr int kRow = 64 + 8;  // elements of an LDS tile's row (the pad spreads rows over banks)
 constexpr float kLog2e = 1.4426950408889634f;
 
 // One operand of a 16 x 16 x 32 product: 8 consecutive contraction entries of a
@@ -46,169 +45,367 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
                                                  0, 0);
 }
 
-// c += a . b, small products first
+// c + a . b.  The products of the lower planes are summed by themselves and added
+// once: each addition to c costs a rounding at c's size.
 __device__ __forceinline__ f32x4 mm(const Frag<1>& a, const Frag<1>& b, f32x4 c) { return mfma(a.v[0], b.v[0], c); }
 __device__ __forceinline__ f32x4 mm(const Frag<1>& a, const Frag<3>& b, f32x4 c) {
-  c = mfma(a.v[0], b.v[2], c);
-  c = mfma(a.v[0], b.v[1], c);
-  return mfma(a.v[0], b.v[0], c);
+  f32x4 t = mfma(a.v[0], b.v[2], f32x4{0.f, 0.f, 0.f, 0.f});
+  t = mfma(a.v[0], b.v[1], t);
+  return mfma(a.v[0], b.v[0], c) + t;
 }
 __device__ __forceinline__ f32x4 mm(const Frag<3>& a, const Frag<3>& b, f32x4 c) {
-  c = mfma(a.v[0], b.v[2], c);
-  c = mfma(a.v[1], b.v[1], c);
-  c = mfma(a.v[2], b.v[0], c);
-  c = mfma(a.v[0], b.v[1], c);
-  c = mfma(a.v[1], b.v[0], c);
-  return mfma(a.v[0], b.v[0], c);
+  f32x4 t = mfma(a.v[0], b.v[2], f32x4{0.f, 0.f, 0.f, 0.f});
+  t = mfma(a.v[1], b.v[1], t);
+  t = mfma(a.v[2], b.v[0], t);
+  t = mfma(a.v[0], b.v[1], t);
+  t = mfma(a.v[1], b.v[0], t);
+  return mfma(a.v[0], b.v[0], c) + t;
 }
 
-// Planes of 8 fp32 values: each plane is what is left, rounded to bf16 (the
-// differences are exact).
+// Two fp32 rounded to bf16 in one dword, a in the low half (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+__device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Planes of 8 fp32 values: each plane is what the ones before it left, rounded to bf16
+// (the differences are exact; those of an infinity are NaN, so what an infinity enters
+// comes out as NaN where there are several planes).
 template <int NP>
 __device__ __forceinline__ Frag<NP> split(const float (&f)[8]) {
-  Frag<NP> r;
+  u32x4 w[NP];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    float rest = f[k];
+  for (int k = 0; k < 4; ++k) {
+    float a = f[2 * k], b = f[2 * k + 1];
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const uint16_t b = f32_to_bf16(rest);
-      r.v[p][k] = static_cast<short>(b);
-      if (p + 1 < NP) {
-        // (an infinity's difference with itself would be NaN in the next planes)
-        const float d = rest - bf16_to_f32(b);
-        rest = (__float_as_uint(f[k]) & 0x7f800000u) == 0x7f800000u ? 0.f : d;
-      }
+      const uint32_t v = pack2(a, b);
+      w[p][k] = v;
+      if (p + 1 < NP) a -= lo_f(v), b -= hi_f(v);
     }
   }
+  Frag<NP> r;
+#pragma unroll
+  for (int p = 0; p < NP; ++p) r.v[p] = __builtin_bit_cast(s16x8, w[p]);
   return r;
 }
 
 template <int NP>
 __device__ __forceinline__ void join(const Frag<NP>& r, float (&f)[8]) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    float v = bf16_to_f32(static_cast<uint16_t>(r.v[NP - 1][k]));
+  for (int k = 0; k < 4; ++k) {
+    const u32x4 top = __builtin_bit_cast(u32x4, r.v[NP - 1]);
+    float a = lo_f(top[k]), b = hi_f(top[k]);
 #pragma unroll
-    for (int p = NP - 2; p >= 0; --p) v += bf16_to_f32(static_cast<uint16_t>(r.v[p][k]));
-    f[k] = v;
+    for (int p = NP - 2; p >= 0; --p) {
+      const u32x4 w = __builtin_bit_cast(u32x4, r.v[p]);
+      a += lo_f(w[k]), b += hi_f(w[k]);
+    }
+    f[2 * k] = a, f[2 * k + 1] = b;
   }
 }
 
-// 8 elements at p, the first `valid` of them real (the others 0); vec: p is aligned
-// to 16 bytes where valid == 8.
+// 8 elements as they lie in memory.
 template <int DT>
-__device__ __forceinline__ Frag<kPlanes<DT>> load8(const void* base, int64_t at, int valid, bool vec) {
-  if constexpr (DT == DT_BF16) {
-    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-    Frag<1> r;
-    if (vec && valid >= 8) {
-      r.v[0] = *reinterpret_cast<const s16x8*>(p);
-    } else {
+struct Raw;
+template <>
+struct Raw<DT_BF16> {
+  u32x4 w;
+  __device__ __forceinline__ Frag<1> frag() const { return Frag<1>{{__builtin_bit_cast(s16x8, w)}}; }
+  // bit 15 or 31 of a word: an exponent of all ones (an infinity or NaN)
+  __device__ __forceinline__ uint32_t odd() const {
+    uint32_t r = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) r.v[0][k] = k < valid ? static_cast<short>(p[k]) : short(0);
-    }
+    for (int k = 0; k < 4; ++k) r |= ((w[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
     return r;
-  } else {
-    const float* p = static_cast<const float*>(base) + at;
-    float f[8];
-    if (vec && valid >= 8) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) f[k] = a[k], f[4 + k] = b[k];
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = k < valid ? p[k] : 0.f;
-    }
+  }
+};
+template <>
+struct Raw<DT_F32> {
+  f32x4 lo, hi;
+  __device__ __forceinline__ Frag<3> frag() const {
+    const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return split<3>(f);
   }
-}
-
-// 4 elements as fp32, likewise (vec: aligned to 4 elements).
-template <int DT>
-__device__ __forceinline__ f32x4 load4(const void* base, int64_t at, int valid, bool vec) {
-  f32x4 r;
-  if (vec && valid >= 4) {
-    float f[4];
-    load_vec<DT, 4>(base, at, f);
-    r = f32x4{f[0], f[1], f[2], f[3]};
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) r[k] = k < valid ? load_any(base, DT, at + k) : 0.f;
-  }
-  return r;
-}
-
-template <int DT>
-__device__ __forceinline__ void store4(void* base, int64_t at, int valid, bool vec, f32x4 v) {
-  if (vec && valid >= 4) {
-    const float f[4] = {v[0], v[1], v[2], v[3]};
-    store_vec<DT, 4>(base, at, f);
-  } else {
+  __device__ __forceinline__ uint32_t odd() const {
+    uint32_t r = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (k < valid) store_any(base, DT, at + k, v[k]);
+      r |= ((__float_as_uint(lo[k]) & 0x7f800000u) + 0x00800000u) |
+           ((__float_as_uint(hi[k]) & 0x7f800000u) + 0x00800000u);
+    return r & 0x80000000u;
   }
-}
+};
 
-// An LDS tile of bf16 planes: rows of `stride` elements.
-template <int NP>
-struct Tile {
-  uint16_t* p;
-  int stride, plane;  // elements
-  __device__ __forceinline__ void put8(int row, int col, const Frag<NP>& r) const {
-#pragma unroll
-    for (int k = 0; k < NP; ++k) *reinterpret_cast<s16x8*>(p + k * plane + row * stride + col) = r.v[k];
+// Rows (tokens, or channels of a state) of a tensor from one of them on: element
+// (row, col) lies at base + row * stride + col; rows from n on and columns from `cols` on
+// read as 0.  VEC: column counts and strides are multiples of 8 and base is aligned to 16
+// bytes: reads go through a buffer resource, whose range check makes the zeros (an offset
+// no range reaches stands for what is not there), without a branch.
+constexpr uint32_t kNowhere = 0x80000000u;
+constexpr int64_t kMaxStride = int64_t(1) << 22;  // VEC: 64 rows stay below kNowhere
+
+template <int DT, bool VEC>
+struct Rows {
+  static constexpr int E = DT == DT_BF16 ? 2 : 4;
+  const char* base;
+  int64_t stride;
+  int n, cols;
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Rows(const void* p, int64_t at, int64_t stride_, int n_, int cols_)
+      : base(static_cast<const char*>(p) + at * E), stride(stride_), n(n_), cols(cols_) {
+    if constexpr (VEC) r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00020000);
   }
-  __device__ __forceinline__ Frag<NP> get8(int row, int col) const {
-    Frag<NP> r;
-#pragma unroll
-    for (int k = 0; k < NP; ++k) r.v[k] = *reinterpret_cast<const s16x8*>(p + k * plane + row * stride + col);
-    return r;
+  __device__ __forceinline__ uint32_t off(int row, int col) const {
+    const uint32_t o = static_cast<uint32_t>(row * static_cast<int>(stride) + col) * E;
+    return row < n && col < cols ? o : kNowhere;
   }
-  // 4 values (fp32) split over the planes
-  __device__ __forceinline__ void put4(int row, int col, f32x4 v) const {
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      s16x4 b;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint16_t h = f32_to_bf16(v[e]);
-        b[e] = static_cast<short>(h);
-        if (k + 1 < NP)
-          v[e] = (__float_as_uint(v[e]) & 0x7f800000u) == 0x7f800000u ? 0.f : v[e] - bf16_to_f32(h);
+  __device__ __forceinline__ Raw<DT> get8(int row, int col) const {
+    Raw<DT> v;
+    if constexpr (VEC) {
+      const int o = static_cast<int>(off(row, col));
+      if constexpr (DT == DT_BF16) {
+        v.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+      } else {
+        v.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+        v.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 16, 0));
       }
-      *reinterpret_cast<s16x4*>(p + k * plane + row * stride + col) = b;
-    }
-  }
-  __device__ __forceinline__ f32x4 get4(int row, int col) const {
-    f32x4 v{0.f, 0.f, 0.f, 0.f};
+    } else {
+      const int have = row < n ? cols - col : 0;
+      const int64_t at = row * stride + col;
+      if constexpr (DT == DT_BF16) {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + at;
 #pragma unroll
-    for (int k = NP - 1; k >= 0; --k) {
-      const s16x4 b = *reinterpret_cast<const s16x4*>(p + k * plane + row * stride + col);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a = 2 * k < have ? p[2 * k] : 0u, b = 2 * k + 1 < have ? p[2 * k + 1] : 0u;
+          v.w[k] = a | (b << 16);
+        }
+      } else {
+        const float* p = reinterpret_cast<const float*>(base) + at;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += bf16_to_f32(static_cast<uint16_t>(b[e]));
+        for (int k = 0; k < 4; ++k) {
+          v.lo[k] = k < have ? p[k] : 0.f;
+          v.hi[k] = 4 + k < have ? p[4 + k] : 0.f;
+        }
+      }
     }
     return v;
   }
-  // A transposed operand: entry k of lane (i, g) (i = lane % 16, g = lane / 16) is
-  // element [row0 + 8 g + k][col0 + i].  Two ds_read_b64_tr_b16 a plane: lane i of a
-  // 16-lane group gets element i % 4 of the 8-byte rows read by lanes i / 4 + {0, 4,
-  // 8, 12}, so lane L reads row L / 4 of four, columns 4 (L % 4)...
-  __device__ __forceinline__ Frag<NP> tr8(int row0, int col0, int lane) const {
-    const int L = lane & 15, at = (row0 + 8 * (lane >> 4) + (L >> 2)) * stride + col0 + 4 * (L & 3);
+  // 4 elements as fp32
+  __device__ __forceinline__ f32x4 get4(int row, int col) const {
+    f32x4 v;
+    if constexpr (VEC) {
+      const int o = static_cast<int>(off(row, col));
+      if constexpr (DT == DT_BF16) {
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+        v = f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
+      } else {
+        v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+      }
+    } else {
+      const int have = row < n ? cols - col : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = k < have ? load_any(base, DT, row * stride + col + k) : 0.f;
+    }
+    return v;
+  }
+  __device__ __forceinline__ void put4(int row, int col, f32x4 v) const {
+    if constexpr (VEC) {
+      const int o = static_cast<int>(off(row, col));
+      if constexpr (DT == DT_BF16) {
+        const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
+        __builtin_amdgcn_raw_buffer_store_b64(w, r, o, 0, 0);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, o, 0, 0);
+      }
+    } else {
+      const int have = row < n ? cols - col : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < have) store_any(const_cast<char*>(base), DT, row * stride + col + k, v[k]);
+    }
+  }
+};
+
+// An LDS tile of bf16 planes, W = 64, 128 or 256 columns.  Blocks of 8 columns (16 bytes)
+// of a row are permuted by an exclusive or with f(row), so that both kinds of operand
+// reads meet every bank once: rows li = 0..15 at one block (get8: f takes 16 values, or 8
+// on the rows of one parity where two rows share the banks, W = 64), and rows {0..3, 8..11}
+// or {4..7, 12..15} at two neighbouring blocks (tr8: so do f's upper bits).
+//
+// Offsets are (a lane's own) ^ (the column's part) + (the row block's part):
+//   nat   row li, block g           (8 elements: column 8 g)
+//   quad  row li, 4 elements        (column 4 g)
+//   tr    row 8 g + L / 4, columns 4 (L % 4).. of a transposed read
+template <int W>
+struct Lane {
+  int nat, quad, tr;
+  static __device__ __forceinline__ int f(int row) {
+    if (W == 64) return ((row >> 1 & 1) << 2) | ((row >> 3 & 1) << 1) | (row >> 2 & 1);
+    return ((row & 1) << 3) | ((row >> 1 & 1) << 2) | ((row >> 3 & 1) << 1) | (row >> 2 & 1);
+  }
+  __device__ __forceinline__ Lane() {
+    const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    nat = li * W + ((g ^ f(li)) << 3);
+    quad = li * W + (((g >> 1) ^ f(li)) << 3) + 4 * (g & 1);
+    const int row = 8 * g + (li >> 2);
+    tr = row * W + ((((li & 3) >> 1) ^ f(row)) << 3) + 4 * (li & 1);
+  }
+  // In a loop: the compiler may not take the offsets formed from these for loop
+  // invariants (it would hold all of them in registers, and spill).
+  __device__ __forceinline__ void refresh() { asm volatile("" : "+v"(nat), "+v"(quad), "+v"(tr)); }
+};
+
+template <int NP, int W>
+struct Tile {
+  static constexpr int kPlane = 64 * W;  // elements
+  static constexpr int kBytes = NP * kPlane * 2;
+  uint16_t* p;
+  // 8 elements of any row and column block
+  __device__ __forceinline__ void put8(int row, int col, const Frag<NP>& r) const {
+    uint16_t* q = p + row * W + (((col >> 3) ^ Lane<W>::f(row)) << 3);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) *reinterpret_cast<s16x8*>(q + k * kPlane) = r.v[k];
+  }
+  // row 16 rb + li, columns 32 ks + 8 g..
+  __device__ __forceinline__ Frag<NP> get8(const Lane<W>& l, int rb, int ks) const {
+    const uint16_t* q = p + (l.nat ^ (32 * ks)) + 16 * rb * W;
     Frag<NP> r;
 #pragma unroll
+    for (int k = 0; k < NP; ++k) r.v[k] = *reinterpret_cast<const s16x8*>(q + k * kPlane);
+    return r;
+  }
+  // row 16 rb + li, columns 32 ks + 4 g.. and 32 ks + 16 + 4 g..
+  __device__ __forceinline__ Frag<NP> get44(const Lane<W>& l, int rb, int ks) const {
+    const uint16_t *q = p + (l.quad ^ (32 * ks)) + 16 * rb * W, *q2 = p + (l.quad ^ (32 * ks + 16)) + 16 * rb * W;
+    Frag<NP> r;
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+      r.v[k] = __builtin_shufflevector(*reinterpret_cast<const s16x4*>(q + k * kPlane),
+                                       *reinterpret_cast<const s16x4*>(q2 + k * kPlane), 0, 1, 2, 3, 4, 5, 6, 7);
+    return r;
+  }
+  // row 16 rb + li, columns 16 cb + 4 g..: 4 fp32 values split over the planes
+  __device__ __forceinline__ void put4(const Lane<W>& l, int rb, int cb, f32x4 v) const {
+    uint16_t* q = p + (l.quad ^ (16 * cb)) + 16 * rb * W;
+#pragma unroll
     for (int k = 0; k < NP; ++k) {
-      const uint16_t* q = p + k * plane + at;
-      const s16x4 a = tr(q), b = tr(q + 4 * stride);
-      r.v[k] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
+      *reinterpret_cast<u32x2*>(q + k * kPlane) = w;
+      if (k + 1 < NP) v -= f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
     }
+  }
+  __device__ __forceinline__ f32x4 get4(const Lane<W>& l, int rb, int cb) const {
+    const uint16_t* q = p + (l.quad ^ (16 * cb)) + 16 * rb * W;
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = NP - 1; k >= 0; --k) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(q + k * kPlane);
+      v += f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
+    }
+    return v;
+  }
+  // one element as fp32
+  __device__ __forceinline__ float at(int row, int col) const {
+    const uint16_t* q = p + row * W + (((col >> 3) ^ Lane<W>::f(row)) << 3) + (col & 7);
+    float v = 0.f;
+#pragma unroll
+    for (int k = NP - 1; k >= 0; --k) v += bf16_to_f32(q[k * kPlane]);
+    return v;
+  }
+  // A transposed operand: entry k of lane (li, g) is element [32 ks + 8 g + k][16 cb + li].
+  // Two ds_read_b64_tr_b16 a plane: lane i of a 16-lane group gets element i % 4 of the
+  // 8-byte rows read by lanes i / 4 + {0, 4, 8, 12}, so lane L reads row L / 4 of four,
+  // columns 4 (L % 4)..; the next four rows differ in one bit of f.
+  __device__ __forceinline__ Frag<NP> tr8(const Lane<W>& l, int ks, int cb) const {
+    const int o = l.tr ^ (16 * cb);
+    const uint16_t *q = p + o + 32 * ks * W, *q2 = p + (o ^ 8) + (32 * ks + 4) * W;
+    Frag<NP> r;
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+      r.v[k] = __builtin_shufflevector(tr(q + k * kPlane), tr(q2 + k * kPlane), 0, 1, 2, 3, 4, 5, 6, 7);
     return r;
   }
   static __device__ __forceinline__ s16x4 tr(const uint16_t* q) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         (__attribute__((address_space(3))) s16x4*)(const_cast<uint16_t*>(q)));
+  }
+};
+
+// 64 rows of a tensor on their way to an LDS tile of W columns: loads first (all in
+// flight), the tile once the last chunk's readers are done.
+template <int DT, bool VEC, int W, int THREADS>
+struct Staged {
+  static constexpr int kLoads = 8 * W / THREADS;  // vectors of 8 of a thread
+  Raw<DT> v[kLoads];
+  __device__ __forceinline__ void load(const Rows<DT, VEC>& src) {
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) v[k] = src.get8(row(k), col(k));
+  }
+  template <int NP>
+  __device__ __forceinline__ void put(const Tile<NP, W>& t) const {
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) t.put8(row(k), col(k), v[k].frag());
+  }
+  __device__ __forceinline__ uint32_t odd() const {
+    uint32_t r = 0;
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) r |= v[k].odd();
+    return r;
+  }
+  static __device__ __forceinline__ int row(int k) { return threadIdx.x / (W / 8) + k * (THREADS / (W / 8)); }
+  static __device__ __forceinline__ int col(int) { return threadIdx.x % (W / 8) * 8; }
+};
+
+// The factors of a chunk's decays.  For tokens of two blocks of 16, i's after j's,
+//   exp(s_i - s_j) = a_i exp(start of i's block - end of j's block) b_j
+// with a_i = exp(s_i - start) and b_j = exp(end - s_j): one exponential a token instead of one
+// a pair (a at a block's last token is the whole block's); within a block the pair's own.
+struct Decays {
+  float* a;    // exp(s - its block's start)
+  float* b;    // exp(its block's end - s)
+  float* e;    // exp(s)
+  float* f;    // exp(s_last - s)
+  float* u;
+  double* s;
+  static constexpr int kBytes = kQ * (5 * 4 + 8);
+  __device__ __forceinline__ explicit Decays(char* p) {
+    s = reinterpret_cast<double*>(p);
+    a = reinterpret_cast<float*>(s + kQ);
+    b = a + kQ;
+    e = b + kQ;
+    f = e + kQ;
+    u = f + kQ;
+  }
+  // every wave: lane t with token t's u and s; wave w makes a part of them
+  __device__ __forceinline__ void put(int wave, double sv, float uv) const {
+    const int t = threadIdx.x & 63;
+    auto ex = [](double d) { return __builtin_amdgcn_exp2f(static_cast<float>(d)); };
+    if (wave == 0) {
+      const double before = __shfl(sv, (t & 48) > 0 ? (t & 48) - 1 : 0);
+      a[t] = ex(t < 16 ? sv : sv - before);
+      s[t] = sv;
+    } else if (wave == 1) {
+      b[t] = ex(__shfl(sv, t | 15) - sv);
+    } else if (wave == 2) {
+      e[t] = ex(sv);
+      u[t] = uv;
+    } else {
+      f[t] = ex(__shfl(sv, 63) - sv);
+    }
+  }
+  // exp(start of block ib - end of block jb), jb < ib
+  __device__ __forceinline__ float between(int ib, int jb) const {
+    float v = 1.f;
+    if (jb < 1 && ib > 1) v *= a[31];
+    if (jb < 2 && ib > 2) v *= a[47];
+    return v;
   }
 };
 
@@ -263,7 +460,7 @@ struct Args {
   int64_t seg;      // tokens of a segment
   float* u;         // [H][chunks][kQ] softplus(dt + bias), 0 behind a sequence's end
   double* s;        // [H][chunks][kQ] running sum of u A log2(e) within the chunk
-  bool vec_x, vec_b, vec_c, vec_h, vec_y;  // 16-byte loads of x, B, C, states, y-like
+  bool vec;         // 16-byte accesses of everything that the kernels load and store
 };
 
 // Chunk `id`: false where there is none.
@@ -296,7 +493,6 @@ struct Walk {
   const void* x;        // [tokens][H][P], x_stride apart
   const void* b;        // [tokens][G][N]
   int64_t x_stride, b_stride;
-  bool vec_x, vec_b;
   const float* start;   // [sequences][H][P][N] or null: state at the walk's start
   float* end;           // the same or null: state at its end
   float* seg_state;     // [segments][H][P][N]: state at each segment's start

@@ -58,124 +58,153 @@ __global__ __launch_bounds__(kThreads) void prep_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// rows t0.. of a [tokens][..] tensor to an LDS tile of 64 NT columns; n rows and
-// `cols` columns are real, the others 0.  Returns whether a value is not finite.
-template <int DT, int NT>
-__device__ __forceinline__ bool stage(const Tile<kPlanes<DT>>& tile, const void* src, int64_t t0, int64_t stride,
-                                      int64_t col0, int n, int cols, bool vec) {
-  bool odd = false;
+// acc: states 16 nb + 4 g + r of one channel, from / to a [P][N] state's rows
+template <int NB, int DT, bool VEC>
+__device__ __forceinline__ void load_state(const Rows<DT, VEC>& src, int row, f32x4 (&acc)[NB]) {
+  const int n0 = 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-  for (int k = 0; k < 2 * NT; ++k) {
-    const int at = threadIdx.x + k * kThreads, row = at / (8 * NT), col = (at % (8 * NT)) * 8;
-    const int valid = row < n ? cols - col : 0;
-    const Frag<kPlanes<DT>> f = load8<DT>(src, (t0 + row) * stride + col0 + col, valid, vec);
+  for (int nb = 0; nb < NB; ++nb) acc[nb] = src.get4(row, 16 * nb + n0);
+}
+template <int NB, int DT, bool VEC>
+__device__ __forceinline__ void store_state(const Rows<DT, VEC>& dst, int row, const f32x4 (&acc)[NB]) {
+  const int n0 = 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) odd |= (f.v[0][e] & 0x7f80) == 0x7f80;
-    tile.put8(row, col, f);
-  }
-  return odd;
+  for (int nb = 0; nb < NB; ++nb) dst.put4(row, 16 * nb + n0, acc[nb]);
 }
 
-// acc (n = 16 nb + 4 g + r rows, channel column) from / to a [P][N] state
-template <int NB, int DT>
-__device__ __forceinline__ void load_state(const void* src, int64_t at, int p, int P, int N, int g, bool vec,
-                                           f32x4 (&acc)[NB]) {
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int n = 16 * nb + 4 * g;
-    acc[nb] = load4<DT>(src, at + int64_t(p) * N + n, p < P ? N - n : 0, vec);
-  }
-}
-template <int NB, int DT>
-__device__ __forceinline__ void store_state(void* dst, int64_t at, int p, int P, int N, int g, bool vec,
-                                            const f32x4 (&acc)[NB]) {
-  if (p >= P) return;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int n = 16 * nb + 4 * g;
-    store4<DT>(dst, at + int64_t(p) * N + n, N - n, vec, acc[nb]);
-  }
-}
-
-// 8 products of a transposed x operand and the weights w[row0 + 8 g ..] as three planes
+// 8 products of a transposed x operand and the tokens' weights w[0..8) as three planes
 template <int NP>
 __device__ __forceinline__ Frag<3> weighted(const Frag<NP>& x, const float* w) {
   float f[8];
   join(x, f);
+  const f32x4 lo = *reinterpret_cast<const f32x4*>(w), hi = *reinterpret_cast<const f32x4*>(w + 4);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] *= w[k];
+  for (int k = 0; k < 4; ++k) f[k] *= lo[k], f[4 + k] *= hi[k];
   return split<3>(f);
 }
 
-// acc = decay acc + sum over the chunk's tokens of (w x) (x) b
-template <int NP, int NB>
-__device__ __forceinline__ void update_state(const Tile<NP>& bt, const Frag<3> (&uf)[2], float decay, int lane,
-                                             f32x4 (&acc)[NB]) {
+// acc = decay acc + sum over the chunk's tokens of (w x) (x) b, the sum by itself first:
+// the state's own rounding is one a chunk, not one a product step
+template <int NP, int W, int NB>
+__device__ __forceinline__ void update_state(const Tile<NP, W>& bt, const Lane<W>& l, const Frag<3> (&uf)[2],
+                                             float decay, f32x4 (&acc)[NB]) {
+  // one block's operands ahead of its products, no more: left to itself the compiler reads
+  // every block's first and spills them
+  Frag<NP> b0 = bt.tr8(l, 0, 0), b1 = bt.tr8(l, 1, 0);
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    f32x4 v = acc[nb] * decay;
-    v = mm(bt.tr8(0, 16 * nb, lane), uf[0], v);
-    acc[nb] = mm(bt.tr8(32, 16 * nb, lane), uf[1], v);
+    const Frag<NP> c0 = b0, c1 = b1;
+    if (nb + 1 < NB) b0 = bt.tr8(l, 0, nb + 1), b1 = bt.tr8(l, 1, nb + 1);
+    const f32x4 v = mm(c1, uf[1], mm(c0, uf[0], f32x4{0.f, 0.f, 0.f, 0.f}));
+    acc[nb] = acc[nb] * decay + v;
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
+
+// The segment of a walk's workgroup.
+struct Segment {
+  int64_t m, t0, c0;   // sequence, first token, first chunk
+  int n, chunks;       // tokens, chunks
+  bool first, last;    // of its sequence
+};
+__device__ __forceinline__ bool segment_at(const Args& a, int64_t id, Segment& s) {
+  int64_t j;
+  if (!a.seqs.find(id, a.seg, s.m, j)) return false;
+  const int64_t lo = a.seqs.edge(s.m), hi = a.seqs.edge(s.m + 1);
+  s.t0 = lo + j * a.seg;
+  s.n = static_cast<int>(hi - s.t0 < a.seg ? hi - s.t0 : a.seg);
+  s.chunks = (s.n + kQ - 1) / kQ;
+  s.c0 = a.seqs.base(s.m, kQ) + j * (a.seg / kQ);
+  s.first = j == 0;
+  s.last = s.t0 + s.n == hi;
+  return true;
+}
+
+// Workgroups of 256 threads (waves a SIMD) that `lds` bytes each leave room for on a CU, at
+// most `most`: the registers are bounded by what that many waves can have.
+constexpr int waves_for(int lds, int most) { return 160 * 1024 / lds < most ? 160 * 1024 / lds : most; }
+
+template <int DT, int NT>
+constexpr int kWalkLds = kPlanes<DT> * kQ * (64 * NT + 64) * 2 + kQ * 4;
+// (B, and C where it is staged)
+template <int DT, int NT>
+constexpr int kForwardLds =
+    kPlanes<DT> * kQ * ((DT == DT_BF16 ? 2 : 1) * 64 * NT + 128) * 2 + Decays::kBytes + 16;
 
 // The state over one segment's chunks, forwards (REV false) or backwards.  LOCAL: from
 // zero, for segments that another one follows, to seg_state and seg_decay; else from the
 // state that enters the segment, kept before each chunk.
-template <int DT, int NT, bool REV, bool LOCAL>
-__global__ __launch_bounds__(kThreads) void state_walk(Args a, Walk w) {
-  constexpr int NP = kPlanes<DT>, NB = 4 * NT, NS = 64 * NT + 8;
-  extern __shared__ char smem[];
-  const Tile<NP> bt{reinterpret_cast<uint16_t*>(smem), NS, kQ * NS};
-  const Tile<NP> xt{bt.p + NP * kQ * NS, kRow, kQ * kRow};
-  float* wj = reinterpret_cast<float*>(xt.p + NP * kQ * kRow);
+template <int DT, int NT, bool VEC, bool REV, bool LOCAL>
+__global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 : (NT == 2 ? 3 : 2))) void state_walk(Args a, Walk w) {
+  constexpr int NP = kPlanes<DT>, NB = 4 * NT, W = 64 * NT;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Tile<NP, W> bt{reinterpret_cast<uint16_t*>(smem)};
+  const Tile<NP, 64> xt{reinterpret_cast<uint16_t*>(smem + bt.kBytes)};
+  float* wj = reinterpret_cast<float*>(smem + bt.kBytes + xt.kBytes);
+  Lane<W> lw;
+  Lane<64> lx;
   const int lane = threadIdx.x & 63, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int P = static_cast<int>(a.p.P), N = static_cast<int>(a.p.N);
   const int ptiles = (P + kTile - 1) / kTile;
-  const int h = blockIdx.y / ptiles, p0 = (blockIdx.y % ptiles) * kTile, p = p0 + 16 * wave + (lane & 15);
-  int64_t m, j;
-  if (!a.seqs.find(blockIdx.x, a.seg, m, j)) return;
-  const int64_t lo = a.seqs.edge(m), hi = a.seqs.edge(m + 1);
-  const int64_t t0 = lo + j * a.seg, t1 = t0 + a.seg < hi ? t0 + a.seg : hi;
-  const bool at_start = REV ? t1 == hi : j == 0, at_end = REV ? j == 0 : t1 == hi;
+  const int h = blockIdx.y / ptiles, p0 = (blockIdx.y % ptiles) * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
+  Segment s;
+  if (!segment_at(a, blockIdx.x, s)) return;
+  const bool at_start = REV ? s.last : s.first, at_end = REV ? s.first : s.last;
   if (LOCAL && at_end) return;
-  const int64_t n_chunks = (t1 - t0 + kQ - 1) / kQ, c0 = a.seqs.base(m, kQ) + j * (a.seg / kQ);
-  const int64_t state = ((LOCAL || !at_start ? int64_t(blockIdx.x) : m) * a.p.H + h) * P * N;
-  const bool active = p0 + 16 * wave < P;
+  const int row = 16 * wave + (lane & 15);  // this lane's channel, from p0 on
+  const bool active = 16 * wave < cols;
+  auto state = [&](const void* p, int64_t at) {
+    return Rows<DT_F32, VEC>(p, ((at * a.p.H + h) * P + p0) * N, N, cols, N);
+  };
   f32x4 acc[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float* from = LOCAL ? nullptr : (at_start ? w.start : w.seg_state);
-  if (from != nullptr) load_state<NB, DT_F32>(from, state, p, P, N, g, a.vec_h, acc);
+  if (from != nullptr) load_state<NB>(state(from, at_start ? s.m : int64_t(blockIdx.x)), row, acc);
+  const int64_t at = (int64_t(h) * a.chunks + s.c0) * kQ;
+  const int64_t xcol = int64_t(h) * P + p0, bcol = int64_t(h / (a.p.H / a.p.G)) * N;
+  Staged<DT, VEC, 64, kThreads> sx;
+  Staged<DT, VEC, W, kThreads> sb;
+  double sv;
+  float uv = 0.f;
+  auto fetch = [&](int i) {
+    const int64_t t = s.t0 + int64_t(i) * kQ;
+    const int n = s.n - i * kQ < kQ ? s.n - i * kQ : kQ;
+    sx.load(Rows<DT, VEC>(w.x, t * w.x_stride + xcol, w.x_stride, n, cols));
+    sb.load(Rows<DT, VEC>(w.b, t * w.b_stride + bcol, w.b_stride, n, N));
+    sv = a.s[at + i * kQ + lane];
+    if (!REV) uv = a.u[at + i * kQ + lane];
+  };
   double total = 0.0;
-  for (int64_t k = 0; k < n_chunks; ++k) {
-    const int64_t i = REV ? n_chunks - 1 - k : k, id = c0 + i, t = t0 + i * kQ;
-    const int n = static_cast<int>(t1 - t < kQ ? t1 - t : kQ);
+  fetch(REV ? s.chunks - 1 : 0);
+#pragma unroll 1
+  for (int k = 0; k < s.chunks; ++k) {
+    lw.refresh(), lx.refresh();
+    const int i = REV ? s.chunks - 1 - k : k;
     if (!LOCAL && w.kept != nullptr && !(k == 0 && from == nullptr))
-      store_state<NB, DT>(w.kept, (id * a.p.H + h) * P * N, p, P, N, g, a.vec_h, acc);
-    const int64_t at = (int64_t(h) * a.chunks + id) * kQ;
-    const double last = a.s[at + kQ - 1];
+      store_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + i) * a.p.H + h) * P + p0) * N, N, cols, N), row, acc);
+    sx.put(xt);
+    sb.put(bt);
+    const double last = __shfl(sv, 63);
     total += last;
-    if (threadIdx.x < kQ) {
-      const double s = a.s[at + threadIdx.x];
-      wj[threadIdx.x] = REV ? __builtin_amdgcn_exp2f(static_cast<float>(s))
-                            : a.u[at + threadIdx.x] * __builtin_amdgcn_exp2f(static_cast<float>(last - s));
-    }
-    stage<DT, 1>(xt, w.x, t, w.x_stride, int64_t(h) * P + p0, n, P - p0 < kTile ? P - p0 : kTile, w.vec_x);
-    stage<DT, NT>(bt, w.b, t, w.b_stride, int64_t(h / (a.p.H / a.p.G)) * N, n, N, w.vec_b);
+    const float decay = __builtin_amdgcn_exp2f(static_cast<float>(last));
+    if (wave == 0)
+      wj[lane] = REV ? __builtin_amdgcn_exp2f(static_cast<float>(sv))
+                     : uv * __builtin_amdgcn_exp2f(static_cast<float>(last - sv));
     __syncthreads();
+    if (k + 1 < s.chunks) fetch(REV ? i - 1 : i + 1);
     if (active) {
-      const Frag<3> uf[2] = {weighted(xt.tr8(0, 16 * wave, lane), wj + 8 * g),
-                             weighted(xt.tr8(32, 16 * wave, lane), wj + 32 + 8 * g)};
-      update_state<NP, NB>(bt, uf, __builtin_amdgcn_exp2f(static_cast<float>(last)), lane, acc);
+      const Frag<3> uf[2] = {weighted(xt.tr8(lx, 0, wave), wj + 8 * g),
+                             weighted(xt.tr8(lx, 1, wave), wj + 32 + 8 * g)};
+      update_state(bt, lw, uf, decay, acc);
     }
     __syncthreads();
   }
   if (LOCAL) {
-    store_state<NB, DT_F32>(w.seg_state, state, p, P, N, g, a.vec_h, acc);
+    store_state<NB>(state(w.seg_state, blockIdx.x), row, acc);
     if (threadIdx.x == 0 && p0 == 0) w.seg_decay[int64_t(blockIdx.x) * a.p.H + h] = total;
   } else if (at_end && w.end != nullptr) {
-    store_state<NB, DT_F32>(w.end, (m * a.p.H + h) * P * N, p, P, N, g, a.vec_h, acc);
+    store_state<NB>(state(w.end, s.m), row, acc);
   }
 }
 
@@ -206,93 +235,115 @@ __global__ __launch_bounds__(kThreads) void join_segments(Args a, Walk w) {
 }
 
 // ---------------------------------------------------------------------------
-template <int DT, int NT>
-__global__ __launch_bounds__(kThreads) void forward_walk(Args a, Walk w, void* __restrict__ y) {
-  constexpr int NP = kPlanes<DT>, NB = 4 * NT, NS = 64 * NT + 8;
+template <int DT, int NT, bool VEC>
+__global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void forward_walk(Args a, Walk w, void* y) {
+  constexpr int NP = kPlanes<DT>, NB = 4 * NT, W = 64 * NT;
   constexpr bool kCInLds = DT == DT_BF16;  // (three planes of it beside B's would not fit)
-  extern __shared__ char smem[];
-  const Tile<NP> bt{reinterpret_cast<uint16_t*>(smem), NS, kQ * NS};
-  const Tile<NP> ct{bt.p + NP * kQ * NS, NS, kQ * NS};
-  const Tile<NP> xt{ct.p + (kCInLds ? NP * kQ * NS : 0), kRow, kQ * kRow};
-  const Tile<NP> mt{xt.p + NP * kQ * kRow, kRow, kQ * kRow};
-  double* ss = reinterpret_cast<double*>(mt.p + NP * kQ * kRow);
-  float* us = reinterpret_cast<float*>(ss + kQ);
-  float* wj = us + kQ;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Tile<NP, W> bt{reinterpret_cast<uint16_t*>(smem)};
+  const Tile<NP, W> ct{reinterpret_cast<uint16_t*>(smem + bt.kBytes)};
+  const Tile<NP, 64> xt{reinterpret_cast<uint16_t*>(smem + (kCInLds ? 2 : 1) * bt.kBytes)};
+  const Tile<NP, 64> mt{xt.p + xt.kBytes / 2};
+  const Decays dec(reinterpret_cast<char*>(mt.p + mt.kBytes / 2));
+  int* odd = reinterpret_cast<int*>(reinterpret_cast<char*>(dec.s) + Decays::kBytes);  // [2], by chunk parity
+  Lane<W> lw;
+  Lane<64> lx;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int P = static_cast<int>(a.p.P), N = static_cast<int>(a.p.N);
   const int ptiles = (P + kTile - 1) / kTile;
-  const int h = blockIdx.y / ptiles, p0 = (blockIdx.y % ptiles) * kTile, p = p0 + 16 * wave + li;
-  int64_t m, j;
-  if (!a.seqs.find(blockIdx.x, a.seg, m, j)) return;
-  const int64_t lo = a.seqs.edge(m), hi = a.seqs.edge(m + 1);
-  const int64_t t0 = lo + j * a.seg, t1 = t0 + a.seg < hi ? t0 + a.seg : hi;
-  const int64_t n_chunks = (t1 - t0 + kQ - 1) / kQ, c0 = a.seqs.base(m, kQ) + j * (a.seg / kQ);
-  const bool active = p0 + 16 * wave < P;
-  const int cols = P - p0 < kTile ? P - p0 : kTile;
-  const int64_t group = int64_t(h / (a.p.H / a.p.G)) * N;
+  const int h = blockIdx.y / ptiles, p0 = (blockIdx.y % ptiles) * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
+  Segment s;
+  if (!segment_at(a, blockIdx.x, s)) return;
+  const int row = 16 * wave + li;  // this lane's channel of the state, from p0 on
+  const bool active = 16 * wave < cols;
   const float skip = a.p.D == nullptr ? 0.f : load_any(a.p.D, a.p.d_dt, h);
+  auto state = [&](const void* p, int64_t at) {
+    return Rows<DT_F32, VEC>(p, ((at * a.p.H + h) * P + p0) * N, N, cols, N);
+  };
   f32x4 acc[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float* from = j == 0 ? w.start : w.seg_state;
-  if (from != nullptr)
-    load_state<NB, DT_F32>(from, ((j == 0 ? m : int64_t(blockIdx.x)) * a.p.H + h) * P * N, p, P, N, g, a.vec_h, acc);
+  const float* from = s.first ? w.start : w.seg_state;
+  if (from != nullptr) load_state<NB>(state(from, s.first ? s.m : int64_t(blockIdx.x)), row, acc);
   // the block right of the diagonal that a 32-token product step reads (no wave writes it)
-  if ((wave & 1) == 0) mt.put4(16 * wave + li, 16 * wave + 16 + 4 * g, f32x4{0.f, 0.f, 0.f, 0.f});
-  for (int64_t k = 0; k < n_chunks; ++k) {
-    const int64_t id = c0 + k, t = t0 + k * kQ;
-    const int n = static_cast<int>(t1 - t < kQ ? t1 - t : kQ);
-    const int64_t at = (int64_t(h) * a.chunks + id) * kQ;
-    const double last = a.s[at + kQ - 1];
-    if (threadIdx.x < kQ) {
-      const double s = a.s[at + threadIdx.x];
-      const float u = a.u[at + threadIdx.x];
-      ss[threadIdx.x] = s;
-      us[threadIdx.x] = u;
-      wj[threadIdx.x] = u * __builtin_amdgcn_exp2f(static_cast<float>(last - s));
-    }
-    const bool odd = stage<DT, 1>(xt, a.p.x, t, a.p.x_stride, int64_t(h) * P + p0, n, cols, a.vec_x);
-    stage<DT, NT>(bt, a.p.B, t, a.p.b_stride, group, n, N, a.vec_b);
-    if (kCInLds) stage<DT, NT>(ct, a.p.C, t, a.p.c_stride, group, n, N, a.vec_c);
-    const bool bad = __syncthreads_or(odd);
+  if ((wave & 1) == 0) mt.put4(lx, wave, wave + 1, f32x4{0.f, 0.f, 0.f, 0.f});
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+  const int64_t at = (int64_t(h) * a.chunks + s.c0) * kQ;
+  const int64_t xcol = int64_t(h) * P + p0, bcol = int64_t(h / (a.p.H / a.p.G)) * N;
+  Staged<DT, VEC, 64, kThreads> sx;
+  Staged<DT, VEC, W, kThreads> sb, sc;
+  double sv;
+  float uv;
+  auto tokens = [&](int k) { return s.n - k * kQ < kQ ? s.n - k * kQ : kQ; };
+  auto c_rows = [&](int k) {
+    return Rows<DT, VEC>(a.p.C, (s.t0 + int64_t(k) * kQ) * a.p.c_stride + bcol, a.p.c_stride, tokens(k), N);
+  };
+  auto fetch = [&](int k) {
+    const int64_t t = s.t0 + int64_t(k) * kQ;
+    sx.load(Rows<DT, VEC>(a.p.x, t * a.p.x_stride + xcol, a.p.x_stride, tokens(k), cols));
+    sb.load(Rows<DT, VEC>(a.p.B, t * a.p.b_stride + bcol, a.p.b_stride, tokens(k), N));
+    if (kCInLds) sc.load(c_rows(k));
+    sv = a.s[at + k * kQ + lane];
+    uv = a.u[at + k * kQ + lane];
+  };
+  fetch(0);
+  __syncthreads();  // odd is 0
+#pragma unroll 1
+  for (int k = 0; k < s.chunks; ++k) {
+    lw.refresh(), lx.refresh();
+    const int n = tokens(k);
+    sx.put(xt);
+    sb.put(bt);
+    if (kCInLds) sc.put(ct);
+    dec.put(wave, sv, uv);
+    if (sx.odd() != 0) odd[k & 1] = 1;
+    __syncthreads();
+    const bool bad = odd[k & 1] != 0;
     // rows i = 16 wave + li of M, as M^T[j][i] blocks: 4 neighbouring j a lane
     {
-      const int i = 16 * wave + li;
       f32x4 gm[4];
 #pragma unroll
       for (int jb = 0; jb < 4; ++jb) gm[jb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const Rows<DT, VEC> crow = c_rows(k);
 #pragma unroll
       for (int ks = 0; ks < 2 * NT; ++ks) {
-        const int col = 32 * ks + 8 * g;
-        const Frag<NP> cf = kCInLds ? ct.get8(i, col)
-                                    : load8<DT>(a.p.C, (t + i) * a.p.c_stride + group + col, i < n ? N - col : 0,
-                                                a.vec_c);
+        const Frag<NP> cf = kCInLds ? ct.get8(lw, wave, ks) : crow.get8(row, 32 * ks + 8 * g).frag();
 #pragma unroll
         for (int jb = 0; jb < 4; ++jb)
-          if (jb <= wave) gm[jb] = mm(bt.get8(16 * jb + li, col), cf, gm[jb]);
+          if (jb <= wave) gm[jb] = mm(bt.get8(lw, jb, ks), cf, gm[jb]);
       }
-      const double si = ss[i];
+      const float ai = dec.a[row];
 #pragma unroll
       for (int jb = 0; jb < 4; ++jb) {
         if (jb > wave) continue;
+        const f32x4 u = *reinterpret_cast<const f32x4*>(dec.u + 16 * jb + 4 * g);
         f32x4 v;
+        if (jb < wave) {
+          const float af = ai * dec.between(wave, jb);
+          const f32x4 b = *reinterpret_cast<const f32x4*>(dec.b + 16 * jb + 4 * g);
+          v = gm[jb] * ((af * b) * u);
+        } else {
+          const double si = dec.s[row];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int jj = 16 * jb + 4 * g + r;
-          v[r] = jj <= i ? gm[jb][r] * (__builtin_amdgcn_exp2f(static_cast<float>(si - ss[jj])) * us[jj]) : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            const float d = static_cast<float>(si - dec.s[16 * jb + 4 * g + r]);
+            v[r] = 4 * g + r <= li ? gm[jb][r] * (__builtin_amdgcn_exp2f(d) * u[r]) : 0.f;
+          }
         }
-        mt.put4(i, 16 * jb + 4 * g, v);
+        mt.put4(lx, wave, jb, v);
       }
     }
     if (w.kept != nullptr && !(k == 0 && from == nullptr))
-      store_state<NB, DT>(w.kept, (id * a.p.H + h) * P * N, p, P, N, g, a.vec_h, acc);
+      store_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + k) * a.p.H + h) * P + p0) * N, N, cols, N), row, acc);
+    if (k + 1 < s.chunks) fetch(k + 1);
     f32x4 ya[4];
 #pragma unroll
     for (int ib = 0; ib < 4; ++ib) ya[ib] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (active) {
       // h C: the state's registers are the operand, whose entry e of lane group g is state
       // 32 ks + 16 (e / 4) + 4 g + e % 4; C's entries are read in the same order
+      const Rows<DT, VEC> crow = c_rows(k);
 #pragma unroll
       for (int ks = 0; ks < 2 * NT; ++ks) {
         float f[8];
@@ -301,31 +352,24 @@ __global__ __launch_bounds__(kThreads) void forward_walk(Args a, Walk w, void* _
         const Frag<NP> hf = split<NP>(f);
 #pragma unroll
         for (int ib = 0; ib < 4; ++ib) {
-          const int i = 16 * ib + li, col = 32 * ks + 4 * g;
           Frag<NP> cf;
           if (kCInLds) {
-#pragma unroll
-            for (int q = 0; q < NP; ++q) {
-              const uint16_t* s = ct.p + q * ct.plane + i * NS + col;
-              cf.v[q] = __builtin_shufflevector(*reinterpret_cast<const s16x4*>(s),
-                                                *reinterpret_cast<const s16x4*>(s + 16), 0, 1, 2, 3, 4, 5, 6, 7);
-            }
+            cf = ct.get44(lw, ib, ks);
           } else {
-            const int64_t src = (t + i) * a.p.c_stride + group + col;
-            const f32x4 c_lo = load4<DT>(a.p.C, src, i < n ? N - col : 0, a.vec_c);
-            const f32x4 c_hi = load4<DT>(a.p.C, src + 16, i < n ? N - col - 16 : 0, a.vec_c);
-            const float cv[8] = {c_lo[0], c_lo[1], c_lo[2], c_lo[3], c_hi[0], c_hi[1], c_hi[2], c_hi[3]};
+            const f32x4 lo = crow.get4(16 * ib + li, 32 * ks + 4 * g), hi = crow.get4(16 * ib + li, 32 * ks + 16 + 4 * g);
+            const float cv[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             cf = split<NP>(cv);
           }
           ya[ib] = mm(hf, cf, ya[ib]);
         }
       }
 #pragma unroll
-      for (int ib = 0; ib < 4; ++ib) ya[ib] *= __builtin_amdgcn_exp2f(static_cast<float>(ss[16 * ib + li]));
+      for (int ib = 0; ib < 4; ++ib) ya[ib] *= dec.e[16 * ib + li];
     }
-    __syncthreads();  // M is whole
+    __syncthreads();  // M is whole, odd has been read
+    if (threadIdx.x == 0) odd[k & 1] = 0;
     if (active) {
-      const Frag<NP> xf[2] = {xt.tr8(0, 16 * wave, lane), xt.tr8(32, 16 * wave, lane)};
+      const Frag<NP> xf[2] = {xt.tr8(lx, 0, wave), xt.tr8(lx, 1, wave)};
       Frag<NP> xm[2] = {xf[0], xf[1]};
       if (bad) {
         // 0 x_j of a later token's infinity or NaN would reach the rows before it: those
@@ -338,34 +382,38 @@ __global__ __launch_bounds__(kThreads) void forward_walk(Args a, Walk w, void* _
 #pragma unroll
               for (int q = 0; q < NP; ++q) xm[ks].v[q][e] = 0;
       }
+      const Rows<DT, VEC> yrow(y, ((s.t0 + int64_t(k) * kQ) * a.p.H + h) * P + p0, a.p.H * P, n, cols);
 #pragma unroll
       for (int ib = 0; ib < 4; ++ib) {
-        const int i = 16 * ib + li;
-        ya[ib] = mm(xm[0], mt.get8(i, 8 * g), ya[ib]);
-        if (ib >= 2) ya[ib] = mm(xm[1], mt.get8(i, 32 + 8 * g), ya[ib]);
-        const f32x4 xi = xt.get4(i, 16 * wave + 4 * g);
+        ya[ib] = mm(xm[0], mt.get8(lx, ib, 0), ya[ib]);
+        if (ib >= 2) ya[ib] = mm(xm[1], mt.get8(lx, ib, 1), ya[ib]);
         if (bad) {
-          for (int jj = 0; jj <= i; ++jj) {
-            const f32x4 xj = xt.get4(jj, 16 * wave + 4 * g);
-            float mij = 0.f;
+          const int i = 16 * ib + li;
+          for (int jj = 0; jj <= i; ++jj)
 #pragma unroll
-            for (int q = 0; q < NP; ++q) mij += bf16_to_f32(mt.p[q * mt.plane + i * kRow + jj]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if ((__float_as_uint(xj[r]) & 0x7f800000u) == 0x7f800000u) ya[ib][r] += mij * xj[r];
-          }
+            for (int r = 0; r < 4; ++r) {
+              const float xj = xt.at(jj, 16 * wave + 4 * g + r);
+              if (!(fabsf(xj) < INFINITY)) ya[ib][r] += mt.at(i, jj) * xj;
+            }
         }
-        if (a.p.D != nullptr) ya[ib] += skip * xi;
-        if (i < n)
-          store4<DT>(y, ((t + i) * a.p.H + h) * P + p0 + 16 * wave + 4 * g, cols - 16 * wave - 4 * g, a.vec_y, ya[ib]);
+        if (a.p.D != nullptr) ya[ib] += skip * xt.get4(lx, ib, wave);
+        yrow.put4(16 * ib + li, 16 * wave + 4 * g, ya[ib]);
       }
-      const Frag<3> uf[2] = {weighted(xf[0], wj + 8 * g), weighted(xf[1], wj + 32 + 8 * g)};
-      update_state<NP, NB>(bt, uf, __builtin_amdgcn_exp2f(static_cast<float>(last)), lane, acc);
+      auto weights = [&](int t) { return dec.f + t; };
+      // (u f: the weights of the chunk's tokens in the state behind it)
+      Frag<3> uf[2];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        float wt[8] __attribute__((aligned(16)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wt[e] = weights(32 * ks + 8 * g)[e] * dec.u[32 * ks + 8 * g + e];
+        uf[ks] = weighted(xf[ks], wt);
+      }
+      update_state(bt, lw, uf, dec.e[kQ - 1], acc);
     }
     __syncthreads();  // the tiles are free
   }
-  if (t1 == hi && w.end != nullptr)
-    store_state<NB, DT_F32>(w.end, (m * a.p.H + h) * P * N, p, P, N, g, a.vec_h, acc);
+  if (s.last && w.end != nullptr) store_state<NB>(state(w.end, s.m), row, acc);
 }
 
 // ---------------------------------------------------------------------------
@@ -395,7 +443,14 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Scan p, float* __restric
     const bool live = c < P;
     const float x = live ? load_any(p.x, p.x_dt, b * p.x_stride + h * P + c) : 0.f;
     const int64_t at = (bh * P + c) * N + n;
-    f32x4 v = load4<DT_F32>(state, at, live ? N - n : 0, vec);
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
+    if (vec && live && n < N) {
+      v = *reinterpret_cast<const f32x4*>(state + at);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (live && n + k < N) v[k] = state[at + k];
+    }
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -404,7 +459,13 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Scan p, float* __restric
         s += v[k] * cv[k];
       }
     }
-    if (live) store4<DT_F32>(state, at, N - n, vec, v);
+    if (vec && live && n < N) {
+      *reinterpret_cast<f32x4*>(state + at) = v;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (live && n + k < N) state[at + k] = v[k];
+    }
 #pragma unroll
     for (int d = 1; d < LPR; d <<= 1) s += __shfl_xor(s, d);
     if (live && lane == 0) {
@@ -417,10 +478,14 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Scan p, float* __restric
 int n_tiles(int64_t N) { return N <= 64 ? 1 : (N <= 128 ? 2 : 4); }
 
 template <typename F>
-void with_types(const Scan& p, F&& f) {
-  const int nt = n_tiles(p.N);
+void with_types(const Args& a, F&& f) {
+  const int nt = n_tiles(a.p.N);
 #define MOC_SCAN_CASE(DT, NT) \
-  if (p.x_dt == DT && nt == NT) return f(std::integral_constant<int, DT>{}, std::integral_constant<int, NT>{});
+  if (a.p.x_dt == DT && nt == NT) { \
+    if (a.vec) f(std::integral_constant<int, DT>{}, std::integral_constant<int, NT>{}, std::true_type{}); \
+    else f(std::integral_constant<int, DT>{}, std::integral_constant<int, NT>{}, std::false_type{}); \
+    return; \
+  }
   MOC_SCAN_CASE(DT_BF16, 1) MOC_SCAN_CASE(DT_BF16, 2) MOC_SCAN_CASE(DT_BF16, 4)
   MOC_SCAN_CASE(DT_F32, 1) MOC_SCAN_CASE(DT_F32, 2) MOC_SCAN_CASE(DT_F32, 4)
 #undef MOC_SCAN_CASE
@@ -438,10 +503,9 @@ void allow_lds(K* kernel, size_t bytes) {
 
 template <bool REV, bool LOCAL>
 void run_walk(const Args& a, const Walk& w, hipStream_t st) {
-  with_types(a.p, [&](auto DT, auto NT) {
-    constexpr int np = kPlanes<DT.value>;
-    const size_t lds = size_t(np) * kQ * (64 * NT.value + 8 + kRow) * 2 + kQ * 4;
-    auto* k = state_walk<DT.value, NT.value, REV, LOCAL>;
+  with_types(a, [&](auto DT, auto NT, auto VEC) {
+    constexpr size_t lds = kWalkLds<DT.value, NT.value>;
+    auto* k = state_walk<DT.value, NT.value, VEC.value, REV, LOCAL>;
     allow_lds(k, lds);
     const dim3 grid(static_cast<unsigned>(pieces(a.seqs, a.seg)),
                     static_cast<unsigned>(a.p.H * ((a.p.P + kTile - 1) / kTile)));
@@ -483,11 +547,8 @@ Args make_args(const Scan& p, void* prep) {
   const size_t n = size_t(p.H) * a.chunks * kQ;
   a.u = static_cast<float*>(prep);
   a.s = reinterpret_cast<double*>(static_cast<char*>(prep) + up(n * 4));
-  a.vec_x = p.P % 8 == 0 && p.x_stride % 8 == 0 && aligned({p.x}, 16);
-  a.vec_b = p.N % 8 == 0 && p.b_stride % 8 == 0 && aligned({p.B}, 16);
-  a.vec_c = p.N % 8 == 0 && p.c_stride % 8 == 0 && aligned({p.C}, 16);
-  a.vec_h = p.N % 8 == 0;
-  a.vec_y = p.P % 4 == 0;
+  a.vec = p.P % 8 == 0 && p.N % 8 == 0 && aligned({p.x, p.B, p.C}, 16);
+  for (int64_t st : {p.x_stride, p.b_stride, p.c_stride, p.H * p.P}) a.vec = a.vec && st % 8 == 0 && st < kMaxStride;
   return a;
 }
 
@@ -542,26 +603,21 @@ void scan_forward(const Scan& p, void* y, const float* init, float* fin, void* s
                   hipStream_t st) {
   char* ws = static_cast<char*>(workspace);
   Args a = make_args(p, saved != nullptr ? saved : ws);
-  a.vec_y = a.vec_y && aligned({y}, 16);
-  a.vec_h = a.vec_h && aligned({init, fin}, 16);
+  a.vec = a.vec && aligned({y, init, fin, saved, workspace}, 16);
   Walk w{};
   w.x = p.x;
   w.b = p.B;
   w.x_stride = p.x_stride;
   w.b_stride = p.b_stride;
-  w.vec_x = a.vec_x;
-  w.vec_b = a.vec_b;
   w.start = init;
   w.end = fin;
   w.kept = saved != nullptr ? static_cast<char*>(saved) + prep_bytes(p) : nullptr;
   carve_walk(a, saved != nullptr ? ws : ws + prep_bytes(p), w);
   launch_prep(a, st);
   launch_segments(a, w, false, st);
-  with_types(p, [&](auto DT, auto NT) {
-    constexpr int np = kPlanes<DT.value>;
-    constexpr int wide = DT.value == DT_BF16 ? 2 : 1;  // B, and C where it is staged
-    const size_t lds = size_t(np) * kQ * (wide * (64 * NT.value + 8) + 2 * kRow) * 2 + kQ * 16;
-    auto* k = forward_walk<DT.value, NT.value>;
+  with_types(a, [&](auto DT, auto NT, auto VEC) {
+    constexpr size_t lds = kForwardLds<DT.value, NT.value>;
+    auto* k = forward_walk<DT.value, NT.value, VEC.value>;
     allow_lds(k, lds);
     const dim3 grid(static_cast<unsigned>(pieces(a.seqs, a.seg)),
                     static_cast<unsigned>(p.H * ((p.P + kTile - 1) / kTile)));

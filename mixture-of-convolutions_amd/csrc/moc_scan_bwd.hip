@@ -39,42 +39,89 @@ struct Back {
   float* part;          // [chunks][3 H]: dA, dD, ddt_bias
   float *dB_part, *dC_part;  // [subs][tokens][G][N] or null (one sub: dB, dC directly)
   int subs, per_sub;    // parts of a group's heads, heads of a part
-  bool vec_dy, vec_dx, vec_h;
 };
 
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
 // sum over lanes i % 16 (column sums of a result block)
-__device__ __forceinline__ float sum16(float v) {
+template <typename T>
+__device__ __forceinline__ T sum16(T v) {
 #pragma unroll
   for (int m = 1; m < 16; m <<= 1) v += __shfl_xor(v, m);
   return v;
 }
 // sum over lane groups (row sums)
-__device__ __forceinline__ float sum_groups(float v) {
+template <typename T>
+__device__ __forceinline__ T sum_groups(T v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
 }
-__device__ __forceinline__ float sum64(float v) { return sum_groups(sum16(v)); }
+template <typename T>
+__device__ __forceinline__ T sum64(T v) {
+  return sum_groups(sum16(v));
+}
 
+// sum of the products of two vectors' elements
+template <typename Acc>
+__device__ __forceinline__ Acc dot(const Raw<DT_BF16>& a, const Raw<DT_BF16>& b) {
+  Acc s = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s += lo_f(a.w[k]) * lo_f(b.w[k]) + hi_f(a.w[k]) * hi_f(b.w[k]);
+  return s;
+}
+template <typename Acc>
+__device__ __forceinline__ Acc dot(const Raw<DT_F32>& a, const Raw<DT_F32>& b) {
+  Acc s = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s += static_cast<Acc>(a.lo[k]) * b.lo[k] + static_cast<Acc>(a.hi[k]) * b.hi[k];
+  return s;
+}
+
+// LDS of backward_chunk.
 template <int DT, int NT>
-__global__ __launch_bounds__(kThreads, 2) void backward_chunk(Args a, Back b) {
-  constexpr int NP = kPlanes<DT>;
-  constexpr int kPlane = kQ * kRow, kTileBytes = NP * kPlane * 2;
-  extern __shared__ char smem[];
-  auto tile = [&](int k) { return Tile<NP>{reinterpret_cast<uint16_t*>(smem + k * kTileBytes), kRow, kPlane}; };
-  const Tile<NP> xt = tile(0), yt = tile(1), ht = tile(2), dt = tile(3), mt = tile(4);
-  double* ss = reinterpret_cast<double*>(smem + 5 * kTileBytes);
-  double* scan_s = ss + kQ;
-  float* us = reinterpret_cast<float*>(scan_s + kQ);
-  float* Kp = us + kQ;       // [4][64] column sums by row block
-  float* Rv = Kp + 4 * kQ;   // row sums
-  float* dg = Rv + kQ;       // diagonal
-  float* qp = dg + kQ;       // [4][64] q by state slice
-  float* gp = qp + 4 * kQ;   // [4][64] g by state slice
-  float* zp = gp + 4 * kQ;   // [4] z by wave, [4] <x, dy> by wave
+struct Layout {
+  static constexpr int NP = kPlanes<DT>;
+  // state tiles of 64 at a time: all of them and B's beside them (bf16), or one (three planes)
+  static constexpr int TW = DT == DT_BF16 ? NT : 1, W = 64 * TW;
+  static constexpr bool kBInLds = DT == DT_BF16;
+  using Acc = typename std::conditional<DT == DT_BF16, float, double>::type;
+  static constexpr int kSums = (4 + 2 + 4 + 4 + 1) * kQ;  // Acc values
+  static constexpr int kBytes = 3 * Tile<NP, 64>::kBytes + (kBInLds ? 3 : 2) * Tile<NP, W>::kBytes + Decays::kBytes +
+                                kSums * static_cast<int>(sizeof(Acc));
+  // waves a SIMD: two workgroups of 8 waves a CU where LDS holds them
+  static constexpr int kWaves = 2;
+};
+
+constexpr int kHalves = 2;
+constexpr int kBack = 256 * kHalves;  // threads of backward_chunk
+
+// Wave w: row / channel / state slice w % 4, and of the column blocks of a result (tokens
+// 16 q.., 16 jb..) those of parity w / 4.  For fp32 the sums that da is formed from are
+// kept in 64 bits (Acc): da is one number for a whole chunk to a large part (z, and the
+// sums over the tokens behind), so that its rounding does not average out over tokens.
+template <int DT, int NT, bool VEC>
+__global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chunk(Args a, Back b) {
+  using LY = Layout<DT, NT>;
+  using Acc = typename LY::Acc;
+  constexpr int NP = LY::NP, TW = LY::TW, W = LY::W, Q = 4 / kHalves;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int kT = Tile<NP, 64>::kBytes, kS = Tile<NP, W>::kBytes;
+  const Tile<NP, 64> xt{reinterpret_cast<uint16_t*>(smem)}, yt{reinterpret_cast<uint16_t*>(smem + kT)},
+      mt{reinterpret_cast<uint16_t*>(smem + 2 * kT)};
+  const Tile<NP, W> ht{reinterpret_cast<uint16_t*>(smem + 3 * kT)}, dt{reinterpret_cast<uint16_t*>(smem + 3 * kT + kS)},
+      bt{reinterpret_cast<uint16_t*>(smem + 3 * kT + 2 * kS)};
+  char* rest = smem + 3 * kT + (LY::kBInLds ? 3 : 2) * kS;
+  const Decays dec(rest);
+  Acc* Kp = reinterpret_cast<Acc*>(rest + Decays::kBytes);  // [4][64] column sums by row block
+  Acc* Rv = Kp + 4 * kQ;                                    // [2][64] row sums by half
+  Acc* qp = Rv + 2 * kQ;                                    // [4][64] q by state slice
+  Acc* gp = qp + 4 * kQ;                                    // [4][64] g by channel slice
+  Acc* dg = gp + 4 * kQ;                                    // [64] the diagonal
+  __shared__ Acc zp[2][4 * kHalves];                        // z, <x, dy> by wave
+  Lane<64> lx;
+  Lane<W> lw;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wid & 3, half = wid >> 2;
   const int H = static_cast<int>(a.p.H), P = static_cast<int>(a.p.P), G = static_cast<int>(a.p.G),
             N = static_cast<int>(a.p.N);
   const int grp = blockIdx.y / b.subs, sub = blockIdx.y % b.subs, hpg = H / G;
@@ -83,227 +130,260 @@ __global__ __launch_bounds__(kThreads, 2) void backward_chunk(Args a, Back b) {
   Chunk c;
   if (!chunk_at(a, blockIdx.x, c)) {
     // no such chunk: its rows of the sums over chunks are 0
-    for (int k = threadIdx.x; k < 3 * (h_hi - h_lo); k += kThreads)
+    for (int k = threadIdx.x; k < 3 * (h_hi - h_lo); k += kBack)
       b.part[int64_t(blockIdx.x) * 3 * H + (k % 3) * H + h_lo + k / 3] = 0.f;
     return;
   }
-  const int n = c.n;
+  const int n = c.n, ptiles = (P + kTile - 1) / kTile, ntiles = (N + 63) / 64;
   const bool use_h = !c.first || b.has_init, use_dh = !c.last || b.has_dfin;
   const int64_t gcol = int64_t(grp) * N;
+  const Rows<DT, VEC> brow(a.p.B, c.t0 * a.p.b_stride + gcol, a.p.b_stride, n, N);
+  const Rows<DT, VEC> crow(a.p.C, c.t0 * a.p.c_stride + gcol, a.p.c_stride, n, N);
   const int i = 16 * wave + li;  // this lane's row i of G, V (result column)
+  auto blk = [&](int k) { return k * kHalves + half; };  // this wave's column blocks
+
+  // the loads of a head's (and channel tile's) tensors, ahead of their use
+  Staged<DT, VEC, 64, kBack> sx, sy;
+  Staged<DT, VEC, W, kBack> sh, sd;
+  double sv = 0.0;
+  float uv = 0.f;
+  auto fetch_states = [&](int h, int pt, int nt) {
+    const int p0 = pt * kTile, cols = P - p0 < kTile ? P - p0 : kTile, n0 = nt * 64;
+    const int64_t at = ((c.id * H + h) * P + p0) * N + n0;
+    const int width = N - n0 < W ? N - n0 : W;
+    sh.load(Rows<DT, VEC>(b.h, at, N, use_h ? cols : 0, width));
+    sd.load(Rows<DT, VEC>(b.dh, at, N, use_dh ? cols : 0, width));
+  };
+  auto fetch = [&](int h, int pt) {
+    const int p0 = pt * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
+    sx.load(Rows<DT, VEC>(a.p.x, c.t0 * a.p.x_stride + int64_t(h) * P + p0, a.p.x_stride, n, cols));
+    sy.load(Rows<DT, VEC>(b.dy, (c.t0 * H + h) * P + p0, int64_t(H) * P, n, cols));
+    fetch_states(h, pt, 0);
+    const int64_t at = (int64_t(h) * a.chunks + c.id) * kQ + lane;
+    if (pt == 0) sv = a.s[at], uv = a.u[at];
+  };
+  fetch(h_lo, 0);
 
   // G^T blocks [j][i] of row block `wave`
-  f32x4 gm[4], ds[4];
+  f32x4 gm[Q], ds[Q];
 #pragma unroll
-  for (int jb = 0; jb < 4; ++jb) gm[jb] = ds[jb] = zero4();
+  for (int k = 0; k < Q; ++k) gm[k] = ds[k] = zero4();
+  if (LY::kBInLds) {
+    Staged<DT, VEC, W, kBack> sb;
+    sb.load(brow);
+    sb.put(bt);
+  }
 #pragma unroll
   for (int ks = 0; ks < 2 * NT; ++ks) {
-    const int col = 32 * ks + 8 * g;
-    const Frag<NP> cf = load8<DT>(a.p.C, (c.t0 + i) * a.p.c_stride + gcol + col, i < n ? N - col : 0, a.vec_c);
+    const Frag<NP> cf = crow.get8(i, 32 * ks + 8 * g).frag();
 #pragma unroll
-    for (int jb = 0; jb < 4; ++jb) {
-      if (jb > wave) continue;
-      const int j = 16 * jb + li;
-      gm[jb] = mm(load8<DT>(a.p.B, (c.t0 + j) * a.p.b_stride + gcol + col, j < n ? N - col : 0, a.vec_b), cf, gm[jb]);
-    }
+    for (int k = 0; k < Q; ++k)
+      if (blk(k) <= wave) gm[k] = mm(brow.get8(16 * blk(k) + li, 32 * ks + 8 * g).frag(), cf, gm[k]);
   }
-  // dB^T, dC^T blocks: states 64 nt + 16 wave + 4 g + r, tokens 16 q + li
-  f32x4 dBa[NT][4], dCa[NT][4];
+  // the block right of the diagonal that a 32-token product step reads (no other wave writes it)
+  if ((wave & 1) == 0 && half == (wave + 1) % kHalves) mt.put4(lx, wave, wave + 1, zero4());
+  // dB^T, dC^T blocks: states 64 nt + 16 wave + 4 g + r, tokens 16 blk + li
+  f32x4 dBa[NT][Q], dCa[NT][Q];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) dBa[nt][q] = dCa[nt][q] = zero4();
-  const int ptiles = (P + kTile - 1) / kTile;
+    for (int k = 0; k < Q; ++k) dBa[nt][k] = dCa[nt][k] = zero4();
 
+#pragma unroll 1
   for (int h = h_lo; h < h_hi; ++h) {
-    const int64_t at = (int64_t(h) * a.chunks + c.id) * kQ;
     const float skip = a.p.D == nullptr ? 0.f : load_any(a.p.D, a.p.d_dt, h);
-    __syncthreads();  // (the last head's readers are done)
-    if (threadIdx.x < kQ) {
-      ss[threadIdx.x] = a.s[at + threadIdx.x];
-      us[threadIdx.x] = a.u[at + threadIdx.x];
+    Acc qa[Q], ga[Q], ka[Q][4], ra = 0, da = 0, za = 0, xy = 0;
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+      qa[k] = ga[k] = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ka[k][r] = 0;
     }
-    float qa[4] = {0.f, 0.f, 0.f, 0.f}, ga[4] = {0.f, 0.f, 0.f, 0.f}, ka[4][4], ra = 0.f, da = 0.f;
-#pragma unroll
-    for (int jb = 0; jb < 4; ++jb)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) ka[jb][r] = 0.f;
-    float za = 0.f, xy = 0.f;
+#pragma unroll 1
     for (int pt = 0; pt < ptiles; ++pt) {
+      lx.refresh(), lw.refresh();
       const int p0 = pt * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
-      if (pt > 0) __syncthreads();
+      if (pt > 0) __syncthreads();  // (the last tile's readers; a head's last barrier is behind them too)
+      if (a.p.D != nullptr) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int w = threadIdx.x + k * kThreads, row = w >> 3, col = (w & 7) * 8;
-        const int valid = row < n ? cols - col : 0;
-        const Frag<NP> fx = load8<DT>(a.p.x, (c.t0 + row) * a.p.x_stride + int64_t(h) * P + p0 + col, valid, a.vec_x);
-        const Frag<NP> fy = load8<DT>(b.dy, ((c.t0 + row) * H + h) * P + p0 + col, valid, b.vec_dy);
-        float vx[8], vy[8];
-        join(fx, vx);
-        join(fy, vy);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) xy += vx[e] * vy[e];
-        xt.put8(row, col, fx);
-        yt.put8(row, col, fy);
+        for (int k = 0; k < sx.kLoads; ++k) xy += dot<Acc>(sx.v[k], sy.v[k]);
       }
+      if (pt == 0) dec.put(wave, sv, uv);  // (both halves write the same)
+      sx.put(xt);
+      sy.put(yt);
+      auto put_states = [&]() {
+        if (use_h && use_dh) {
+#pragma unroll
+          for (int k = 0; k < sh.kLoads; ++k) za += dot<Acc>(sh.v[k], sd.v[k]);
+        }
+        if (use_h) sh.put(ht);
+        if (use_dh) sd.put(dt);
+      };
+      put_states();
       __syncthreads();
       // V^T, then W and what of it goes where
-      f32x4 vm[4];
+      {
+        f32x4 vm[Q];
 #pragma unroll
-      for (int jb = 0; jb < 4; ++jb) vm[jb] = zero4();
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const Frag<NP> yf = yt.get8(i, 32 * ks + 8 * g);
-#pragma unroll
-        for (int jb = 0; jb < 4; ++jb)
-          if (jb <= wave) vm[jb] = mm(xt.get8(16 * jb + li, 32 * ks + 8 * g), yf, vm[jb]);
-      }
-      const double si = ss[i];
-#pragma unroll
-      for (int jb = 0; jb < 4; ++jb) {
-        if (jb > wave) continue;
-        f32x4 gl;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = 16 * jb + 4 * g + r;
-          const float L = j <= i ? __builtin_amdgcn_exp2f(static_cast<float>(si - ss[j])) : 0.f;
-          const float u = us[j];
-          gl[r] = j <= i ? gm[jb][r] * L : 0.f;
-          const float wv = j <= i ? gl[r] * vm[jb][r] : 0.f;
-          ds[jb][r] += j <= i ? vm[jb][r] * (L * u) : 0.f;
-          if (j == i) {
-            da += wv;
-          } else {
-            ka[jb][r] += wv;
-            ra += u * wv;
-          }
-        }
-        if (pt == 0) mt.put4(i, 16 * jb + 4 * g, gl);
-      }
-      if (pt == 0 && (wave & 1) == 0) mt.put4(i, 16 * wave + 16 + 4 * g, zero4());
-      __syncthreads();
-      // dx^T[p][j]: channels p0 + 16 wave + 4 g + r, tokens 16 q + li
-      const bool active = 16 * wave < cols;
-      f32x4 x1[4], x2[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) x1[q] = x2[q] = zero4();
-      if (active) {
+        for (int k = 0; k < Q; ++k) vm[k] = zero4();
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          const Frag<NP> yf = yt.tr8(32 * ks, 16 * wave, lane);
+          const Frag<NP> yf = yt.get8(lx, wave, ks);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (32 * ks + 31 >= 16 * q) x1[q] = mm(yf, mt.tr8(32 * ks, 16 * q, lane), x1[q]);
+          for (int k = 0; k < Q; ++k)
+            if (blk(k) <= wave) vm[k] = mm(xt.get8(lx, blk(k), ks), yf, vm[k]);
+        }
+        const float ai = dec.a[i];
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+          const int jb = blk(k);
+          if (jb > wave) continue;
+          const f32x4 u = *reinterpret_cast<const f32x4*>(dec.u + 16 * jb + 4 * g);
+          f32x4 L;
+          if (jb < wave) {
+            L = (ai * dec.between(wave, jb)) * *reinterpret_cast<const f32x4*>(dec.b + 16 * jb + 4 * g);
+          } else {
+            const double si = dec.s[i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              L[r] = __builtin_amdgcn_exp2f(static_cast<float>(si - dec.s[16 * jb + 4 * g + r]));
+          }
+          f32x4 gl = gm[k] * L, vl = vm[k] * (L * u);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool in = jb < wave || 4 * g + r <= li, diag = jb == wave && 4 * g + r == li;
+            gl[r] = in ? gl[r] : 0.f;
+            vl[r] = in ? vl[r] : 0.f;
+            const float wv = in ? gl[r] * vm[k][r] : 0.f;
+            if (diag) {
+              da += wv;
+            } else {
+              ka[k][r] += wv;
+              ra += static_cast<Acc>(u[r]) * wv;
+            }
+          }
+          ds[k] += vl;
+          if (pt == 0) mt.put4(lx, wave, jb, gl);
         }
       }
-      if (use_h || use_dh) {
+      const bool active = 16 * wave < cols;
+      // dx^T[p][j]: channels p0 + 16 wave + 4 g + r, tokens 16 blk + li; the state's part first
+      f32x4 xa[Q];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (nt * 64 >= N) continue;
+      for (int k = 0; k < Q; ++k) xa[k] = zero4();
+#pragma unroll
+      for (int nt0 = 0; nt0 < NT; nt0 += TW) {
+        if (nt0 >= ntiles) continue;
+        if (nt0 > 0) {
           __syncthreads();  // (the last state tile's readers)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int w = threadIdx.x + k * kThreads, row = w >> 3, col = nt * 64 + (w & 7) * 8;
-            const int valid = row < cols ? N - col : 0;
-            const int64_t src = ((c.id * H + h) * P + p0 + row) * N + col;
-            const Frag<NP> fh = load8<DT>(b.h, src, use_h ? valid : 0, b.vec_h);
-            const Frag<NP> fd = load8<DT>(b.dh, src, use_dh ? valid : 0, b.vec_h);
-            float vh[8], vd[8];
-            join(fh, vh);
-            join(fd, vd);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) za += vh[e] * vd[e];
-            ht.put8(row, (w & 7) * 8, fh);
-            dt.put8(row, (w & 7) * 8, fd);
-          }
+          put_states();
           __syncthreads();
-          if (active && use_dh) {
+        }
+        if (nt0 + TW < ntiles) {
+          fetch_states(h, pt, nt0 + TW);
+        } else if (pt + 1 < ptiles) {
+          fetch(h, pt + 1);
+        } else if (h + 1 < h_hi) {
+          fetch(h + 1, 0);
+        }
+        if (active && use_dh) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              const int col = nt * 64 + 32 * ks + 8 * g;
-              const Frag<NP> df = dt.get8(16 * wave + li, 32 * ks + 8 * g);
+          for (int ks = 0; ks < 2 * TW; ++ks) {
+            const Frag<NP> df = dt.get8(lw, wave, ks);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int j = 16 * q + li;
-                x2[q] = mm(df, load8<DT>(a.p.B, (c.t0 + j) * a.p.b_stride + gcol + col, j < n ? N - col : 0, a.vec_b),
-                           x2[q]);
-              }
+            for (int k = 0; k < Q; ++k) {
+              const Frag<NP> bf = LY::kBInLds
+                                      ? bt.get8(lw, blk(k), ks)
+                                      : brow.get8(16 * blk(k) + li, 64 * nt0 + 32 * ks + 8 * g).frag();
+              xa[k] = mm(df, bf, xa[k]);
             }
           }
-          // states 64 nt + 16 wave + ...: h^T dy and dh^T x
-          const int sc = nt * 64 + 16 * wave + 4 * g;
-          if (nt * 64 + 16 * wave < N) {
-            Frag<NP> hf[2], df[2];
+        }
+        // states 64 nt + 16 wave + ...: h^T dy and dh^T x
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              hf[ks] = ht.tr8(32 * ks, 16 * wave, lane);
-              df[ks] = dt.tr8(32 * ks, 16 * wave, lane);
+        for (int tw = 0; tw < TW; ++tw) {
+          const int nt = nt0 + tw;
+          if (64 * nt + 16 * wave >= N) continue;
+          if (use_h) {
+            const Frag<NP> h0 = ht.tr8(lw, 0, 4 * tw + wave), h1 = ht.tr8(lw, 1, 4 * tw + wave);
+#pragma unroll
+            for (int k = 0; k < Q; ++k) {
+              const f32x4 v = mm(h1, yt.get8(lx, blk(k), 1), mm(h0, yt.get8(lx, blk(k), 0), zero4()));
+              const f32x4 cv = crow.get4(16 * blk(k) + li, 64 * nt + 16 * wave + 4 * g);
+              dCa[nt][k] += dec.e[16 * blk(k) + li] * v;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) qa[k] += static_cast<Acc>(v[r]) * cv[r];
             }
+          }
+          if (use_dh) {
+            const Frag<NP> d0 = dt.tr8(lw, 0, 4 * tw + wave), d1 = dt.tr8(lw, 1, 4 * tw + wave);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int t = 16 * q + li;
-              const float st = static_cast<float>(ss[t]);
-              if (use_h) {
-                f32x4 v = mm(hf[0], yt.get8(t, 8 * g), zero4());
-                v = mm(hf[1], yt.get8(t, 32 + 8 * g), v);
-                v *= __builtin_amdgcn_exp2f(st);
-                dCa[nt][q] += v;
-                const f32x4 cv = load4<DT>(a.p.C, (c.t0 + t) * a.p.c_stride + gcol + sc, t < n ? N - sc : 0, a.vec_c);
-                qa[q] += v[0] * cv[0] + v[1] * cv[1] + v[2] * cv[2] + v[3] * cv[3];
-              }
-              if (use_dh) {
-                f32x4 v = mm(df[0], xt.get8(t, 8 * g), zero4());
-                v = mm(df[1], xt.get8(t, 32 + 8 * g), v);
-                v *= __builtin_amdgcn_exp2f(static_cast<float>(ss[kQ - 1] - ss[t]));
-                dBa[nt][q] += v * us[t];
-                const f32x4 bv = load4<DT>(a.p.B, (c.t0 + t) * a.p.b_stride + gcol + sc, t < n ? N - sc : 0, a.vec_b);
-                ga[q] += v[0] * bv[0] + v[1] * bv[1] + v[2] * bv[2] + v[3] * bv[3];
-              }
+            for (int k = 0; k < Q; ++k) {
+              const f32x4 v = mm(d1, xt.get8(lx, blk(k), 1), mm(d0, xt.get8(lx, blk(k), 0), zero4()));
+              dBa[nt][k] += (dec.f[16 * blk(k) + li] * dec.u[16 * blk(k) + li]) * v;
             }
           }
         }
       }
-      if (active && b.dx != nullptr) {
+      if (active && use_dh) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int j = 16 * q + li;
-          const float f = __builtin_amdgcn_exp2f(static_cast<float>(ss[kQ - 1] - ss[j]));
-          f32x4 v = us[j] * (x1[q] + f * x2[q]);
-          if (a.p.D != nullptr) v += skip * yt.get4(j, 16 * wave + 4 * g);
-          if (j < n)
-            store4<DT>(b.dx, ((c.t0 + j) * H + h) * P + p0 + 16 * wave + 4 * g, cols - 16 * wave - 4 * g, b.vec_dx, v);
+        for (int k = 0; k < Q; ++k) {
+          const f32x4 xv = xt.get4(lx, blk(k), wave);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ga[k] += static_cast<Acc>(xv[r]) * xa[k][r];
+          xa[k] *= dec.f[16 * blk(k) + li];
+        }
+      }
+      __syncthreads();  // M is whole
+      if (active) {
+        const Rows<DT, VEC> out(b.dx, (c.t0 * H + h) * P + p0, int64_t(H) * P, n, cols);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const Frag<NP> yf = yt.tr8(lx, ks, wave);
+#pragma unroll
+          for (int k = 0; k < Q; ++k)
+            if (32 * ks + 31 >= 16 * blk(k)) xa[k] = mm(yf, mt.tr8(lx, ks, blk(k)), xa[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+          const int j = 16 * blk(k) + li;
+          f32x4 v = dec.u[j] * xa[k];
+          if (a.p.D != nullptr) v += skip * yt.get4(lx, blk(k), wave);
+          out.put4(j, 16 * wave + 4 * g, v);
         }
       }
     }
     // the head's sums over channels and states
 #pragma unroll
-    for (int jb = 0; jb < 4; ++jb)
+    for (int k = 0; k < Q; ++k) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float v = sum16(ka[jb][r]);
-        if (li == 0) Kp[wave * kQ + 16 * jb + 4 * g + r] = v;
+        const Acc v = sum16(ka[k][r]);
+        if (li == 0) Kp[wave * kQ + 16 * blk(k) + 4 * g + r] = v;
       }
+      const Acc v = sum_groups(qa[k]), v2 = sum_groups(ga[k]);
+      if (g == 0) qp[wave * kQ + 16 * blk(k) + li] = v, gp[wave * kQ + 16 * blk(k) + li] = v2;
+    }
     ra = sum_groups(ra);
     da = sum_groups(da);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float v = sum_groups(qa[q]), v2 = sum_groups(ga[q]);
-      if (g == 0) qp[wave * kQ + 16 * q + li] = v, gp[wave * kQ + 16 * q + li] = v2;
+    if (g == 0) {
+      Rv[half * kQ + i] = ra;
+      if (half == wave % kHalves) dg[i] = da;
     }
-    if (g == 0) Rv[i] = ra, dg[i] = da;
     za = sum64(za);
     xy = sum64(xy);
-    if (lane == 0) zp[wave] = za, zp[4 + wave] = xy;
-    __syncthreads();
-    if (wave == 0) {
+    if (lane == 0) zp[0][wid] = za, zp[1][wid] = xy;
+    const float u = dec.u[lane], e = dec.e[lane], f = dec.f[lane], e_last = dec.e[kQ - 1];
+    __syncthreads();  // the sums are whole, every tile and factor has been read
+    if (wid == 0) {
       const int t = lane;
-      const float K = (Kp[t] + Kp[kQ + t]) + (Kp[2 * kQ + t] + Kp[3 * kQ + t]);
-      const float q = (qp[t] + qp[kQ + t]) + (qp[2 * kQ + t] + qp[3 * kQ + t]);
-      const float gt = (gp[t] + gp[kQ + t]) + (gp[2 * kQ + t] + gp[3 * kQ + t]);
-      const float u = us[t];
-      const float z = ((zp[0] + zp[1]) + (zp[2] + zp[3])) * __builtin_amdgcn_exp2f(static_cast<float>(ss[kQ - 1]));
+      auto four = [&](const Acc* p) { return (p[t] + p[kQ + t]) + (p[2 * kQ + t] + p[3 * kQ + t]); };
+      const Acc K = four(Kp), q = e * four(qp), gt = f * four(gp);
+      Acc z = 0, xd = 0;
+#pragma unroll
+      for (int k = 0; k < 4 * kHalves; ++k) z += zp[0][k], xd += zp[1][k];
       // suffix sums of one part, prefix sums (before t) of the other, in 64 bits
-      double suf = static_cast<double>(Rv[t]) - static_cast<double>(u) * K + q;
+      double suf = static_cast<double>(Rv[t] + Rv[kQ + t]) - static_cast<double>(u) * K + q;
       double pre = static_cast<double>(u) * gt;
       const double own = pre;
 #pragma unroll
@@ -312,63 +392,56 @@ __global__ __launch_bounds__(kThreads, 2) void backward_chunk(Args a, Back b) {
         if (t + d < 64) suf += o;
         if (t >= d) pre += o2;
       }
-      const float dat = static_cast<float>(suf + (pre - own) + z);
-      const float A = load_any(a.p.A, a.p.a_dt, h);
-      float du = K + dg[t] + gt + A * dat;
+      const double dat = suf + (pre - own) + static_cast<double>(z) * e_last;
+      double du = K + dg[t] + gt + load_any(a.p.A, a.p.a_dt, h) * dat;
       if (a.p.softplus) du *= -expm1f(-u);
       const bool real = t < n;
-      if (real && b.ddt != nullptr) store_any(b.ddt, DT, (c.t0 + t) * H + h, du);
-      const float sA = sum64(real ? u * dat : 0.f), sb = sum64(real ? du : 0.f);
+      if (real) store_any(b.ddt, DT, (c.t0 + t) * H + h, static_cast<float>(du));
+      const double sA = sum64(real ? u * dat : 0.0), sb = sum64(real ? du : 0.0);
       if (lane == 0) {
         float* out = b.part + int64_t(blockIdx.x) * 3 * H + h;
-        out[0] = sA;
-        out[H] = (zp[4] + zp[5]) + (zp[6] + zp[7]);
-        out[2 * H] = sb;
+        out[0] = static_cast<float>(sA);
+        out[H] = static_cast<float>(xd);
+        out[2 * H] = static_cast<float>(sb);
       }
     }
   }
   // what the chunk's own tokens give of dB and dC, summed over the heads
-  __syncthreads();
 #pragma unroll
-  for (int jb = 0; jb < 4; ++jb)
-    if (jb <= wave) mt.put4(i, 16 * jb + 4 * g, ds[jb]);
-  if ((wave & 1) == 0) mt.put4(i, 16 * wave + 16 + 4 * g, zero4());
+  for (int k = 0; k < Q; ++k)
+    if (blk(k) <= wave) mt.put4(lx, wave, blk(k), ds[k]);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    if (nt * 64 >= N) continue;
+    if (nt >= ntiles) continue;
+    lx.refresh();
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int w = threadIdx.x + k * kThreads, row = w >> 3, col = nt * 64 + (w & 7) * 8;
-      const int valid = row < n ? N - col : 0;
-      xt.put8(row, (w & 7) * 8, load8<DT>(a.p.B, (c.t0 + row) * a.p.b_stride + gcol + col, valid, a.vec_b));
-      yt.put8(row, (w & 7) * 8, load8<DT>(a.p.C, (c.t0 + row) * a.p.c_stride + gcol + col, valid, a.vec_c));
-    }
+    sx.load(Rows<DT, VEC>(a.p.B, c.t0 * a.p.b_stride + gcol + 64 * nt, a.p.b_stride, n, N - 64 * nt));
+    sy.load(Rows<DT, VEC>(a.p.C, c.t0 * a.p.c_stride + gcol + 64 * nt, a.p.c_stride, n, N - 64 * nt));
+    sx.put(xt);
+    sy.put(yt);
     __syncthreads();
-    const int sc = nt * 64 + 16 * wave + 4 * g;
-    if (nt * 64 + 16 * wave >= N) continue;
+    const int sc = 64 * nt + 16 * wave;
+    if (sc >= N) continue;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const Frag<NP> bf = xt.tr8(32 * ks, 16 * wave, lane), cf = yt.tr8(32 * ks, 16 * wave, lane);
+      const Frag<NP> bf = xt.tr8(lx, ks, wave), cf = yt.tr8(lx, ks, wave);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int k = 0; k < Q; ++k) {
         // dC_i: j <= i; dB_j: i >= j
-        if (32 * ks < 16 * q + 16) dCa[nt][q] = mm(bf, mt.get8(16 * q + li, 32 * ks + 8 * g), dCa[nt][q]);
-        if (32 * ks + 31 >= 16 * q) dBa[nt][q] = mm(cf, mt.tr8(32 * ks, 16 * q, lane), dBa[nt][q]);
+        if (32 * ks < 16 * blk(k) + 16) dCa[nt][k] = mm(bf, mt.get8(lx, blk(k), ks), dCa[nt][k]);
+        if (32 * ks + 31 >= 16 * blk(k)) dBa[nt][k] = mm(cf, mt.tr8(lx, ks, blk(k)), dBa[nt][k]);
       }
     }
+    const int64_t at = (c.t0 * G + grp) * N, all = a.p.seq.n_tokens * int64_t(G) * N * sub;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int t = 16 * q + li;
-      if (t >= n) continue;
-      const int64_t dst = ((c.t0 + t) * G + grp) * N + sc;
+    for (int k = 0; k < Q; ++k) {
+      const int t = 16 * blk(k) + li;
       if (b.subs == 1) {
-        store4<DT>(b.dB, dst, N - sc, b.vec_h, dBa[nt][q]);
-        store4<DT>(b.dC, dst, N - sc, b.vec_h, dCa[nt][q]);
+        Rows<DT, VEC>(b.dB, at, int64_t(G) * N, n, N).put4(t, sc + 4 * g, dBa[nt][k]);
+        Rows<DT, VEC>(b.dC, at, int64_t(G) * N, n, N).put4(t, sc + 4 * g, dCa[nt][k]);
       } else {
-        const int64_t all = a.p.seq.n_tokens * int64_t(G) * N;
-        store4<DT_F32>(b.dB_part, sub * all + dst, N - sc, b.vec_h, dBa[nt][q]);
-        store4<DT_F32>(b.dC_part, sub * all + dst, N - sc, b.vec_h, dCa[nt][q]);
+        Rows<DT_F32, VEC>(b.dB_part, all + at, int64_t(G) * N, n, N).put4(t, sc + 4 * g, dBa[nt][k]);
+        Rows<DT_F32, VEC>(b.dC_part, all + at, int64_t(G) * N, n, N).put4(t, sc + 4 * g, dCa[nt][k]);
       }
     }
   }
@@ -423,14 +496,12 @@ void scan_backward(const Scan& p, const void* dy, bool has_init, const float* df
   Args a = make_args(p, const_cast<void*>(saved));
   const Bytes n = bytes_of(a);
   char* ws = static_cast<char*>(workspace);
-  a.vec_h = a.vec_h && aligned({dfin, g.dinit}, 16);
+  a.vec = a.vec && aligned({dy, dfin, saved, workspace, g.dx, g.dB, g.dC, g.dinit}, 16);
   Walk w{};
   w.x = dy;
   w.b = p.C;
   w.x_stride = p.H * p.P;
   w.b_stride = p.c_stride;
-  w.vec_x = p.P % 8 == 0 && aligned({dy}, 16);
-  w.vec_b = a.vec_c;
   w.start = dfin;
   w.end = g.dinit;
   w.kept = ws + n.walk;
@@ -454,25 +525,25 @@ void scan_backward(const Scan& p, const void* dy, bool has_init, const float* df
   b.per_sub = static_cast<int>((hpg + b.subs - 1) / b.subs);
   b.dB_part = reinterpret_cast<float*>(ws + n.walk + n.dh + n.part);
   b.dC_part = reinterpret_cast<float*>(ws + n.walk + n.dh + n.part + n.sub);
-  b.vec_dy = w.vec_x;
-  b.vec_dx = p.P % 4 == 0 && aligned({g.dx}, 16);
-  b.vec_h = p.N % 8 == 0 && aligned({g.dB, g.dC}, 16);
-  auto go = [&](auto DT, auto NT) {
-    constexpr int np = kPlanes<DT.value>;
-    const size_t lds = size_t(np) * 5 * kQ * kRow * 2 + kQ * (2 * 8 + 15 * 4) + 64;
-    auto* k = backward_chunk<DT.value, NT.value>;
+  auto go = [&](auto DT, auto NT, auto VEC) {
+    constexpr size_t lds = Layout<DT.value, NT.value>::kBytes;
+    auto* k = backward_chunk<DT.value, NT.value, VEC.value>;
     if (lds > 65536)
       (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize,
                                 static_cast<int>(lds));
-    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.G * b.subs)), dim3(kThreads),
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.G * b.subs)), dim3(kBack),
                        static_cast<unsigned>(lds), st, a, b);
   };
   using BF = std::integral_constant<int, DT_BF16>;
   using F = std::integral_constant<int, DT_F32>;
   auto nt = [&](auto DT) {
-    if (p.N <= 64) go(DT, std::integral_constant<int, 1>{});
-    else if (p.N <= 128) go(DT, std::integral_constant<int, 2>{});
-    else go(DT, std::integral_constant<int, 4>{});
+    auto with = [&](auto NT) {
+      if (a.vec) go(DT, NT, std::true_type{});
+      else go(DT, NT, std::false_type{});
+    };
+    if (p.N <= 64) with(std::integral_constant<int, 1>{});
+    else if (p.N <= 128) with(std::integral_constant<int, 2>{});
+    else with(std::integral_constant<int, 4>{});
   };
   if (p.x_dt == DT_BF16) nt(BF{});
   else nt(F{});
