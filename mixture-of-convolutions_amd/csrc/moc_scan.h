@@ -48,11 +48,6 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
 // c + a . b.  The products of the lower planes are summed by themselves and added
 // once: each addition to c costs a rounding at c's size.
 __device__ __forceinline__ f32x4 mm(const Frag<1>& a, const Frag<1>& b, f32x4 c) { return mfma(a.v[0], b.v[0], c); }
-__device__ __forceinline__ f32x4 mm(const Frag<1>& a, const Frag<3>& b, f32x4 c) {
-  f32x4 t = mfma(a.v[0], b.v[2], f32x4{0.f, 0.f, 0.f, 0.f});
-  t = mfma(a.v[0], b.v[1], t);
-  return mfma(a.v[0], b.v[0], c) + t;
-}
 __device__ __forceinline__ f32x4 mm(const Frag<3>& a, const Frag<3>& b, f32x4 c) {
   f32x4 t = mfma(a.v[0], b.v[2], f32x4{0.f, 0.f, 0.f, 0.f});
   t = mfma(a.v[1], b.v[1], t);
@@ -60,6 +55,19 @@ __device__ __forceinline__ f32x4 mm(const Frag<3>& a, const Frag<3>& b, f32x4 c)
   t = mfma(a.v[0], b.v[1], t);
   t = mfma(a.v[1], b.v[0], t);
   return mfma(a.v[0], b.v[0], c) + t;
+}
+
+// a0 . b0 + a1 . b1 with b in three planes, the low planes first
+__device__ __forceinline__ f32x4 mm2(const Frag<1>& a0, const Frag<1>& a1, const Frag<3>& b0, const Frag<3>& b1) {
+  f32x4 c = mfma(a0.v[0], b0.v[2], f32x4{0.f, 0.f, 0.f, 0.f});
+  c = mfma(a1.v[0], b1.v[2], c);
+  c = mfma(a0.v[0], b0.v[1], c);
+  c = mfma(a1.v[0], b1.v[1], c);
+  c = mfma(a0.v[0], b0.v[0], c);
+  return mfma(a1.v[0], b1.v[0], c);
+}
+__device__ __forceinline__ f32x4 mm2(const Frag<3>& a0, const Frag<3>& a1, const Frag<3>& b0, const Frag<3>& b1) {
+  return mm(a1, b1, mm(a0, b0, f32x4{0.f, 0.f, 0.f, 0.f}));
 }
 
 // Two fp32 rounded to bf16 in one dword, a in the low half (v_cvt_pk_bf16_f32).
@@ -145,9 +153,11 @@ struct Raw<DT_F32> {
 
 // Rows (tokens, or channels of a state) of a tensor from one of them on: element
 // (row, col) lies at base + row * stride + col; rows from n on and columns from `cols` on
-// read as 0.  VEC: column counts and strides are multiples of 8 and base is aligned to 16
-// bytes: reads go through a buffer resource, whose range check makes the zeros (an offset
-// no range reaches stands for what is not there), without a branch.
+// read as 0 and are not written.  VEC: column counts and strides are multiples of 8 and
+// base is aligned to 16 bytes: accesses go through a buffer resource that ends behind row
+// n - 1, whose range check makes the zeros without a branch (a lane whose columns are not
+// there has an offset that no range reaches), and a lane's offset is the same for every
+// chunk of a walk.
 constexpr uint32_t kNowhere = 0x80000000u;
 constexpr int64_t kMaxStride = int64_t(1) << 22;  // VEC: 64 rows stay below kNowhere
 
@@ -157,26 +167,30 @@ struct Rows {
   const char* base;
   int64_t stride;
   int n, cols;
-  __amdgpu_buffer_rsrc_t r;
   __device__ __forceinline__ Rows(const void* p, int64_t at, int64_t stride_, int n_, int cols_)
-      : base(static_cast<const char*>(p) + at * E), stride(stride_), n(n_), cols(cols_) {
-    if constexpr (VEC) r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00020000);
+      : base(static_cast<const char*>(p) + at * E), stride(stride_), n(n_), cols(cols_) {}
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
+    const int bytes = n > 0 ? ((n - 1) * static_cast<int>(stride) + cols) * E : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00020000);
   }
-  __device__ __forceinline__ uint32_t off(int row, int col) const {
+  __device__ __forceinline__ int off(int row, int col) const {
     const uint32_t o = static_cast<uint32_t>(row * static_cast<int>(stride) + col) * E;
-    return row < n && col < cols ? o : kNowhere;
+    return static_cast<int>(col < cols ? o : kNowhere);
   }
-  __device__ __forceinline__ Raw<DT> get8(int row, int col) const {
+  // (row + more, col), `more` the same for every lane
+  __device__ __forceinline__ Raw<DT> get8(int row, int col, int more = 0) const {
     Raw<DT> v;
     if constexpr (VEC) {
-      const int o = static_cast<int>(off(row, col));
+      const int o = off(row, col), s = more * static_cast<int>(stride) * E;
+      const auto r = rsrc();
       if constexpr (DT == DT_BF16) {
-        v.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+        v.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, s, 0));
       } else {
-        v.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
-        v.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 16, 0));
+        v.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, s, 0));
+        v.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o + 16, s, 0));
       }
     } else {
+      row += more;
       const int have = row < n ? cols - col : 0;
       const int64_t at = row * stride + col;
       if constexpr (DT == DT_BF16) {
@@ -201,12 +215,12 @@ struct Rows {
   __device__ __forceinline__ f32x4 get4(int row, int col) const {
     f32x4 v;
     if constexpr (VEC) {
-      const int o = static_cast<int>(off(row, col));
+      const int o = off(row, col);
       if constexpr (DT == DT_BF16) {
-        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc(), o, 0, 0));
         v = f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
       } else {
-        v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+        v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), o, 0, 0));
       }
     } else {
       const int have = row < n ? cols - col : 0;
@@ -217,12 +231,12 @@ struct Rows {
   }
   __device__ __forceinline__ void put4(int row, int col, f32x4 v) const {
     if constexpr (VEC) {
-      const int o = static_cast<int>(off(row, col));
+      const int o = off(row, col);
       if constexpr (DT == DT_BF16) {
         const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
-        __builtin_amdgcn_raw_buffer_store_b64(w, r, o, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b64(w, rsrc(), o, 0, 0);
       } else {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, o, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rsrc(), o, 0, 0);
       }
     } else {
       const int have = row < n ? cols - col : 0;
@@ -346,7 +360,7 @@ struct Staged {
   Raw<DT> v[kLoads];
   __device__ __forceinline__ void load(const Rows<DT, VEC>& src) {
 #pragma unroll
-    for (int k = 0; k < kLoads; ++k) v[k] = src.get8(row(k), col(k));
+    for (int k = 0; k < kLoads; ++k) v[k] = src.get8(row(0), col(k), k * (THREADS / (W / 8)));
   }
   template <int NP>
   __device__ __forceinline__ void put(const Tile<NP, W>& t) const {
@@ -372,16 +386,18 @@ struct Decays {
   float* b;    // exp(its block's end - s)
   float* e;    // exp(s)
   float* f;    // exp(s_last - s)
+  float* w;    // u f: a token's weight in the state behind the chunk
   float* u;
   double* s;
-  static constexpr int kBytes = kQ * (5 * 4 + 8);
+  static constexpr int kBytes = kQ * (6 * 4 + 8);
   __device__ __forceinline__ explicit Decays(char* p) {
     s = reinterpret_cast<double*>(p);
     a = reinterpret_cast<float*>(s + kQ);
     b = a + kQ;
     e = b + kQ;
     f = e + kQ;
-    u = f + kQ;
+    w = f + kQ;
+    u = w + kQ;
   }
   // every wave: lane t with token t's u and s; wave w makes a part of them
   __device__ __forceinline__ void put(int wave, double sv, float uv) const {
@@ -397,7 +413,9 @@ struct Decays {
       e[t] = ex(sv);
       u[t] = uv;
     } else {
-      f[t] = ex(__shfl(sv, 63) - sv);
+      const float fv = ex(__shfl(sv, 63) - sv);
+      f[t] = fv;
+      w[t] = uv * fv;
     }
   }
   // exp(start of block ib - end of block jb), jb < ib
@@ -484,7 +502,7 @@ __device__ __forceinline__ bool chunk_at(const Args& a, int64_t id, Chunk& c) {
 Args make_args(const Scan& p, void* prep);
 size_t prep_bytes(const Scan& p);
 // tokens of a segment: see moc_scan.hip
-int64_t segment(const Scan& p, bool backward);
+int64_t segment(const Scan& p);
 void launch_prep(const Args& a, hipStream_t st);
 
 // Walks of the state over a sequence's chunks (moc_scan.hip).  rev == false: the state

@@ -95,8 +95,7 @@ __device__ __forceinline__ void update_state(const Tile<NP, W>& bt, const Lane<W
   for (int nb = 0; nb < NB; ++nb) {
     const Frag<NP> c0 = b0, c1 = b1;
     if (nb + 1 < NB) b0 = bt.tr8(l, 0, nb + 1), b1 = bt.tr8(l, 1, nb + 1);
-    const f32x4 v = mm(c1, uf[1], mm(c0, uf[0], f32x4{0.f, 0.f, 0.f, 0.f}));
-    acc[nb] = acc[nb] * decay + v;
+    acc[nb] = acc[nb] * decay + mm2(c0, c1, uf[0], uf[1]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -373,7 +372,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
       Frag<NP> xm[2] = {xf[0], xf[1]};
       if (bad) {
         // 0 x_j of a later token's infinity or NaN would reach the rows before it: those
-        // products are left out here and made one by one below
+        // products are left out here and added to y one by one below
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -387,28 +386,27 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
       for (int ib = 0; ib < 4; ++ib) {
         ya[ib] = mm(xm[0], mt.get8(lx, ib, 0), ya[ib]);
         if (ib >= 2) ya[ib] = mm(xm[1], mt.get8(lx, ib, 1), ya[ib]);
-        if (bad) {
-          const int i = 16 * ib + li;
+        // (without D skip is 0: no branch between a product and the first use of its result,
+        // whose wait states the compiler has been seen to leave out on the path around a body)
+        ya[ib] += skip * xt.get4(lx, ib, wave);
+        yrow.put4(16 * ib + li, 16 * wave + 4 * g, ya[ib]);
+      }
+      if (bad) {
+#pragma unroll 1
+        for (int ib = 0; ib < 4; ++ib) {
+          const int i = 16 * ib + li, col = 16 * wave + 4 * g;
+          f32x4 v = yrow.get4(i, col);
+#pragma unroll 1
           for (int jj = 0; jj <= i; ++jj)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float xj = xt.at(jj, 16 * wave + 4 * g + r);
-              if (!(fabsf(xj) < INFINITY)) ya[ib][r] += mt.at(i, jj) * xj;
+              const float xj = xt.at(jj, col + r);
+              if (!(fabsf(xj) < INFINITY)) v[r] += mt.at(i, jj) * xj;
             }
+          yrow.put4(i, col, v);
         }
-        if (a.p.D != nullptr) ya[ib] += skip * xt.get4(lx, ib, wave);
-        yrow.put4(16 * ib + li, 16 * wave + 4 * g, ya[ib]);
       }
-      auto weights = [&](int t) { return dec.f + t; };
-      // (u f: the weights of the chunk's tokens in the state behind it)
-      Frag<3> uf[2];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        float wt[8] __attribute__((aligned(16)));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) wt[e] = weights(32 * ks + 8 * g)[e] * dec.u[32 * ks + 8 * g + e];
-        uf[ks] = weighted(xf[ks], wt);
-      }
+      const Frag<3> uf[2] = {weighted(xf[0], dec.w + 8 * g), weighted(xf[1], dec.w + 32 + 8 * g)};
       update_state(bt, lw, uf, dec.e[kQ - 1], acc);
     }
     __syncthreads();  // the tiles are free
@@ -523,13 +521,20 @@ size_t prep_bytes(const Scan& p) {
   return up(n * 4) + up(n * 8);
 }
 
-// Segments: a walk's workgroups are heads x segments, and about 1024 of them (four a CU)
-// fill the card; a segment has 256 tokens at least, as every one but the last is
-// walked twice.
-int64_t segment(const Scan& p, bool) {
+// Segments: a walk's workgroups are heads x segments, and 768 of them are on the card at
+// a time (three a CU, what registers and LDS allow): one round of them, as a second one
+// would run with the card part empty.  A segment has 256 tokens at least, as every one but
+// the last is walked twice.
+int64_t segment(const Scan& p) {
   const int64_t n = p.seq.n_tokens, heads = p.H * ((p.P + kTile - 1) / kTile);
   const int64_t longest = p.seq.cu == nullptr ? p.seq.seq_len : n;
-  const int64_t want = (1024 + heads - 1) / heads;  // segments of the whole token axis
+  int64_t want = 768 / heads;  // segments of the whole token axis
+  if (want < 1) want = 1;
+  if (p.seq.cu == nullptr) {  // the same number in every sequence
+    want /= n / longest;
+    if (want < 1) want = 1;
+    want *= n / longest;
+  }
   int64_t seg = (n + want - 1) / want;
   seg = (seg + kQ - 1) / kQ * kQ;
   if (seg < 256) seg = 256;
@@ -543,7 +548,7 @@ Args make_args(const Scan& p, void* prep) {
   a.seqs.l = p.seq;
   a.seqs.count = p.seq.cu == nullptr ? p.seq.n_tokens / p.seq.seq_len : p.seq.n_seqs + 2;
   a.chunks = pieces(a.seqs, kQ);
-  a.seg = segment(p, false);
+  a.seg = segment(p);
   const size_t n = size_t(p.H) * a.chunks * kQ;
   a.u = static_cast<float*>(prep);
   a.s = reinterpret_cast<double*>(static_cast<char*>(prep) + up(n * 4));
