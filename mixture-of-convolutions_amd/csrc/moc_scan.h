@@ -70,6 +70,14 @@ __device__ __forceinline__ f32x4 mm2(const Frag<3>& a0, const Frag<3>& a1, const
   return mm(a1, b1, mm(a0, b0, f32x4{0.f, 0.f, 0.f, 0.f}));
 }
 
+// Wait states between products made in a branch and the first use of their results behind
+// it: the compiler has been seen to leave them out on a path around a branch's body.
+__device__ __forceinline__ void settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 7");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // Two fp32 rounded to bf16 in one dword, a in the low half (v_cvt_pk_bf16_f32).
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

@@ -22,6 +22,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
+template <int V>
+using Int = std::integral_constant<int, V>;
+
 // ---------------------------------------------------------------------------
 // u and s of every chunk and head.  Lanes are tokens for the running sum (in 64 bits:
 // s_i - s_j is formed from it, where a 32-bit sum of tens would lose the differences of
@@ -299,40 +302,50 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
     if (sx.odd() != 0) odd[k & 1] = 1;
     __syncthreads();
     const bool bad = odd[k & 1] != 0;
-    // rows i = 16 wave + li of M, as M^T[j][i] blocks: 4 neighbouring j a lane
-    {
-      f32x4 gm[4];
+    // blocks of M, as M^T[j][i]: 4 neighbouring j a lane.  The ten on and below the diagonal
+    // are 2, 2, 3 and 3 a wave; a wave's own code each, so that no branch parts its reads
+    const Rows<DT, VEC> crow = c_rows(k);
+    auto m_blocks = [&](auto... pair) {
+      constexpr int kPairs = sizeof...(pair);
+      constexpr int ib[] = {pair.value / 4 ...}, jb[] = {pair.value % 4 ...};
+      f32x4 gm[kPairs];
 #pragma unroll
-      for (int jb = 0; jb < 4; ++jb) gm[jb] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const Rows<DT, VEC> crow = c_rows(k);
+      for (int q = 0; q < kPairs; ++q) gm[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < 2 * NT; ++ks) {
-        const Frag<NP> cf = kCInLds ? ct.get8(lw, wave, ks) : crow.get8(row, 32 * ks + 8 * g).frag();
+        Frag<NP> cf;
 #pragma unroll
-        for (int jb = 0; jb < 4; ++jb)
-          if (jb <= wave) gm[jb] = mm(bt.get8(lw, jb, ks), cf, gm[jb]);
+        for (int q = 0; q < kPairs; ++q) {
+          if (q == 0 || ib[q] != ib[q > 0 ? q - 1 : 0])
+            cf = kCInLds ? ct.get8(lw, ib[q], ks) : crow.get8(li, 32 * ks + 8 * g, 16 * ib[q]).frag();
+          gm[q] = mm(bt.get8(lw, jb[q], ks), cf, gm[q]);
+        }
       }
-      const float ai = dec.a[row];
 #pragma unroll
-      for (int jb = 0; jb < 4; ++jb) {
-        if (jb > wave) continue;
-        const f32x4 u = *reinterpret_cast<const f32x4*>(dec.u + 16 * jb + 4 * g);
+      for (int q = 0; q < kPairs; ++q) {
+        const f32x4 u = *reinterpret_cast<const f32x4*>(dec.u + 16 * jb[q] + 4 * g);
         f32x4 v;
-        if (jb < wave) {
-          const float af = ai * dec.between(wave, jb);
-          const f32x4 b = *reinterpret_cast<const f32x4*>(dec.b + 16 * jb + 4 * g);
-          v = gm[jb] * ((af * b) * u);
+        if (jb[q] < ib[q]) {
+          const float af = dec.a[16 * ib[q] + li] * dec.between(ib[q], jb[q]);
+          const f32x4 b = *reinterpret_cast<const f32x4*>(dec.b + 16 * jb[q] + 4 * g);
+          v = gm[q] * ((af * b) * u);
         } else {
-          const double si = dec.s[row];
+          const double si = dec.s[16 * ib[q] + li];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float d = static_cast<float>(si - dec.s[16 * jb + 4 * g + r]);
-            v[r] = 4 * g + r <= li ? gm[jb][r] * (__builtin_amdgcn_exp2f(d) * u[r]) : 0.f;
+            const float e = __builtin_amdgcn_exp2f(static_cast<float>(si - dec.s[16 * jb[q] + 4 * g + r])) * u[r];
+            const float m = gm[q][r] * e;
+            v[r] = 4 * g + r <= li ? m : 0.f;
           }
         }
-        mt.put4(lx, wave, jb, v);
+        mt.put4(lx, ib[q], jb[q], v);
       }
-    }
+    };
+    // (a pair is 4 i + j, in blocks)
+    if (wave == 0) m_blocks(Int<0>{}, Int<12>{});
+    else if (wave == 1) m_blocks(Int<4>{}, Int<5>{});
+    else if (wave == 2) m_blocks(Int<8>{}, Int<9>{}, Int<10>{});
+    else m_blocks(Int<13>{}, Int<14>{}, Int<15>{});
     if (w.kept != nullptr && !(k == 0 && from == nullptr))
       store_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + k) * a.p.H + h) * P + p0) * N, N, cols, N), row, acc);
     if (k + 1 < s.chunks) fetch(k + 1);
@@ -342,7 +355,6 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
     if (active) {
       // h C: the state's registers are the operand, whose entry e of lane group g is state
       // 32 ks + 16 (e / 4) + 4 g + e % 4; C's entries are read in the same order
-      const Rows<DT, VEC> crow = c_rows(k);
 #pragma unroll
       for (int ks = 0; ks < 2 * NT; ++ks) {
         float f[8];

@@ -233,6 +233,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
           for (int k = 0; k < Q; ++k)
             if (blk(k) <= wave) vm[k] = mm(xt.get8(lx, blk(k), ks), yf, vm[k]);
         }
+        settle();
         const float ai = dec.a[i];
 #pragma unroll
         for (int k = 0; k < Q; ++k) {
@@ -344,6 +345,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
           for (int k = 0; k < Q; ++k)
             if (32 * ks + 31 >= 16 * blk(k)) xa[k] = mm(yf, mt.tr8(lx, ks, blk(k)), xa[k]);
         }
+        settle();
 #pragma unroll
         for (int k = 0; k < Q; ++k) {
           const int j = 16 * blk(k) + li;
@@ -432,6 +434,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
         if (32 * ks + 31 >= 16 * blk(k)) dBa[nt][k] = mm(cf, mt.tr8(lx, ks, blk(k)), dBa[nt][k]);
       }
     }
+    settle();
     const int64_t at = (c.t0 * G + grp) * N, all = a.p.seq.n_tokens * int64_t(G) * N * sub;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
