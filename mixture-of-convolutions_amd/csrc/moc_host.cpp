@@ -51,7 +51,7 @@ bool unwatched() {
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
-    if (t != nullptr && t->requires_grad()) return true;
+    if (t != nullptr && t->defined() && t->requires_grad()) return true;
   return false;
 }
 
@@ -366,6 +366,352 @@ std::optional<std::tuple<Tensor, OptTensor>> stateful(const Tensor& x, const Ten
   return std::make_tuple(y, want ? OptTensor(fin) : OptTensor());
 }
 
+// ---------------------------------------------------------------------------
+// The operators next to the layers (moc/blocks.py), each as one call: with gradients
+// as a node, else straight.  Us a call, Python functions -> here, in blocks.py.
+
+// a parameter's storage code (any floating dtype that the kernels read), or -1
+int param_code(const Tensor& t) {
+  if (!t.defined()) return 0;
+  return t.scalar_type() == at::kHalf ? 2 : dtype_code(t.scalar_type());
+}
+
+// A parameter of the operators: absent, or plain, on x's device, of the shape and readable.
+bool param_ok(const Tensor& t, const Tensor& x, at::IntArrayRef shape) {
+  return !t.defined() || (plain(t) && t.device() == x.device() && t.sizes() == shape && param_code(t) >= 0);
+}
+
+Tensor like(const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : Tensor(); }
+Tensor f32(at::IntArrayRef shape, const Tensor& x) { return at::empty(shape, x.options().dtype(at::kFloat)); }
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// (a node takes what may be absent as an optional: an undefined tensor is no input of it)
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor dense(const OptTensor& t) { return t.has_value() ? t->contiguous() : Tensor(); }
+
+// Which of a node's tensor inputs need a gradient; edges are counted over those present.
+struct Needs {
+  AutogradContext* ctx;
+  size_t edge = 0;
+  bool operator()(bool present) { return present && ctx->needs_input_grad(edge++); }
+};
+
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// The packed offsets, as the library takes them; false where they are not ones it takes.
+bool offsets_ok(const OptTensor& cu, const Tensor& x) {
+  return !cu.has_value() ||
+         (plain(*cu) && cu->device() == x.device() && cu->dim() == 1 && cu->numel() >= 2 &&
+          (cu->scalar_type() == at::kInt || cu->scalar_type() == at::kLong));
+}
+
+struct Packing {
+  Tensor cu;
+  int64_t tokens, seq_len;
+  const void* p() const { return ptr(cu); }
+  int i64() const { return cu.defined() && cu.scalar_type() == at::kLong; }
+  int64_t n_seqs() const { return cu.defined() ? cu.numel() - 1 : 0; }
+};
+
+// --- layer norm
+
+struct NormFn : public torch::autograd::Function<NormFn> {
+  static Tensor run(const Tensor& x, const Tensor& w, const Tensor& b, double eps, Tensor* mean, Tensor* rstd) {
+    const int64_t D = x.size(-1), rows = x.numel() / D;
+    Tensor y = at::empty_like(x);
+    if (mean != nullptr) {
+      const Tensor both = f32({2, rows}, x);
+      *mean = both.select(0, 0);
+      *rstd = both.select(0, 1);
+    }
+    check(moc_norm_forward(ptr(x), ptr(w), ptr(b), ptr(y), static_cast<float*>(mean ? ptr(*mean) : nullptr),
+                           static_cast<float*>(rstd ? ptr(*rstd) : nullptr), rows, D, dtype_code(x.scalar_type()),
+                           param_code(w), param_code(b), static_cast<float>(eps), stream_of(x)),
+          "moc_norm_forward");
+    return y;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x0, const OptTensor& w0, const OptTensor& b0, double eps) {
+    const Tensor x = x0.contiguous(), w = dense(w0), b = dense(b0);
+    Tensor mean, rstd;
+    Tensor y = run(x, w, b, eps, &mean, &rstd);
+    ctx->save_for_backward({x, w, b, mean, rstd});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+    variable_list out(4);
+    {
+      at::NoGradGuard ng;
+      const c10::DeviceGuard dg(x.device());
+      const Tensor dy = grads[0].to(x.scalar_type()).contiguous();
+      const int64_t D = x.size(-1), rows = x.numel() / D;
+      Needs need{ctx};
+      if (need(true)) out[0] = at::empty_like(x);
+      if (need(w.defined())) out[1] = like(w);
+      if (need(b.defined())) out[2] = like(b);
+      const bool sums = out[1].defined() || out[2].defined();
+      const size_t n = sums ? moc_norm_backward_workspace_bytes(rows, D) : 0;
+      const Tensor ws = sums ? bytes(n, x) : Tensor();
+      check(moc_norm_backward(ptr(x), ptr(w), ptr(dy), static_cast<float*>(ptr(saved[3])),
+                              static_cast<float*>(ptr(saved[4])), ptr(out[0]), ptr(out[1]), ptr(out[2]), rows, D,
+                              dtype_code(x.scalar_type()), param_code(w), param_code(b), ptr(ws), n, stream_of(x)),
+            "moc_norm_backward");
+    }
+    return at::GradMode::is_enabled() ? once(std::move(out), grads) : out;
+  }
+};
+
+OptTensor norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+  if (!unwatched() || !plain(x) || dtype_code(x.scalar_type()) < 0 || x.dim() < 1 || x.numel() == 0)
+    return std::nullopt;
+  if (!param_ok(w, x, {x.size(-1)}) || !param_ok(b, x, {x.size(-1)})) return std::nullopt;
+  const c10::DeviceGuard dg(x.device());
+  if (wants_grad({&x, &w, &b})) return NormFn::apply(x, opt(w), opt(b), eps);
+  at::NoGradGuard ng;
+  return NormFn::run(x.contiguous(), dense(w), dense(b), eps, nullptr, nullptr);
+}
+
+// --- causal convolution
+
+struct ConvFn : public torch::autograd::Function<ConvFn> {
+  static Tensor run(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& cache, Tensor* fin, int act,
+                    const Packing& k) {
+    Tensor y = at::empty_like(x);
+    check(moc_conv_forward(ptr(x), ptr(w), ptr(b), ptr(cache), ptr(y), fin ? ptr(*fin) : nullptr, k.p(), k.i64(),
+                           k.n_seqs(), k.tokens, k.seq_len, w.size(1), w.size(0), dtype_code(x.scalar_type()),
+                           param_code(w), param_code(b), act, stream_of(x)),
+          "moc_conv_forward");
+    return y;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x0, const Tensor& w0, const OptTensor& b0, int64_t act,
+                        const Packing* k) {
+    const Tensor x = x0.contiguous(), w = dense(w0), b = dense(b0);
+    Tensor y = run(x, w, b, Tensor(), nullptr, static_cast<int>(act), *k);
+    ctx->save_for_backward({x, w, b, k->cu});
+    ctx->saved_data["k"] = std::vector<int64_t>{act, k->tokens, k->seq_len};
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+    const auto v = ctx->saved_data["k"].toIntVector();
+    const Packing k{saved[3], v[1], v[2]};
+    variable_list out(5);
+    {
+      at::NoGradGuard ng;
+      const c10::DeviceGuard dg(x.device());
+      const Tensor dy = grads[0].to(x.scalar_type()).contiguous();
+      Needs need{ctx};
+      if (need(true)) out[0] = at::empty_like(x);
+      if (need(true)) out[1] = like(w);
+      if (need(b.defined())) out[2] = like(b);
+      const bool sums = out[1].defined() || out[2].defined();
+      const size_t n = sums ? moc_conv_backward_workspace_bytes(k.tokens, w.size(1), w.size(0)) : 0;
+      const Tensor ws = sums ? bytes(n, x) : Tensor();
+      check(moc_conv_backward(ptr(x), ptr(w), ptr(b), ptr(dy), ptr(out[0]), ptr(out[1]), ptr(out[2]), k.p(), k.i64(),
+                              k.n_seqs(), k.tokens, k.seq_len, w.size(1), w.size(0), dtype_code(x.scalar_type()),
+                              param_code(w), param_code(b), static_cast<int>(v[0]), ptr(ws), n, stream_of(x)),
+            "moc_conv_backward");
+    }
+    return at::GradMode::is_enabled() ? once(std::move(out), grads) : out;
+  }
+};
+
+// (y, state or None) of a fixed-length [B, T, D] or packed [N, D] x.  Nothing also where
+// gradients flow with a cache or a final state (blocks.py puts those together).
+std::optional<std::tuple<Tensor, OptTensor>> conv(const Tensor& x, const Tensor& w, const Tensor& b,
+                                                  const OptTensor& cache, int act, bool want, const OptTensor& cu) {
+  if (!unwatched() || !plain(x) || dtype_code(x.scalar_type()) < 0 || !w.defined() || w.dim() != 2) return std::nullopt;
+  const int64_t S = w.size(0), D = w.size(1);
+  if (x.dim() != (cu.has_value() ? 2 : 3) || x.size(-1) != D || x.numel() == 0 || S < 1 || S > 16) return std::nullopt;
+  if (!param_ok(w, x, {S, D}) || !param_ok(b, x, {D}) || !offsets_ok(cu, x)) return std::nullopt;
+  if (cu.has_value() && (cache.has_value() || want)) return std::nullopt;
+  if (cache.has_value() && (!plain(*cache) || cache->device() != x.device() || cache->scalar_type() != x.scalar_type() ||
+                            cache->sizes() != at::IntArrayRef({x.size(0), D, S})))
+    return std::nullopt;
+  const c10::DeviceGuard dg(x.device());
+  const Packing k{cu.has_value() ? cu->contiguous() : Tensor(), x.numel() / D, cu.has_value() ? 0 : x.size(1)};
+  if (cache.has_value() && x.size(1) == 1) {
+    for (int64_t i = 0; i < 3; ++i)
+      if (cache->size(i) > 1 && cache->stride(i) == 0) return std::nullopt;
+    at::NoGradGuard ng;
+    const Tensor xc = x.contiguous(), wc = dense(w), bc = dense(b);
+    Tensor y = at::empty_like(xc);
+    check(moc_conv_update(ptr(xc), ptr(wc), ptr(bc), ptr(*cache), cache->stride(0), cache->stride(1), cache->stride(2),
+                          ptr(y), x.size(0), D, S, dtype_code(x.scalar_type()), param_code(w), param_code(b), act,
+                          stream_of(x)),
+          "moc_conv_update");
+    written(*cache);
+    return std::make_tuple(y, want ? cache : OptTensor());
+  }
+  if (wants_grad({&x, &w, &b, cache.has_value() ? &*cache : nullptr})) {
+    if (cache.has_value() || want) return std::nullopt;
+    return std::make_tuple(ConvFn::apply(x, w, opt(b), static_cast<int64_t>(act), &k), OptTensor());
+  }
+  at::NoGradGuard ng;
+  Tensor fin = want ? at::empty({x.size(0), D, S}, x.options()) : Tensor();
+  Tensor y = ConvFn::run(x.contiguous(), dense(w), dense(b), cache.has_value() ? cache->contiguous() : Tensor(),
+                         want ? &fin : nullptr, act, k);
+  return std::make_tuple(y, want ? OptTensor(fin) : OptTensor());
+}
+
+// --- selective scan
+
+// ops.token_rows: t itself where a token's `inner` dimensions are contiguous and tokens
+// evenly apart, a copy otherwise
+Tensor token_rows(const Tensor& t, int64_t inner, int64_t& step) {
+  const int64_t lead = t.dim() - inner;
+  int64_t n = 1;
+  bool ok = true;
+  for (int64_t i = t.dim() - 1; i >= lead; --i) {
+    ok = ok && (t.size(i) == 1 || t.stride(i) == n);
+    n *= t.size(i);
+  }
+  step = n;
+  bool any = false;
+  for (int64_t i = lead - 1; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (!any) step = t.stride(i);
+    else ok = ok && t.stride(i) == t.size(lead - 1) * step;
+    any = true;
+  }
+  if (ok && step >= n) return t;
+  step = n;
+  return t.contiguous();
+}
+
+// The inputs of a scan and the library's table of them.
+struct ScanCall {
+  Tensor x, dt, A, B, C, D, bias;
+  Packing k;
+  int softplus;
+  MocScan table() {
+    MocScan t{};
+    x = token_rows(x, 2, t.x_stride);
+    dt = token_rows(dt, 1, t.dt_stride);
+    B = token_rows(B, 2, t.b_stride);
+    C = token_rows(C, 2, t.c_stride);
+    A = dense(A), D = dense(D), bias = dense(bias);
+    t.x = ptr(x), t.dt = ptr(dt), t.a = ptr(A), t.b = ptr(B), t.c = ptr(C), t.d = ptr(D), t.dt_bias = ptr(bias);
+    t.cu_seqlens = k.p(), t.cu_seqlens_i64 = k.i64(), t.n_seqs = k.n_seqs();
+    t.n_tokens = k.tokens, t.seq_len = k.seq_len;
+    t.heads = x.size(-2), t.head_dim = x.size(-1), t.groups = B.size(-2), t.state_dim = B.size(-1);
+    t.x_dtype = dtype_code(x.scalar_type()), t.a_dtype = param_code(A), t.d_dtype = param_code(D);
+    t.bias_dtype = param_code(bias), t.dt_softplus = softplus;
+    return t;
+  }
+  // (y, final state); saved: what the backward reads
+  Tensor run(const Tensor& init, Tensor* fin, Tensor* saved) {
+    const MocScan t = table();
+    Tensor y = at::empty(x.sizes(), x.options());
+    const auto size = [](size_t n) {
+      TORCH_CHECK(n > 0 || moc_last_error()[0] == 0, "moc_scan_forward: ", moc_last_error());
+      return n;
+    };
+    if (fin != nullptr) *fin = f32({x.size(0), t.heads, t.head_dim, t.state_dim}, x);
+    if (saved != nullptr) *saved = bytes(size(moc_scan_saved_bytes(&t)), x);
+    const Tensor ws = bytes(size(moc_scan_forward_workspace_bytes(&t, saved != nullptr)), x);
+    check(moc_scan_forward(&t, ptr(y), static_cast<float*>(ptr(init)), static_cast<float*>(fin ? ptr(*fin) : nullptr),
+                           saved ? ptr(*saved) : nullptr, saved ? saved->numel() : 0, ptr(ws), ws.numel(),
+                           stream_of(x)),
+          "moc_scan_forward");
+    return y;
+  }
+};
+
+struct ScanFn : public torch::autograd::Function<ScanFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B,
+                               const Tensor& C, const OptTensor& D, const OptTensor& bias, const OptTensor& cache,
+                               int64_t softplus, bool want, const Packing* k) {
+    ScanCall c{x, dt, A, B, C, dense(D), dense(bias), *k, static_cast<int>(softplus)};
+    Tensor fin, saved;
+    const Tensor init = dense(cache);
+    Tensor y = c.run(init, want ? &fin : nullptr, &saved);
+    ctx->save_for_backward({c.x, c.dt, c.A, c.B, c.C, c.D, c.bias, saved, k->cu});
+    ctx->saved_data["k"] = std::vector<int64_t>{softplus, init.defined(), k->tokens, k->seq_len};
+    ctx->set_materialize_grads(false);
+    if (want) return {y, fin};
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto v = ctx->saved_data["k"].toIntVector();
+    ScanCall c{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], Packing{saved[8], v[2], v[3]},
+               static_cast<int>(v[0])};
+    variable_list out(11);
+    const Tensor &dy0 = grads[0], dfin0 = grads.size() > 1 ? grads[1] : Tensor();
+    if (!dy0.defined() && !dfin0.defined()) return out;
+    {
+      at::NoGradGuard ng;
+      const c10::DeviceGuard dg(c.x.device());
+      const MocScan t = c.table();
+      const Tensor dy = dy0.defined() ? dy0.to(c.x.scalar_type()).contiguous() : at::zeros(c.x.sizes(), c.x.options());
+      const Tensor dfin = dfin0.defined() ? dfin0.to(at::kFloat).contiguous() : Tensor();
+      const Tensor ins[7] = {c.x, c.dt, c.A, c.B, c.C, c.D, c.bias};
+      Needs need{ctx};
+      bool needs[7];
+      for (int i = 0; i < 7; ++i) {
+        out[i] = like(ins[i]);
+        needs[i] = need(ins[i].defined());
+      }
+      if (need(v[1] != 0)) out[7] = f32({c.x.size(0), t.heads, t.head_dim, t.state_dim}, c.x);
+      const MocScanGrads g{ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(out[3]), ptr(out[4]), ptr(out[5]), ptr(out[6]),
+                           static_cast<float*>(ptr(out[7]))};
+      const Tensor ws = bytes(moc_scan_backward_workspace_bytes(&t), c.x);
+      check(moc_scan_backward(&t, ptr(dy), v[1] != 0, static_cast<float*>(ptr(dfin)), ptr(saved[7]), saved[7].numel(),
+                              &g, ptr(ws), ws.numel(), stream_of(c.x)),
+            "moc_scan_backward");
+      for (int i = 0; i < 7; ++i)
+        if (!needs[i]) out[i] = Tensor();
+    }
+    return at::GradMode::is_enabled() ? once(std::move(out), grads) : out;
+  }
+};
+
+// (y, state or None) of fixed-length [B, T, ..] or packed [N, ..] inputs
+std::optional<std::tuple<Tensor, OptTensor>> scan(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B,
+                                                  const Tensor& C, const Tensor& D, const Tensor& bias,
+                                                  const OptTensor& cache, bool softplus, bool want, const OptTensor& cu) {
+  const int64_t lead = cu.has_value() ? 1 : 2;
+  if (!unwatched() || dtype_code(x.scalar_type()) < 0 || x.dim() != lead + 2 || dt.dim() != lead + 1 ||
+      B.dim() != lead + 2 || C.sizes() != B.sizes())
+    return std::nullopt;
+  for (const Tensor* t : {&x, &dt, &B, &C})
+    if (!plain(*t) || t->device() != x.device() || t->scalar_type() != x.scalar_type() || t->numel() == 0 ||
+        t->sizes().slice(0, lead) != x.sizes().slice(0, lead))
+      return std::nullopt;
+  const int64_t H = x.size(-2), P = x.size(-1), G = B.size(-2), N = B.size(-1);
+  if (dt.size(-1) != H || H % G != 0 || P > 128 || N > 256 || !A.defined()) return std::nullopt;
+  if (!param_ok(A, x, {H}) || !param_ok(D, x, {H}) || !param_ok(bias, x, {H}) || !offsets_ok(cu, x)) return std::nullopt;
+  if (cu.has_value() && (cache.has_value() || want)) return std::nullopt;
+  if (cache.has_value() && (!plain(*cache) || cache->device() != x.device() || cache->scalar_type() != at::kFloat ||
+                            cache->sizes() != at::IntArrayRef({x.size(0), H, P, N})))
+    return std::nullopt;
+  const c10::DeviceGuard dg(x.device());
+  const Packing k{cu.has_value() ? cu->contiguous() : Tensor(), x.numel() / (H * P), cu.has_value() ? 0 : x.size(1)};
+  if (cache.has_value() && x.size(1) == 1) {
+    if (!cache->is_contiguous()) return std::nullopt;
+    at::NoGradGuard ng;
+    ScanCall c{x, dt, A, B, C, D, bias, k, softplus};
+    const MocScan t = c.table();
+    Tensor y = at::empty(x.sizes(), x.options());
+    check(moc_scan_update(&t, static_cast<float*>(ptr(*cache)), ptr(y), stream_of(x)), "moc_scan_update");
+    written(*cache);
+    return std::make_tuple(y, want ? cache : OptTensor());
+  }
+  if (wants_grad({&x, &dt, &A, &B, &C, &D, &bias, cache.has_value() ? &*cache : nullptr})) {
+    const auto out = ScanFn::apply(x, dt, A, B, C, opt(D), opt(bias), cache, static_cast<int64_t>(softplus), want, &k);
+    return std::make_tuple(out[0], want ? OptTensor(out[1]) : OptTensor());
+  }
+  at::NoGradGuard ng;
+  ScanCall c{x, dt, A, B, C, D, bias, k, softplus};
+  Tensor fin;
+  Tensor y = c.run(cache.has_value() ? cache->contiguous() : Tensor(), want ? &fin : nullptr, nullptr);
+  return std::make_tuple(y, want ? OptTensor(fin) : OptTensor());
+}
+
 // the nodes' Python type, under the name of the Python function they stand for
 template <typename F>
 void name_node(const char* name) {
@@ -388,6 +734,7 @@ struct Args {
     return own ? THPVariable_Unpack(h.ptr()) : Tensor();
   }
   OptTensor opt(py::handle h) { return h.is_none() ? OptTensor() : OptTensor((*this)(h)); }
+  Tensor or_none(py::handle h) { return h.is_none() ? Tensor() : (*this)(h); }
 };
 
 }  // namespace
@@ -395,6 +742,35 @@ struct Args {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   name_node<LayerFn>("_MoCLayerFunctionBackward");
   name_node<FuncFn>("_MoCFunctionBackward");
+  name_node<NormFn>("_LayerNormFunctionBackward");
+  name_node<ConvFn>("_CausalConvFunctionBackward");
+  name_node<ScanFn>("_SelectiveScanFunctionBackward");
+  m.def("norm", [](py::handle x, py::handle w, py::handle b, double eps) -> OptTensor {
+    Args a;
+    const Tensor tx = a(x), tw = a.or_none(w), tb = a.or_none(b);
+    if (!a.own) return std::nullopt;
+    const py::gil_scoped_release unlocked;
+    return norm(tx, tw, tb, eps);
+  });
+  m.def("conv", [](py::handle x, py::handle w, py::handle b, py::handle cache, int act, bool want,
+                   py::handle cu) -> std::optional<std::tuple<Tensor, OptTensor>> {
+    Args a;
+    const Tensor tx = a(x), tw = a(w), tb = a.or_none(b);
+    const OptTensor tc = a.opt(cache), tu = a.opt(cu);
+    if (!a.own) return std::nullopt;
+    const py::gil_scoped_release unlocked;
+    return conv(tx, tw, tb, tc, act, want, tu);
+  });
+  m.def("scan", [](py::handle x, py::handle dt, py::handle A, py::handle B, py::handle C, py::handle D, py::handle bias,
+                   py::handle cache, bool softplus, bool want,
+                   py::handle cu) -> std::optional<std::tuple<Tensor, OptTensor>> {
+    Args a;
+    const Tensor tx = a(x), tdt = a(dt), tA = a(A), tB = a(B), tC = a(C), tD = a.or_none(D), tb = a.or_none(bias);
+    const OptTensor tc = a.opt(cache), tu = a.opt(cu);
+    if (!a.own) return std::nullopt;
+    const py::gil_scoped_release unlocked;
+    return scan(tx, tdt, tA, tB, tC, tD, tb, tc, softplus, want, tu);
+  });
   m.def("layer", [](py::handle x, py::handle z, py::handle router, py::handle basis, int act, int route,
                     py::handle cu) -> OptTensor {
     Args a;

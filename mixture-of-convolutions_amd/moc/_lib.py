@@ -268,7 +268,7 @@ class _NoHost:
     def _none(*_):
         return None
 
-    layer = func = stateful = _none
+    layer = func = stateful = norm = conv = scan = _none
 
 
 def host():

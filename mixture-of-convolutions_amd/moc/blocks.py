@@ -10,7 +10,8 @@ sequence the decode step, in place on the cache and not differentiable.
 * ``layer_norm`` / ``LayerNorm``: the norm whose output the MoC layers route by.
 
 All run as hand-written HIP kernels of libmoc_hip.so, forward, backward and step;
-there is no fallback.
+there is no fallback.  Calls go through the host module (csrc/moc_host.cpp) where they
+are ones that it takes; the Python functions below are the same calls for all others.
 """
 from __future__ import annotations
 
@@ -22,7 +23,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .api import SUPPORTED_DTYPES, _final_state, activation_flag
+from .api import SUPPORTED_DTYPES, _final_state, _is_length, activation_flag
 
 
 # ---------------------------------------------------------------------------
@@ -69,6 +70,11 @@ def _check_state(cache: torch.Tensor, shape: tuple, dtype: torch.dtype, x: torch
         raise ValueError("a step writes its cache in place: no two of its elements may share memory")
 
 
+def _on_gpu(x) -> bool:
+    """Whether the host module is asked first (it hands back what is not its own)."""
+    return isinstance(x, torch.Tensor) and x.is_cuda
+
+
 def _operand(t: torch.Tensor | None) -> torch.Tensor | None:
     """A parameter as the kernels read it: contiguous, fp32, bf16 or fp16."""
     return None if t is None else ops._operand(t)
@@ -107,6 +113,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     """Layer norm over the last axis of ``x`` (bf16 or fp32, any rank from 1):
     ``(x - mean) / sqrt(var + eps) * weight + bias`` with fp32 statistics.
     ``weight`` and ``bias`` are ``[dim]`` in any floating dtype, or None."""
+    if _on_gpu(x):
+        y = _lib.host().norm(x, weight, bias, eps)
+        if y is not None:
+            return y
     _check_tensors(x, weight=weight, bias=bias)
     if x.ndim < 1 or x.numel() == 0:
         raise ValueError(f"x must have a last axis and no empty one, got shape {tuple(x.shape)}")
@@ -174,6 +184,11 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     in place on it (returned as the state); with more tokens the history before
     them.  The final state is the last S inputs, as a new tensor."""
     act = activation_flag(activation)
+    if _on_gpu(x) and (cu_seqlens is None) == (max_seqlen is None):
+        if cu_seqlens is None or (x.ndim == 2 and _is_length(max_seqlen)):
+            out = _lib.host().conv(x, weight, bias, cache, act, bool(output_final_state), cu_seqlens)
+            if out is not None:
+                return out
     _check_tensors(x, weight=weight, bias=bias)
     _check_packing(x, cu_seqlens, max_seqlen, cache, output_final_state)
     restore = False
@@ -308,6 +323,13 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     tensor.  States and sums are fp32; with bf16 inputs the state and the token-to-token
     weights are rounded to bf16 where they enter a matrix product.  An infinity or NaN in
     one token reaches the outputs of that token and later ones of its sequence only."""
+    softplus = bool(dt_softplus)
+    if _on_gpu(x) and (cu_seqlens is None) == (max_seqlen is None):
+        if cu_seqlens is None or (x.ndim == 3 and _is_length(max_seqlen)):
+            out = _lib.host().scan(x, dt, A, B, C, D, dt_bias, cache, softplus, bool(output_final_state),
+                                   cu_seqlens)
+            if out is not None:
+                return out
     _check_tensors(x, dt=dt, A=A, B=B, C=C, D=D, dt_bias=dt_bias)
     _check_packing(x, cu_seqlens, max_seqlen, cache, output_final_state)
     restore = False
@@ -335,7 +357,6 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     if P > _lib.SCAN_MAX_HEAD_DIM or N > _lib.SCAN_MAX_STATE_DIM:
         raise ValueError(f"P must be at most {_lib.SCAN_MAX_HEAD_DIM} and N at most {_lib.SCAN_MAX_STATE_DIM}, "
                          f"got {P} and {N}")
-    softplus = bool(dt_softplus)
     A, D, dt_bias = _operand(A), _operand(D), _operand(dt_bias)
     if cu_seqlens is not None:
         cu_seqlens = cu_seqlens.contiguous()

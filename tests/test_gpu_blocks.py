@@ -681,3 +681,39 @@ def test_library_refuses_what_python_would():
     with pytest.raises(RuntimeError, match="kernel_size must be in"):
         moc.ops.launch_conv_forward(x, dev(rnd(17, 8)), None, None, activation_flag=0)
     assert _lib.lib().moc_last_error()
+
+
+def test_python_functions_are_the_host_modules(monkeypatch):
+    """Without the host module the Python functions make the same calls."""
+    def everything():
+        out = []
+        w, b = dev(rnd(96, seed=2)).requires_grad_(), dev(rnd(96, seed=3, dtype=BF16)).requires_grad_()
+        cw = dev(rnd(4, 96, seed=4)).requires_grad_()
+        x = dev(rnd(2, 70, 96, seed=1, dtype=BF16)).requires_grad_()
+        cu = torch.tensor([0, 5, 70], dtype=torch.int32, device=DEV)
+        ins = {k: dev(v).requires_grad_() for k, v in scan_inputs((2, 70), 4, 24, 2, 16, BF16, par=F32).items()}
+        one = lambda k: {q: (v[0] if v.ndim > 1 else v) for q, v in k.items()}  # noqa: E731
+        init = dev(rnd(2, 4, 24, 16, seed=9)).requires_grad_()
+        for y in (moc.layer_norm(x, w, b), moc.layer_norm(x), moc.causal_conv(x, cw, b, "silu")[0],
+                  moc.causal_conv(x[0], cw, cu_seqlens=cu, max_seqlen=65)[0],
+                  moc.selective_scan(**ins)[0], moc.selective_scan(**one(ins), cu_seqlens=cu, max_seqlen=65)[0],
+                  *moc.selective_scan(**ins, cache=init, output_final_state=True)):
+            leaves = [t for t in (x, w, b, cw, init, *ins.values())]
+            out += [y, *[g for g in torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True,
+                                                              allow_unused=True)
+                         if g is not None]]
+        with torch.no_grad():
+            out += moc.causal_conv(x, cw, b, "silu", output_final_state=True)
+            c = out[-1].clone()
+            out += moc.causal_conv(x, cw, b, cache=c, output_final_state=True)
+            out += moc.causal_conv(x[:, :1], cw, b, cache=c, output_final_state=True)
+            out += moc.selective_scan(**ins, output_final_state=True)
+            c = out[-1].clone()
+            out += moc.selective_scan(**{k: (v[:, 1:2] if v.ndim > 1 else v) for k, v in ins.items()}, cache=c,
+                                      output_final_state=True)
+        return out
+
+    here = everything()
+    monkeypatch.setattr(_lib, "_host", _lib._NoHost)
+    there = everything()
+    assert len(here) == len(there) and all(torch.equal(a, b) for a, b in zip(here, there))
