@@ -437,7 +437,7 @@ int moc_conv_forward(const void* x, const void* weight, const void* bias, const 
                      int activation, void* stream);
 
 /* Workspace bytes of moc_conv_backward with dweight or dbias. */
-size_t moc_conv_backward_workspace_bytes(int64_t n_tokens, int64_t dim, int64_t kernel_size);
+size_t moc_conv_backward_workspace_bytes(int64_t n_tokens, int64_t dim, int64_t kernel_size, int x_dtype);
 
 /* Gradients of moc_conv_forward without a cache for dy [n_tokens, dim]; dx, dweight,
  * dbias may each be NULL.  Sums over tokens are formed in a fixed order. */

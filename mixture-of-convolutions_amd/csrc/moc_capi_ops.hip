@@ -183,9 +183,9 @@ int moc_conv_forward(const void* x, const void* weight, const void* bias, const 
   return launched("moc_conv_forward launch");
 }
 
-size_t moc_conv_backward_workspace_bytes(int64_t n_tokens, int64_t dim, int64_t kernel_size) {
+size_t moc_conv_backward_workspace_bytes(int64_t n_tokens, int64_t dim, int64_t kernel_size, int x_dtype) {
   if (n_tokens <= 0 || dim <= 0 || kernel_size <= 0) return 0;
-  return moc::conv_backward_workspace({layout(nullptr, 0, 0, n_tokens, n_tokens), dim, kernel_size, 0, 0, 0, 0});
+  return moc::conv_backward_workspace({layout(nullptr, 0, 0, n_tokens, n_tokens), dim, kernel_size, x_dtype, 0, 0, 0});
 }
 
 int moc_conv_backward(const void* x, const void* weight, const void* bias, const void* dy, void* dx, void* dweight,

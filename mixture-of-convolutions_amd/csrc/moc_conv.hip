@@ -23,6 +23,7 @@ namespace moc {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kAhead = 4, kAheadBack = 2;  // rows loaded together
 
 struct ConvArgs {
   const void* x;
@@ -39,12 +40,6 @@ struct ConvArgs {
   int w_dt, b_dt, act, rows;  // rows: tokens of a strip
 };
 
-template <int V>
-__device__ __forceinline__ void load_par(const void* p, int dt, int64_t i, float (&out)[V]) {
-#pragma unroll
-  for (int k = 0; k < V; ++k) out[k] = p == nullptr ? 0.f : load_any(p, dt, i + k);
-}
-
 // x[t - k] for k = 1..S-1 of a row at position pos of its sequence [lo, ..):
 // win[S-1-k]; rows before the sequence come from the cache or are 0.
 template <int DT, int S, int V>
@@ -53,12 +48,12 @@ __device__ __forceinline__ void history(const ConvArgs& a, int64_t t, int64_t lo
   for (int k = 1; k < S; ++k) {
     const int64_t u = t - k;
     if (u >= lo) {
-      load_vec<DT, V>(a.x, u * a.D + c, win[S - 1 - k]);
+      load_vec<DT, V>(a.x, u * a.D + c, a.D - c, win[S - 1 - k]);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float v = 0.f;
-        if (a.cache != nullptr)  // fixed length: sequence lo / seq_len, slot S - (lo - u)
+        if (a.cache != nullptr && c + i < a.D)  // fixed length: sequence lo / seq_len, slot S - (lo - u)
           v = load_any(a.cache, DT, ((lo / a.seq.seq_len) * a.D + c + i) * S + (S - (lo - u)));
         win[S - 1 - k][i] = v;
       }
@@ -76,17 +71,13 @@ __global__ __launch_bounds__(64 * kWaves) void conv_fwd(ConvArgs a) {
   const int64_t r1 = r0 + a.rows < n ? r0 + a.rows : n;
   float w[S][V], b[V], win[S][V];
 #pragma unroll
-  for (int s = 0; s < S; ++s) load_par<V>(a.w, a.w_dt, s * a.D + c, w[s]);
-  load_par<V>(a.bias, a.b_dt, c, b);
+  for (int s = 0; s < S; ++s) load_param<V>(a.w, a.w_dt, s * a.D + c, a.D - c, 0.f, w[s]);
+  load_param<V>(a.bias, a.b_dt, c, a.D - c, 0.f, b);
   int64_t lo, hi;
   a.seq.bounds(r0, lo, hi);
   history<DT, S, V>(a, r0, lo, c, win);
-  for (int64_t t = r0; t < r1; ++t) {
-    if (t >= hi) {
-      a.seq.bounds(t, lo, hi);
-      history<DT, S, V>(a, t, lo, c, win);
-    }
-    load_vec<DT, V>(a.x, t * a.D + c, win[S - 1]);
+  const int64_t left = a.D - c;
+  auto row = [&](int64_t t) {  // win[S - 1] holds x[t]
     float p[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -95,11 +86,10 @@ __global__ __launch_bounds__(64 * kWaves) void conv_fwd(ConvArgs a) {
       for (int s = 0; s < S; ++s) p[i] += w[s][i] * win[s][i];
       if (a.act) p[i] *= sigmoid_f(p[i]);
     }
-    store_vec<DT, V>(a.y, t * a.D + c, p);
+    store_vec<DT, V>(a.y, t * a.D + c, left, p);
     if (a.fin != nullptr && hi - t <= S) {  // slots of the last S rows (fixed length)
       const int64_t q = lo / a.seq.seq_len;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
+      for (int i = 0; i < V && i < left; ++i) {
         const int64_t at = (q * a.D + c + i) * S;
         store_any(a.fin, DT, at + S - (hi - t), win[S - 1][i]);
         // a sequence shorter than the state: its first row also writes the older slots
@@ -112,6 +102,29 @@ __global__ __launch_bounds__(64 * kWaves) void conv_fwd(ConvArgs a) {
     for (int s = 0; s + 1 < S; ++s)
 #pragma unroll
       for (int i = 0; i < V; ++i) win[s][i] = win[s + 1][i];
+  };
+  int64_t t = r0;
+  while (t < r1) {
+    if (t >= hi) {
+      a.seq.bounds(t, lo, hi);
+      history<DT, S, V>(a, t, lo, c, win);
+    }
+    const int64_t end = hi < r1 ? hi : r1;
+    // kAhead rows' loads in flight at a time
+    for (; t + kAhead <= end; t += kAhead) {
+      RawVec<DT, V> x[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) x[k].load(a.x, (t + k) * a.D + c, left);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        x[k].get(win[S - 1]);
+        row(t + k);
+      }
+    }
+    for (; t < end; ++t) {
+      load_vec<DT, V>(a.x, t * a.D + c, left, win[S - 1]);
+      row(t);
+    }
   }
 }
 
@@ -133,8 +146,8 @@ __global__ __launch_bounds__(64 * kWaves) void conv_bwd(ConvArgs a) {
   if (r0 < n && c < a.D) {
     float w[S][V], b[V], win[S][V], acc[S][V];  // acc[k]: dx of row u - k so far
 #pragma unroll
-    for (int s = 0; s < S; ++s) load_par<V>(a.w, a.w_dt, s * a.D + c, w[s]);
-    load_par<V>(a.bias, a.b_dt, c, b);
+    for (int s = 0; s < S; ++s) load_param<V>(a.w, a.w_dt, s * a.D + c, a.D - c, 0.f, w[s]);
+    load_param<V>(a.bias, a.b_dt, c, a.D - c, 0.f, b);
 #pragma unroll
     for (int k = 0; k < S; ++k)
 #pragma unroll
@@ -142,56 +155,91 @@ __global__ __launch_bounds__(64 * kWaves) void conv_bwd(ConvArgs a) {
     int64_t lo, hi;
     a.seq.bounds(r0, lo, hi);
     history<DT, S, V>(a, r0, lo, c, win);
-    // rows u < r1 are this strip's; the S - 1 rows behind them only reach back into it
-    for (int64_t u = r0; u < r1 + S - 1; ++u) {
-      const bool real = u < n;
-      if (real && u >= hi) {
-        a.seq.bounds(u, lo, hi);
-        history<DT, S, V>(a, u, lo, c, win);
+    const int64_t left = a.D - c;
+    // g of row u (dy read into g, x into win[S - 1]), its part of the sums where the row is
+    // this strip's own, and of the gradients of the rows it reaches back to
+    auto row = [&](int64_t u, float (&g)[V]) {
+      if (a.act) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float p = b[i];
+#pragma unroll
+          for (int s = 0; s < S; ++s) p += w[s][i] * win[s][i];
+          const float sg = sigmoid_f(p);
+          g[i] *= sg * (1.f + p * (1.f - sg));
+        }
       }
-      if (real && (u < r1 || lo < r1)) {
-        float g[V];
-        load_vec<DT, V>(a.x, u * a.D + c, win[S - 1]);
-        load_vec<DT, V>(a.dy, u * a.D + c, g);
-        if (a.act) {
+      if (u < r1) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float p = b[i];
+        for (int i = 0; i < V; ++i) {
+          db[i] += g[i];
 #pragma unroll
-            for (int s = 0; s < S; ++s) p += w[s][i] * win[s][i];
-            const float sg = sigmoid_f(p);
-            g[i] *= sg * (1.f + p * (1.f - sg));
-          }
+          for (int s = 0; s < S; ++s) dw[s][i] += g[i] * win[s][i];
         }
-        if (u < r1) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            db[i] += g[i];
-#pragma unroll
-            for (int s = 0; s < S; ++s) dw[s][i] += g[i] * win[s][i];
-          }
-        }
-        const int64_t back = u - lo;  // rows of the same sequence before u
-#pragma unroll
-        for (int k = 0; k < S; ++k) {
-          if (k <= back) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[k][i] += w[S - 1 - k][i] * g[i];
-          }
-        }
-#pragma unroll
-        for (int s = 0; s + 1 < S; ++s)
-#pragma unroll
-          for (int i = 0; i < V; ++i) win[s][i] = win[s + 1][i];
       }
+      const int64_t back = u - lo;  // rows of the same sequence before u
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        if (k <= back) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[k][i] += w[S - 1 - k][i] * g[i];
+        }
+      }
+#pragma unroll
+      for (int s = 0; s + 1 < S; ++s)
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[s][i] = win[s + 1][i];
+    };
+    auto emit = [&](int64_t u) {  // dx of row u - (S - 1) is whole
       const int64_t t = u - (S - 1);
-      if (t >= r0 && t < r1 && a.dx != nullptr) store_vec<DT, V>(a.dx, t * a.D + c, acc[S - 1]);
+      if (t >= r0 && t < r1 && a.dx != nullptr) store_vec<DT, V>(a.dx, t * a.D + c, left, acc[S - 1]);
 #pragma unroll
       for (int k = S - 1; k > 0; --k)
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[k][i] = acc[k - 1][i];
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[0][i] = 0.f;
+    };
+    // rows u < r1 are this strip's; the S - 1 rows behind them only reach back into it
+    int64_t u = r0;
+    while (u < r1 + S - 1) {
+      if (u < n && u >= hi) {
+        a.seq.bounds(u, lo, hi);
+        history<DT, S, V>(a, u, lo, c, win);
+      }
+      auto one = [&]() {
+        float g[V];
+        load_vec<DT, V>(a.x, u * a.D + c, left, win[S - 1]);
+        load_vec<DT, V>(a.dy, u * a.D + c, left, g);
+        row(u, g);
+      };
+      if (u >= r1) {
+        if (u < n && lo < r1) one();
+        emit(u);
+        ++u;
+        continue;
+      }
+      const int64_t end = hi < r1 ? hi : r1;
+      for (; u + kAheadBack <= end; u += kAheadBack) {
+        RawVec<DT, V> x[kAheadBack], dy[kAheadBack];
+#pragma unroll
+        for (int k = 0; k < kAheadBack; ++k) {
+          x[k].load(a.x, (u + k) * a.D + c, left);
+          dy[k].load(a.dy, (u + k) * a.D + c, left);
+        }
+#pragma unroll
+        for (int k = 0; k < kAheadBack; ++k) {
+          float g[V];
+          x[k].get(win[S - 1]);
+          dy[k].get(g);
+          row(u + k, g);
+          emit(u + k);
+        }
+      }
+      for (; u < end; ++u) {
+        one();
+        emit(u);
+      }
     }
   }
   if (a.part == nullptr) return;
@@ -210,7 +258,7 @@ __global__ __launch_bounds__(64 * kWaves) void conv_bwd(ConvArgs a) {
     if (wave == 0 && c < a.D) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        out[s * a.D + c + i] = ((v[i] + lds[0][at + i]) + lds[1][at + i]) + lds[2][at + i];
+        if (c + i < a.D) out[s * a.D + c + i] = ((v[i] + lds[0][at + i]) + lds[1][at + i]) + lds[2][at + i];
     }
     __syncthreads();
   }
@@ -241,38 +289,32 @@ __global__ __launch_bounds__(256) void conv_step(const void* __restrict__ x, con
   }
 }
 
-// Channels of a lane: 16 bytes of them, fewer where S rows of them in fp32 (twice, and
-// the weights and their sums, in the backward) would not stay in registers, or where
-// the channel count or an address does not allow the vector.
-int vec(int64_t D, int dt, int S, bool backward, uintptr_t addr) {
-  int v = dt == DT_BF16 ? 8 : 4;
-  const int most = backward ? (S <= 4 ? 8 : (S <= 8 ? 4 : 2)) : (S <= 8 ? 8 : 4);
-  if (v > most) v = most;
-  const uintptr_t e = dt == DT_BF16 ? 2 : 4;
-  while (v > 1 && (D % v != 0 || addr % (v * e) != 0)) v >>= 1;
-  return v;
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+template <int DT, typename F>
+void with_taps(int64_t S, F&& f) {
+  switch (S) {
+#define MOC_CONV_S(SS) \
+  case SS: return f(Int<DT>{}, Int<SS>{});
+    MOC_CONV_S(1) MOC_CONV_S(2) MOC_CONV_S(3) MOC_CONV_S(4) MOC_CONV_S(5) MOC_CONV_S(6) MOC_CONV_S(7) MOC_CONV_S(8)
+    MOC_CONV_S(9) MOC_CONV_S(10) MOC_CONV_S(11) MOC_CONV_S(12) MOC_CONV_S(13) MOC_CONV_S(14) MOC_CONV_S(15)
+    MOC_CONV_S(16)
+#undef MOC_CONV_S
+    default: return;
+  }
+}
+template <typename F>
+void with_shape(int dt, int64_t S, F&& f) {
+  if (dt == DT_BF16) with_taps<DT_BF16>(S, f);
+  else with_taps<DT_F32>(S, f);
 }
 
-template <typename F>
-bool with_shape(int dt, int S, int v, F&& f) {
-#define MOC_CONV_V(DT, SS, V) \
-  if (dt == DT && S == SS && v == V) { \
-    f(std::integral_constant<int, DT>{}, std::integral_constant<int, SS>{}, std::integral_constant<int, V>{}); \
-    return true; \
-  }
-#define MOC_CONV_S(SS) \
-  MOC_CONV_V(DT_BF16, SS, 8) MOC_CONV_V(DT_BF16, SS, 4) MOC_CONV_V(DT_BF16, SS, 2) MOC_CONV_V(DT_BF16, SS, 1) \
-  MOC_CONV_V(DT_F32, SS, 4) MOC_CONV_V(DT_F32, SS, 2) MOC_CONV_V(DT_F32, SS, 1)
-#define MOC_CONV_L(SS) \
-  MOC_CONV_V(DT_BF16, SS, 4) MOC_CONV_V(DT_BF16, SS, 2) MOC_CONV_V(DT_BF16, SS, 1) \
-  MOC_CONV_V(DT_F32, SS, 4) MOC_CONV_V(DT_F32, SS, 2) MOC_CONV_V(DT_F32, SS, 1)
-  MOC_CONV_S(1) MOC_CONV_S(2) MOC_CONV_S(3) MOC_CONV_S(4) MOC_CONV_S(5) MOC_CONV_S(6) MOC_CONV_S(7) MOC_CONV_S(8)
-  MOC_CONV_L(9) MOC_CONV_L(10) MOC_CONV_L(11) MOC_CONV_L(12) MOC_CONV_L(13) MOC_CONV_L(14) MOC_CONV_L(15)
-  MOC_CONV_L(16)
-#undef MOC_CONV_L
-#undef MOC_CONV_S
-#undef MOC_CONV_V
-  return false;
+// Channels of a lane: 16 bytes of them, fewer where S rows of them in fp32 (twice, and
+// the weights and their sums, in the backward) would not stay in registers.
+constexpr int vec(int dt, int64_t S, bool backward) {
+  const int v = dt == DT_BF16 ? 8 : 4, most = backward ? (S <= 2 ? 8 : (S <= 8 ? 4 : 2)) : (S <= 8 ? 8 : 4);
+  return v < most ? v : most;
 }
 
 // Rows of a strip: as many as still leave about 2048 waves (two a SIMD), 4 to 64.
@@ -286,8 +328,6 @@ int strip(int64_t tokens, int64_t D, int v) {
 }
 
 int64_t strip_groups(int64_t tokens, int r) { return (tokens + kWaves * r - 1) / (kWaves * r); }
-
-uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 ConvArgs args(const Conv& p, const void* x, const void* w, const void* bias) {
   ConvArgs a{};
@@ -305,14 +345,8 @@ ConvArgs args(const Conv& p, const void* x, const void* w, const void* bias) {
 }  // namespace
 
 size_t conv_backward_workspace(const Conv& p) {
-  // (the vector width may be the full one or, for a tensor that is not aligned, less)
-  const size_t row = size_t(p.S + 1) * p.D * sizeof(float);
-  size_t most = 0;
-  for (int v = 1; v <= 8; v *= 2) {
-    const size_t n = strip_groups(p.seq.n_tokens, strip(p.seq.n_tokens, p.D, v));
-    if (n > most) most = n;
-  }
-  return most * row;
+  return size_t(strip_groups(p.seq.n_tokens, strip(p.seq.n_tokens, p.D, vec(p.x_dt, p.S, true)))) * (p.S + 1) * p.D *
+         sizeof(float);
 }
 
 void conv_forward(const Conv& p, const void* x, const void* w, const void* bias, const void* cache, void* y, void* fin,
@@ -321,12 +355,12 @@ void conv_forward(const Conv& p, const void* x, const void* w, const void* bias,
   a.cache = cache;
   a.y = y;
   a.fin = fin;
-  const int v = vec(p.D, p.x_dt, static_cast<int>(p.S), false, bits(x) | bits(y));
+  const int v = vec(p.x_dt, p.S, false);
   a.rows = strip(p.seq.n_tokens, p.D, v);
   const dim3 grid(static_cast<unsigned>((p.D + 64 * v - 1) / (64 * v)),
                   static_cast<unsigned>(strip_groups(p.seq.n_tokens, a.rows)));
-  with_shape(p.x_dt, static_cast<int>(p.S), v, [&](auto DT, auto S, auto V) {
-    hipLaunchKernelGGL((conv_fwd<DT.value, S.value, V.value>), grid, dim3(64 * kWaves), 0, st, a);
+  with_shape(p.x_dt, p.S, [&](auto DT, auto S) {
+    hipLaunchKernelGGL((conv_fwd<DT.value, S.value, vec(DT.value, S.value, false)>), grid, dim3(64 * kWaves), 0, st, a);
   });
 }
 
@@ -337,12 +371,12 @@ void conv_backward(const Conv& p, const void* x, const void* w, const void* bias
   a.dx = dx;
   const bool sums = dw != nullptr || dbias != nullptr;
   a.part = sums ? static_cast<float*>(workspace) : nullptr;
-  const int v = vec(p.D, p.x_dt, static_cast<int>(p.S), true, bits(x) | bits(dy) | bits(dx));
+  const int v = vec(p.x_dt, p.S, true);
   a.rows = strip(p.seq.n_tokens, p.D, v);
   const int64_t groups = strip_groups(p.seq.n_tokens, a.rows);
   const dim3 grid(static_cast<unsigned>((p.D + 64 * v - 1) / (64 * v)), static_cast<unsigned>(groups));
-  with_shape(p.x_dt, static_cast<int>(p.S), v, [&](auto DT, auto S, auto V) {
-    hipLaunchKernelGGL((conv_bwd<DT.value, S.value, V.value>), grid, dim3(64 * kWaves), 0, st, a);
+  with_shape(p.x_dt, p.S, [&](auto DT, auto S) {
+    hipLaunchKernelGGL((conv_bwd<DT.value, S.value, vec(DT.value, S.value, true)>), grid, dim3(64 * kWaves), 0, st, a);
   });
   if (sums) launch_column_sums({a.part, groups, p.S * p.D, p.D, 0, dw, dbias, nullptr, p.w_dt, p.b_dt, 0}, st);
 }
@@ -351,7 +385,7 @@ void conv_update(const void* x, const void* w, const void* bias, void* cache, in
                  void* y, int64_t B, int64_t D, int64_t S, int x_dt, int w_dt, int b_dt, int act, hipStream_t st) {
   const int64_t n = (B * D + 255) / 256;
   const dim3 grid(static_cast<unsigned>(n < (1 << 22) ? n : (1 << 22)));
-  with_shape(x_dt, static_cast<int>(S), 1, [&](auto DT, auto SS, auto) {
+  with_shape(x_dt, S, [&](auto DT, auto SS) {
     hipLaunchKernelGGL((conv_step<DT.value, SS.value>), grid, dim3(256), 0, st, x, w, bias, cache, cb, cd, cs, y, B, D,
                        w_dt, b_dt, act);
   });

@@ -508,7 +508,7 @@ struct ConvFn : public torch::autograd::Function<ConvFn> {
       if (need(true)) out[1] = like(w);
       if (need(b.defined())) out[2] = like(b);
       const bool sums = out[1].defined() || out[2].defined();
-      const size_t n = sums ? moc_conv_backward_workspace_bytes(k.tokens, w.size(1), w.size(0)) : 0;
+      const size_t n = sums ? moc_conv_backward_workspace_bytes(k.tokens, w.size(1), w.size(0), dtype_code(x.scalar_type())) : 0;
       const Tensor ws = sums ? bytes(n, x) : Tensor();
       check(moc_conv_backward(ptr(x), ptr(w), ptr(b), ptr(dy), ptr(out[0]), ptr(out[1]), ptr(out[2]), k.p(), k.i64(),
                               k.n_seqs(), k.tokens, k.seq_len, w.size(1), w.size(0), dtype_code(x.scalar_type()),

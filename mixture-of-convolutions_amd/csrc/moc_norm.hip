@@ -40,51 +40,73 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
   return v;
 }
 
-// w / b of V columns, in any dtype.
-template <int V>
-__device__ __forceinline__ void load_param(const void* p, int dt, int64_t i, float none, float (&out)[V]) {
+// A row's NV vectors of a lane; TAIL: the last one may end behind the row.
+template <int DT, int V, int NV, int TPR, bool TAIL>
+struct Row {
+  RawVec<DT, V> r[NV];
+  __device__ __forceinline__ void load(const void* p, int64_t row, int D, int lane, bool live) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) out[k] = p == nullptr ? none : load_any(p, dt, i + k);
-}
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * V;
+      const int n = live ? D - c : 0;
+      if (TAIL) {
+        r[i].load(p, row * D + c, n);
+      } else if (n > 0) {
+        r[i].load(p, row * D + c, V);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) r[i].e[k] = 0;
+      }
+    }
+  }
+};
 
-template <int DT, int V, int NV, int TPR>
+// Rows are walked a grid apart with the weights in registers and the next row's loads in
+// flight: a workgroup a row would read w and b, twice a bf16 row's bytes, for each of them.
+template <int DT, int V, int NV, int TPR, bool TAIL>
 __global__ __launch_bounds__(kThreads) void norm_fwd(const void* __restrict__ x, const void* __restrict__ w,
                                                      const void* __restrict__ b, void* __restrict__ y,
                                                      float* __restrict__ mean_out, float* __restrict__ rstd_out,
                                                      int64_t rows, int D, int w_dt, int b_dt, float eps) {
   __shared__ float buf[4];
-  const int lane = threadIdx.x % TPR;
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   constexpr int RPW = kThreads / TPR;
   const float inv = 1.0f / static_cast<float>(D);
+  const int64_t step = int64_t(gridDim.x) * RPW;
+  int64_t row = int64_t(blockIdx.x) * RPW + group;
+  Row<DT, V, NV, TPR, TAIL> next;
+  next.load(x, row, D, lane, row < rows);
+  float wv[NV][V], bv[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + lane) * V;
+    if (c < D) {
+      load_param<V>(w, w_dt, c, TAIL ? D - c : V, 1.f, wv[i]);
+      load_param<V>(b, b_dt, c, TAIL ? D - c : V, 0.f, bv[i]);
+    }
+  }
   // (every lane runs every round: a row of a whole workgroup has barriers in it)
-  for (int64_t r0 = int64_t(blockIdx.x) * RPW; r0 < rows; r0 += int64_t(gridDim.x) * RPW) {
-    const int64_t row = r0 + threadIdx.x / TPR;
+  for (; row - group < rows; row += step) {
     const bool live = row < rows;
-    const int64_t base = row * D;
     float v[NV][V];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * V;
-      if (live && c < D) {
-        load_vec<DT, V>(x, base + c, v[i]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[i][k] = 0.f;
-      }
+      next.r[i].get(v[i]);
 #pragma unroll
       for (int k = 0; k < V; ++k) s += v[i][k];
     }
-    const float mean = row_sum<TPR>(s, buf) * inv;
+    next.load(x, row + step, D, lane, row + step < rows);
+    // (a true quotient: a mean of equal elements is that element)
+    const float mean = row_sum<TPR>(s, buf) / static_cast<float>(D);
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if ((i * TPR + lane) * V < D) {
+      const int have = D - (i * TPR + lane) * V;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          v[i][k] -= mean;
-          s += v[i][k] * v[i][k];
-        }
+      for (int k = 0; k < V; ++k) {
+        v[i][k] = (TAIL ? k < have : have > 0) ? v[i][k] - mean : 0.f;
+        s += v[i][k] * v[i][k];
       }
     }
     const float rstd = 1.0f / sqrtf(row_sum<TPR>(s, buf) * inv + eps);
@@ -97,18 +119,15 @@ __global__ __launch_bounds__(kThreads) void norm_fwd(const void* __restrict__ x,
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * V;
       if (c >= D) continue;
-      float wv[V], bv[V];
-      load_param<V>(w, w_dt, c, 1.f, wv);
-      load_param<V>(b, b_dt, c, 0.f, bv);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[i][k] = v[i][k] * rstd * wv[k] + bv[k];
-      store_vec<DT, V>(y, base + c, v[i]);
+      for (int k = 0; k < V; ++k) v[i][k] = v[i][k] * rstd * wv[i][k] + bv[i][k];
+      store_vec<DT, V>(y, row * D + c, TAIL ? D - c : V, v[i]);
     }
   }
 }
 
-// Workgroup wg walks rows (wg + i * gridDim) * RPW + its row group; part[wg] = [dw | db].
-template <int DT, int V, int NV, int TPR, bool SUMS>
+// part[blockIdx.x] = [dw | db] of the workgroup's rows.
+template <int DT, int V, int NV, int TPR, bool TAIL, bool SUMS>
 __global__ __launch_bounds__(kThreads) void norm_bwd(const void* __restrict__ x, const void* __restrict__ w,
                                                      const void* __restrict__ dy, const float* __restrict__ mean_in,
                                                      const float* __restrict__ rstd_in, void* __restrict__ dx,
@@ -118,37 +137,42 @@ __global__ __launch_bounds__(kThreads) void norm_bwd(const void* __restrict__ x,
   constexpr int RPW = kThreads / TPR;
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const float inv = 1.0f / static_cast<float>(D);
+  const int64_t step = int64_t(gridDim.x) * RPW;
+  int64_t row = int64_t(blockIdx.x) * RPW + group;
+  Row<DT, V, NV, TPR, TAIL> nx, ng;
+  float mean_n = 0.f, rstd_n = 0.f;
+  auto fetch = [&](int64_t r) {
+    const bool live = r < rows;
+    nx.load(x, r, D, lane, live);
+    ng.load(dy, r, D, lane, live);
+    mean_n = live ? mean_in[r] : 0.f;
+    rstd_n = live ? rstd_in[r] : 0.f;
+  };
+  fetch(row);
   float dw[NV][V], db[NV][V], wv[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + lane) * V;
 #pragma unroll
     for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = wv[i][k] = 0.f;
-    if (c < D) load_param<V>(w, w_dt, c, 1.f, wv[i]);
+    if (c < D) load_param<V>(w, w_dt, c, TAIL ? D - c : V, 1.f, wv[i]);
   }
   // (every lane runs every round: a row of a whole workgroup has barriers in it)
-  for (int64_t r0 = int64_t(blockIdx.x) * RPW; r0 < rows; r0 += int64_t(gridDim.x) * RPW) {
-    const int64_t row = r0 + group;
-    const bool live = row < rows;
-    const int64_t base = row * D;
-    const float mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
+  for (; row - group < rows; row += step) {
+    const float mean = mean_n, rstd = rstd_n;
     float xh[NV][V], g[NV][V];
     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * V;
-      if (live && c < D) {
-        load_vec<DT, V>(x, base + c, xh[i]);
-        load_vec<DT, V>(dy, base + c, g[i]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) xh[i][k] = mean, g[i][k] = 0.f;
-      }
+      nx.r[i].get(xh[i]);
+      ng.r[i].get(g[i]);
     }
+    fetch(row + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
+        // (past the row's end, or the last row, x reads as 0 and g too: it adds nothing)
         xh[i][k] = (xh[i][k] - mean) * rstd;
         if (SUMS) {
           dw[i][k] += g[i][k] * xh[i][k];
@@ -162,46 +186,37 @@ __global__ __launch_bounds__(kThreads) void norm_bwd(const void* __restrict__ x,
     if (dx == nullptr) continue;
     s0 = row_sum<TPR>(s0, buf) * inv;
     s1 = row_sum<TPR>(s1, buf) * inv;
-    if (!live) continue;
+    if (row >= rows) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * V;
       if (c >= D) continue;
 #pragma unroll
       for (int k = 0; k < V; ++k) g[i][k] = rstd * (g[i][k] - s0 - xh[i][k] * s1);
-      store_vec<DT, V>(dx, base + c, g[i]);
+      store_vec<DT, V>(dx, row * D + c, TAIL ? D - c : V, g[i]);
     }
   }
   if (!SUMS) return;
   float* out = part + int64_t(blockIdx.x) * 2 * D;
-  if (TPR == kThreads) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * V;
-      if (c < D) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) out[c + k] = dw[i][k], out[D + c + k] = db[i][k];
-      }
-    }
-    return;
-  }
+  float* to = TPR == kThreads ? out : lds;
   for (int q = 0; q < RPW; ++q) {  // row groups in order
     if (group == q) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + lane) * V;
-        if (c < D) {
+        if (c >= D) continue;
 #pragma unroll
-          for (int k = 0; k < V; ++k) {
-            lds[c + k] = (q == 0 ? 0.f : lds[c + k]) + dw[i][k];
-            lds[D + c + k] = (q == 0 ? 0.f : lds[D + c + k]) + db[i][k];
-          }
+        for (int k = 0; k < V; ++k) {
+          if (TAIL && c + k >= D) continue;
+          to[c + k] = q == 0 ? dw[i][k] : to[c + k] + dw[i][k];
+          to[D + c + k] = q == 0 ? db[i][k] : to[D + c + k] + db[i][k];
         }
       }
     }
-    __syncthreads();
+    if (TPR < kThreads) __syncthreads();
   }
-  for (int c = threadIdx.x; c < 2 * D; c += kThreads) out[c] = lds[c];
+  if (TPR < kThreads)
+    for (int c = threadIdx.x; c < 2 * D; c += kThreads) out[c] = lds[c];
 }
 
 // Rows too long for a workgroup's registers: the row is read again for each sum.
@@ -277,57 +292,48 @@ __global__ __launch_bounds__(kThreads) void norm_sums_long(const void* __restric
   part[int64_t(blockIdx.y) * 2 * D + D + c] = db;
 }
 
-// How a row is spread: TPR lanes of NV vectors of V elements.
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+// How a row is spread: TPR lanes of NV vectors of 16 bytes.
 struct Plan {
-  int v, nv, tpr;  // nv 0: the long kernels
+  int nv, tpr;  // nv 0: the long kernels
 };
 
-// V: 16-byte vectors where rows and tensors allow them, pairs of bf16 or single
-// elements otherwise.  Lanes: a row of up to 16 vectors takes 16 lanes (four rows a
-// wave, where a wave a row would leave most lanes idle), up to 4 vectors a lane a
-// wave, more the workgroup.
-Plan plan(int64_t D, int dt, bool al16, bool al4) {
-  const int full = dt == DT_BF16 ? 8 : 4;
-  int v = 1;
-  if (D % full == 0 && al16) v = full;
-  else if (dt == DT_BF16 && D % 2 == 0 && al4) v = 2;
-  const int most = v == 1 ? 32 : (v == 2 ? 16 : (v == 4 ? 8 : 4));  // vectors a lane holds
+// A row of up to 16 vectors takes 16 lanes (four rows a wave, where a wave a row would
+// leave most lanes idle), up to 4 vectors a lane a wave, more of it the workgroup, whose
+// sums have two barriers each.  16384 bf16 rows of 2048 (4 vectors a lane): a wave 28 us
+// forward and 45 backward, the workgroup 31 and 60; 5001 fp32 rows of 1131, 5 vectors a
+// lane in a wave: 18 and 38 us, the workgroup 15 and 25.
+Plan plan(int64_t D, int dt) {
+  const int v = dt == DT_BF16 ? 8 : 4;
   const int64_t n = (D + v - 1) / v;
-  if (n <= 16) return {v, 1, 16};
-  for (int tpr : {64, 256}) {
-    const int64_t nv = (n + tpr - 1) / tpr;
-    if (nv <= most) {
-      int r = 1;
-      while (r < nv) r <<= 1;
-      return {v, r, tpr};
-    }
-  }
-  return {v, 0, 256};
+  if (n <= 16) return {1, 16};
+  const int tpr = n <= 4 * 64 ? 64 : 256;
+  const int64_t nv = (n + tpr - 1) / tpr;
+  return {nv <= 1 ? 1 : (nv <= 2 ? 2 : (nv <= 4 ? 4 : (nv <= 8 ? 8 : 0))), tpr};
 }
 
 template <typename F>
-void with_plan(const Plan& p, int dt, F&& f) {
+void with_plan(const Plan& p, int dt, int64_t D, F&& f) {
 #define MOC_NORM_CASE(DT, V, NV, TPR) \
-  if (dt == DT && p.v == V && p.nv == NV && p.tpr == TPR) \
-    return f(std::integral_constant<int, DT>{}, std::integral_constant<int, V>{}, std::integral_constant<int, NV>{}, \
-             std::integral_constant<int, TPR>{});
-#define MOC_NORM_WIDE(DT, V, NV) MOC_NORM_CASE(DT, V, NV, 64) MOC_NORM_CASE(DT, V, NV, 256)
-  MOC_NORM_CASE(DT_BF16, 8, 1, 16) MOC_NORM_CASE(DT_BF16, 2, 1, 16) MOC_NORM_CASE(DT_BF16, 1, 1, 16)
-  MOC_NORM_CASE(DT_F32, 4, 1, 16) MOC_NORM_CASE(DT_F32, 1, 1, 16)
-  MOC_NORM_WIDE(DT_BF16, 8, 1) MOC_NORM_WIDE(DT_BF16, 8, 2) MOC_NORM_WIDE(DT_BF16, 8, 4)
-  MOC_NORM_WIDE(DT_BF16, 2, 1) MOC_NORM_WIDE(DT_BF16, 2, 2) MOC_NORM_WIDE(DT_BF16, 2, 4)
-  MOC_NORM_WIDE(DT_BF16, 2, 8) MOC_NORM_WIDE(DT_BF16, 2, 16)
-  MOC_NORM_WIDE(DT_BF16, 1, 1) MOC_NORM_WIDE(DT_BF16, 1, 2) MOC_NORM_WIDE(DT_BF16, 1, 4)
-  MOC_NORM_WIDE(DT_BF16, 1, 8) MOC_NORM_WIDE(DT_BF16, 1, 16) MOC_NORM_WIDE(DT_BF16, 1, 32)
-  MOC_NORM_WIDE(DT_F32, 4, 1) MOC_NORM_WIDE(DT_F32, 4, 2) MOC_NORM_WIDE(DT_F32, 4, 4) MOC_NORM_WIDE(DT_F32, 4, 8)
-  MOC_NORM_WIDE(DT_F32, 1, 1) MOC_NORM_WIDE(DT_F32, 1, 2) MOC_NORM_WIDE(DT_F32, 1, 4)
-  MOC_NORM_WIDE(DT_F32, 1, 8) MOC_NORM_WIDE(DT_F32, 1, 16) MOC_NORM_WIDE(DT_F32, 1, 32)
-#undef MOC_NORM_WIDE
+  if (dt == DT && p.nv == NV && p.tpr == TPR) { \
+    if (D % V == 0) f(Int<DT>{}, Int<V>{}, Int<NV>{}, Int<TPR>{}, std::false_type{}); \
+    else f(Int<DT>{}, Int<V>{}, Int<NV>{}, Int<TPR>{}, std::true_type{}); \
+    return; \
+  }
+#define MOC_NORM_TYPE(DT, V) \
+  MOC_NORM_CASE(DT, V, 1, 16) MOC_NORM_CASE(DT, V, 1, 64) MOC_NORM_CASE(DT, V, 2, 64) MOC_NORM_CASE(DT, V, 4, 64) \
+  MOC_NORM_CASE(DT, V, 2, 256) MOC_NORM_CASE(DT, V, 4, 256) MOC_NORM_CASE(DT, V, 8, 256)
+  MOC_NORM_TYPE(DT_BF16, 8) MOC_NORM_TYPE(DT_F32, 4)
+#undef MOC_NORM_TYPE
 #undef MOC_NORM_CASE
 }
 
-// Workgroups of a kernel that walks rows (a grid's threads are counted in 32 bits).
-unsigned grid(int64_t n) { return static_cast<unsigned>(n < (1 << 22) ? n : (1 << 22)); }
+// Workgroups of the forward: four a CU, or what the rows give; of the long kernels: a row
+// each, as long as a grid counts them.
+constexpr int64_t kWalkers = 1024;
+unsigned grid(int64_t n, int64_t most) { return static_cast<unsigned>(n < most ? n : most); }
 
 // Workgroups of the backward, and rows of partial sums: two a CU, or what the rows
 // give.
@@ -372,16 +378,16 @@ size_t norm_backward_workspace(int64_t rows, int64_t D) { return size_t(parts(ro
 
 void norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows,
                   int64_t D, int dt, int w_dt, int b_dt, float eps, hipStream_t st) {
-  const Plan p = plan(D, dt, aligned({x, y}, 16), aligned({x, y}, 4));
+  const Plan p = plan(D, dt);
   if (p.nv == 0) {
     auto* k = dt == DT_BF16 ? norm_fwd_long<DT_BF16> : norm_fwd_long<DT_F32>;
-    hipLaunchKernelGGL(k, dim3(grid(rows)), dim3(kThreads), 0, st, x, w, b, y, mean, rstd, rows, D, w_dt, b_dt, eps);
+    hipLaunchKernelGGL(k, dim3(grid(rows, 1 << 22)), dim3(kThreads), 0, st, x, w, b, y, mean, rstd, rows, D, w_dt, b_dt, eps);
     return;
   }
-  with_plan(p, dt, [&](auto DT, auto V, auto NV, auto TPR) {
+  with_plan(p, dt, D, [&](auto DT, auto V, auto NV, auto TPR, auto TAIL) {
     constexpr int rpw = kThreads / TPR.value;
-    hipLaunchKernelGGL((norm_fwd<DT.value, V.value, NV.value, TPR.value>),
-                       dim3(grid((rows + rpw - 1) / rpw)), dim3(kThreads), 0, st, x, w, b, y, mean, rstd, rows,
+    hipLaunchKernelGGL((norm_fwd<DT.value, V.value, NV.value, TPR.value, TAIL.value>),
+                       dim3(grid((rows + rpw - 1) / rpw, kWalkers)), dim3(kThreads), 0, st, x, w, b, y, mean, rstd, rows,
                        static_cast<int>(D), w_dt, b_dt, eps);
   });
 }
@@ -389,14 +395,14 @@ void norm_forward(const void* x, const void* w, const void* b, void* y, float* m
 void norm_backward(const void* x, const void* w, const void* dy, const float* mean, const float* rstd, void* dx,
                    void* dw, void* db, int64_t rows, int64_t D, int dt, int w_dt, int b_dt, void* workspace,
                    hipStream_t st) {
-  const Plan p = plan(D, dt, aligned({x, dy, dx}, 16), aligned({x, dy, dx}, 4));
+  const Plan p = plan(D, dt);
   float* part = static_cast<float*>(workspace);
   const bool sums = dw != nullptr || db != nullptr;
   int64_t n = parts(rows);
   if (p.nv == 0) {
     if (dx != nullptr) {
       auto* k = dt == DT_BF16 ? norm_dx_long<DT_BF16> : norm_dx_long<DT_F32>;
-      hipLaunchKernelGGL(k, dim3(grid(rows)), dim3(kThreads), 0, st, x, w, dy, mean, rstd, dx, rows, D, w_dt);
+      hipLaunchKernelGGL(k, dim3(grid(rows, 1 << 22)), dim3(kThreads), 0, st, x, w, dy, mean, rstd, dx, rows, D, w_dt);
     }
     if (sums) {
       if (n > 64) n = 64;
@@ -405,13 +411,13 @@ void norm_backward(const void* x, const void* w, const void* dy, const float* me
                          dim3(kThreads), 0, st, x, dy, mean, rstd, part, rows, D);
     }
   } else {
-    with_plan(p, dt, [&](auto DT, auto V, auto NV, auto TPR) {
+    with_plan(p, dt, D, [&](auto DT, auto V, auto NV, auto TPR, auto TAIL) {
       constexpr int rpw = kThreads / TPR.value;
       const int64_t wgs = (rows + rpw - 1) / rpw;
       if (wgs < n) n = wgs;
       const size_t lds = TPR.value == kThreads ? 0 : size_t(2 * D) * sizeof(float);
-      auto* k = sums ? norm_bwd<DT.value, V.value, NV.value, TPR.value, true>
-                     : norm_bwd<DT.value, V.value, NV.value, TPR.value, false>;
+      auto* k = sums ? norm_bwd<DT.value, V.value, NV.value, TPR.value, TAIL.value, true>
+                     : norm_bwd<DT.value, V.value, NV.value, TPR.value, TAIL.value, false>;
       hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(n)), dim3(kThreads), sums ? lds : 0, st, x, w, dy, mean, rstd,
                          dx, part, rows, static_cast<int>(D), w_dt);
     });

@@ -217,7 +217,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     seq = [_p, _i, _l, _l, _l]         # cu_seqlens, cu_seqlens_i64, n_seqs, n_tokens, seq_len
     conv = [_l, _l, _i, _i, _i, _i]    # dim, kernel_size, dtypes, activation
     lib.moc_conv_forward.argtypes = [_p] * 6 + seq + conv + [_p]
-    lib.moc_conv_backward_workspace_bytes.argtypes = [_l, _l, _l]
+    lib.moc_conv_backward_workspace_bytes.argtypes = [_l, _l, _l, _i]
     lib.moc_conv_backward_workspace_bytes.restype = _z
     lib.moc_conv_backward.argtypes = [_p] * 7 + seq + conv + [_p, _z, _p]
     lib.moc_conv_update.argtypes = [_p, _p, _p, _p, _l, _l, _l, _p, _l] + conv + [_p]

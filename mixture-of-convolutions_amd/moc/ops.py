@@ -741,7 +741,7 @@ def launch_conv_backward(x, weight, bias, dy, *, activation_flag: int, need_x, n
     db = torch.empty_like(bias) if need_b else None
     (wp, wd), (bp, bd) = _param(weight), _param(bias)
     with _lib.device_guard(x.device):
-        n = L.moc_conv_backward_workspace_bytes(n_tokens, D, S) if need_w or need_b else 0
+        n = L.moc_conv_backward_workspace_bytes(n_tokens, D, S, _lib.dtype_code(x.dtype)) if need_w or need_b else 0
         ws = _workspace(n, x.device)
         rc = L.moc_conv_backward(
             x.data_ptr(), wp, bp, dy.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), cu_ptr, cu64, n_seqs,

@@ -237,11 +237,11 @@ def test_capi_workspaces():
     L = _lib.lib()
     assert L.moc_norm_backward(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 4, 8, 1, 1, 0, FAKE,
                                L.moc_norm_backward_workspace_bytes(4, 8) - 1, None) == ERR_WORKSPACE
-    need = L.moc_conv_backward_workspace_bytes(100, 64, 4)
+    need = L.moc_conv_backward_workspace_bytes(100, 64, 4, 1)
     assert need >= 5 * 64 * 4
     assert L.moc_conv_backward(FAKE, FAKE, None, FAKE, FAKE, FAKE, None, None, 0, 0, 100, 50, 64, 4, 1, 1, 1, 0, FAKE,
                                need - 1, None) == ERR_WORKSPACE
-    assert L.moc_norm_backward_workspace_bytes(0, 8) == 0 and L.moc_conv_backward_workspace_bytes(4, 0, 1) == 0
+    assert L.moc_norm_backward_workspace_bytes(0, 8) == 0 and L.moc_conv_backward_workspace_bytes(4, 0, 1, 1) == 0
 
 
 @pytest.mark.parametrize("kw, code", [
