@@ -23,7 +23,7 @@ namespace moc {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kAhead = 4, kAheadBack = 2;  // rows loaded together
+constexpr int kAhead = 4;  // rows that the forward loads together
 
 struct ConvArgs {
   const void* x;
@@ -130,6 +130,9 @@ __global__ __launch_bounds__(64 * kWaves) void conv_fwd(ConvArgs a) {
 
 template <int DT, int S, int V>
 __global__ __launch_bounds__(64 * kWaves) void conv_bwd(ConvArgs a) {
+  // rows loaded together: S of them bring the windows' registers round without a move (4
+  // taps: 62 us with two rows, 56 with four; 3 taps: 24 with two, 29 with four)
+  constexpr int kAheadBack = S == 3 || S == 4 ? S : 2;
   __shared__ float lds[kWaves - 1][64 * V];
   const int64_t c = (int64_t(blockIdx.x) * 64 + (threadIdx.x & 63)) * V;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

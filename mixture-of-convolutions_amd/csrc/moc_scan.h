@@ -255,6 +255,86 @@ struct Rows {
   }
 };
 
+// Rows at a place that moves by a uniform offset (a head's columns of a token, a head's rows
+// of the states) under one buffer resource: `off` elements from base, row by row `stride`.
+// `have`: how many of the elements asked for are there (at most 0: none).  VEC as in Rows.
+template <int DT, bool VEC>
+struct Span {
+  static constexpr int E = DT == DT_BF16 ? 2 : 4;
+  const char* base;
+  int stride, n;
+  __device__ __forceinline__ Span(const void* p, int64_t at, int64_t stride_, int64_t n_)
+      : base(static_cast<const char*>(p) + at * E), stride(static_cast<int>(stride_)), n(static_cast<int>(n_)) {}
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, n * stride * E, 0x00020000);
+  }
+  __device__ __forceinline__ Raw<DT> get8(int row, int col, int have, int64_t off) const {
+    Raw<DT> v;
+    if constexpr (VEC) {
+      const int o = have > 0 ? (row * stride + col) * E : static_cast<int>(kNowhere);
+      const int s = static_cast<int>(off) * E;
+      if constexpr (DT == DT_BF16) {
+        v.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), o, s, 0));
+      } else {
+        v.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), o, s, 0));
+        v.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), o + 16, s, 0));
+      }
+    } else {
+      if (row >= n) have = 0;
+      const int64_t at = int64_t(row) * stride + col + off;
+      if constexpr (DT == DT_BF16) {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + at;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a = 2 * k < have ? p[2 * k] : 0u, b = 2 * k + 1 < have ? p[2 * k + 1] : 0u;
+          v.w[k] = a | (b << 16);
+        }
+      } else {
+        const float* p = reinterpret_cast<const float*>(base) + at;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v.lo[k] = k < have ? p[k] : 0.f;
+          v.hi[k] = 4 + k < have ? p[4 + k] : 0.f;
+        }
+      }
+    }
+    return v;
+  }
+  __device__ __forceinline__ f32x4 get4(int row, int col, int have) const {
+    f32x4 v;
+    if constexpr (VEC) {
+      const int o = have > 0 ? (row * stride + col) * E : static_cast<int>(kNowhere);
+      if constexpr (DT == DT_BF16) {
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc(), o, 0, 0));
+        v = f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
+      } else {
+        v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), o, 0, 0));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = row < n && k < have ? load_any(base, DT, int64_t(row) * stride + col + k) : 0.f;
+    }
+    return v;
+  }
+  __device__ __forceinline__ void put4(int row, int col, int have, int64_t off, f32x4 v) const {
+    if constexpr (VEC) {
+      const int o = have > 0 ? (row * stride + col) * E : static_cast<int>(kNowhere);
+      const int s = static_cast<int>(off) * E;
+      if constexpr (DT == DT_BF16) {
+        const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
+        __builtin_amdgcn_raw_buffer_store_b64(w, rsrc(), o, s, 0);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rsrc(), o, s, 0);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (row < n && k < have)
+          store_any(const_cast<char*>(base), DT, int64_t(row) * stride + col + k + off, v[k]);
+    }
+  }
+};
+
 // An LDS tile of bf16 planes, W = 64, 128 or 256 columns.  Blocks of 8 columns (16 bytes)
 // of a row are permuted by an exclusive or with f(row), so that both kinds of operand
 // reads meet every bank once: rows li = 0..15 at one block (get8: f takes 16 values, or 8
@@ -369,6 +449,13 @@ struct Staged {
   __device__ __forceinline__ void load(const Rows<DT, VEC>& src) {
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) v[k] = src.get8(row(0), col(k), k * (THREADS / (W / 8)));
+  }
+  // rows 0..rows of a span at `off`, `cols` columns of them
+  __device__ __forceinline__ void load(const Span<DT, VEC>& src, int rows, int cols, int64_t off) {
+    constexpr int kStep = THREADS / (W / 8);
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k)
+      v[k] = src.get8(row(0), col(k), row(0) + k * kStep < rows ? cols - col(k) : 0, off + int64_t(k) * kStep * src.stride);
   }
   template <int NP>
   __device__ __forceinline__ void put(const Tile<NP, W>& t) const {

@@ -565,7 +565,9 @@ Args make_args(const Scan& p, void* prep) {
   a.u = static_cast<float*>(prep);
   a.s = reinterpret_cast<double*>(static_cast<char*>(prep) + up(n * 4));
   a.vec = p.P % 8 == 0 && p.N % 8 == 0 && aligned({p.x, p.B, p.C}, 16);
-  for (int64_t st : {p.x_stride, p.b_stride, p.c_stride, p.H * p.P}) a.vec = a.vec && st % 8 == 0 && st < kMaxStride;
+  // (a chunk's states lie under one buffer resource)
+  a.vec = a.vec && p.H * p.P * p.N * 4 < int64_t(kNowhere) - 16;
+  for (int64_t st : {p.x_stride, p.b_stride, p.c_stride, p.H * p.P, p.G * p.N}) a.vec = a.vec && st % 8 == 0 && st < kMaxStride;
   return a;
 }
 

@@ -43,12 +43,25 @@ struct Back {
 
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
+// v of the lane N places on in its group of 16
+template <int N>
+__device__ __forceinline__ float rotate(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, true));
+}
+template <int N>
+__device__ __forceinline__ double rotate(double v) {
+  const uint64_t w = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(w), 0x120 + N, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(w >> 32), 0x120 + N, 0xf, 0xf, true);
+  return __longlong_as_double((static_cast<uint64_t>(hi) << 32) | lo);
+}
 // sum over lanes i % 16 (column sums of a result block)
 template <typename T>
 __device__ __forceinline__ T sum16(T v) {
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) v += __shfl_xor(v, m);
-  return v;
+  v += rotate<8>(v);
+  v += rotate<4>(v);
+  v += rotate<2>(v);
+  return v + rotate<1>(v);
 }
 // sum over lane groups (row sums)
 template <typename T>
@@ -137,8 +150,13 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   const int n = c.n, ptiles = (P + kTile - 1) / kTile, ntiles = (N + 63) / 64;
   const bool use_h = !c.first || b.has_init, use_dh = !c.last || b.has_dfin;
   const int64_t gcol = int64_t(grp) * N;
-  const Rows<DT, VEC> brow(a.p.B, c.t0 * a.p.b_stride + gcol, a.p.b_stride, n, N);
-  const Rows<DT, VEC> crow(a.p.C, c.t0 * a.p.c_stride + gcol, a.p.c_stride, n, N);
+  const Span<DT, VEC> brow(a.p.B, c.t0 * a.p.b_stride + gcol, a.p.b_stride, n);
+  const Span<DT, VEC> crow(a.p.C, c.t0 * a.p.c_stride + gcol, a.p.c_stride, n);
+  const Span<DT, VEC> xrow(a.p.x, c.t0 * a.p.x_stride, a.p.x_stride, n);
+  const Span<DT, VEC> yrow(b.dy, c.t0 * H * P, int64_t(H) * P, n);
+  const Span<DT, VEC> orow(b.dx, c.t0 * H * P, int64_t(H) * P, n);
+  const Span<DT, VEC> hrow(b.h, c.id * H * P * N, N, int64_t(H) * P);
+  const Span<DT, VEC> drow(b.dh, c.id * H * P * N, N, int64_t(H) * P);
   const int i = 16 * wave + li;  // this lane's row i of G, V (result column)
   auto blk = [&](int k) { return k * kHalves + half; };  // this wave's column blocks
 
@@ -147,41 +165,38 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   Staged<DT, VEC, W, kBack> sh, sd;
   double sv = 0.0;
   float uv = 0.f;
+  auto width = [&](int pt) { return P - pt * kTile < kTile ? P - pt * kTile : kTile; };
   auto fetch_states = [&](int h, int pt, int nt) {
-    const int p0 = pt * kTile, cols = P - p0 < kTile ? P - p0 : kTile, n0 = nt * 64;
-    const int64_t at = ((c.id * H + h) * P + p0) * N + n0;
-    const int width = N - n0 < W ? N - n0 : W;
-    sh.load(Rows<DT, VEC>(b.h, at, N, use_h ? cols : 0, width));
-    sd.load(Rows<DT, VEC>(b.dh, at, N, use_dh ? cols : 0, width));
+    const int64_t off = (int64_t(h) * P + pt * kTile) * N + nt * 64;
+    sh.load(hrow, use_h ? width(pt) : 0, N - nt * 64, off);
+    sd.load(drow, use_dh ? width(pt) : 0, N - nt * 64, off);
   };
   auto fetch = [&](int h, int pt) {
-    const int p0 = pt * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
-    sx.load(Rows<DT, VEC>(a.p.x, c.t0 * a.p.x_stride + int64_t(h) * P + p0, a.p.x_stride, n, cols));
-    sy.load(Rows<DT, VEC>(b.dy, (c.t0 * H + h) * P + p0, int64_t(H) * P, n, cols));
+    const int off = h * P + pt * kTile;
+    sx.load(xrow, kQ, width(pt), off);
+    sy.load(yrow, kQ, width(pt), off);
     fetch_states(h, pt, 0);
     const int64_t at = (int64_t(h) * a.chunks + c.id) * kQ + lane;
     if (pt == 0) sv = a.s[at], uv = a.u[at];
   };
   fetch(h_lo, 0);
 
-  // G^T blocks [j][i] of row block `wave`
+  // G^T blocks [j][i] of row block `wave` (above the diagonal too: no branch parts the code)
   f32x4 gm[Q], ds[Q];
 #pragma unroll
   for (int k = 0; k < Q; ++k) gm[k] = ds[k] = zero4();
   if (LY::kBInLds) {
     Staged<DT, VEC, W, kBack> sb;
-    sb.load(brow);
+    sb.load(brow, kQ, N, 0);
     sb.put(bt);
   }
 #pragma unroll
   for (int ks = 0; ks < 2 * NT; ++ks) {
-    const Frag<NP> cf = crow.get8(i, 32 * ks + 8 * g).frag();
+    const int col = 32 * ks + 8 * g;
+    const Frag<NP> cf = crow.get8(i, col, N - col, 0).frag();
 #pragma unroll
-    for (int k = 0; k < Q; ++k)
-      if (blk(k) <= wave) gm[k] = mm(brow.get8(16 * blk(k) + li, 32 * ks + 8 * g).frag(), cf, gm[k]);
+    for (int k = 0; k < Q; ++k) gm[k] = mm(brow.get8(16 * blk(k) + li, col, N - col, 0).frag(), cf, gm[k]);
   }
-  // the block right of the diagonal that a 32-token product step reads (no other wave writes it)
-  if ((wave & 1) == 0 && half == (wave + 1) % kHalves) mt.put4(lx, wave, wave + 1, zero4());
   // dB^T, dC^T blocks: states 64 nt + 16 wave + 4 g + r, tokens 16 blk + li
   f32x4 dBa[NT][Q], dCa[NT][Q];
 #pragma unroll
@@ -202,24 +217,19 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 #pragma unroll 1
     for (int pt = 0; pt < ptiles; ++pt) {
       lx.refresh(), lw.refresh();
-      const int p0 = pt * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
       if (pt > 0) __syncthreads();  // (the last tile's readers; a head's last barrier is behind them too)
-      if (a.p.D != nullptr) {
 #pragma unroll
-        for (int k = 0; k < sx.kLoads; ++k) xy += dot<Acc>(sx.v[k], sy.v[k]);
-      }
+      for (int k = 0; k < sx.kLoads; ++k) xy += dot<Acc>(sx.v[k], sy.v[k]);
       if (pt == 0) dec.put(wave, sv, uv);  // (both halves write the same)
       sx.put(xt);
       sy.put(yt);
       auto put_states = [&]() {
-        if (use_h && use_dh) {
 #pragma unroll
-          for (int k = 0; k < sh.kLoads; ++k) za += dot<Acc>(sh.v[k], sd.v[k]);
-        }
-        if (use_h) sh.put(ht);
-        if (use_dh) sd.put(dt);
+        for (int k = 0; k < sh.kLoads; ++k) za += dot<Acc>(sh.v[k], sd.v[k]);
+        sh.put(ht);
+        sd.put(dt);
       };
-      put_states();
+      if (use_h || use_dh) put_states();
       __syncthreads();
       // V^T, then W and what of it goes where
       {
@@ -230,52 +240,37 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
         for (int ks = 0; ks < 2; ++ks) {
           const Frag<NP> yf = yt.get8(lx, wave, ks);
 #pragma unroll
-          for (int k = 0; k < Q; ++k)
-            if (blk(k) <= wave) vm[k] = mm(xt.get8(lx, blk(k), ks), yf, vm[k]);
+          for (int k = 0; k < Q; ++k) vm[k] = mm(xt.get8(lx, blk(k), ks), yf, vm[k]);
         }
-        settle();
-        const float ai = dec.a[i];
+        const double si = dec.s[i];
 #pragma unroll
         for (int k = 0; k < Q; ++k) {
-          const int jb = blk(k);
-          if (jb > wave) continue;
-          const f32x4 u = *reinterpret_cast<const f32x4*>(dec.u + 16 * jb + 4 * g);
-          f32x4 L;
-          if (jb < wave) {
-            L = (ai * dec.between(wave, jb)) * *reinterpret_cast<const f32x4*>(dec.b + 16 * jb + 4 * g);
-          } else {
-            const double si = dec.s[i];
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              L[r] = __builtin_amdgcn_exp2f(static_cast<float>(si - dec.s[16 * jb + 4 * g + r]));
-          }
-          f32x4 gl = gm[k] * L, vl = vm[k] * (L * u);
+          const int j0 = 16 * blk(k) + 4 * g;
+          const f32x4 u = *reinterpret_cast<const f32x4*>(dec.u + j0);
+          f32x4 gl;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const bool in = jb < wave || 4 * g + r <= li, diag = jb == wave && 4 * g + r == li;
-            gl[r] = in ? gl[r] : 0.f;
-            vl[r] = in ? vl[r] : 0.f;
-            const float wv = in ? gl[r] * vm[k][r] : 0.f;
-            if (diag) {
-              da += wv;
-            } else {
-              ka[k][r] += wv;
-              ra += static_cast<Acc>(u[r]) * wv;
-            }
+            const bool in = j0 + r <= i, diag = j0 + r == i;
+            const float L = __builtin_amdgcn_exp2f(static_cast<float>(si - dec.s[j0 + r]));
+            const float gv = gm[k][r] * L, vv = vm[k][r] * (L * u[r]), wv = gv * vm[k][r];
+            gl[r] = in ? gv : 0.f;
+            ds[k][r] += in ? vv : 0.f;
+            da += diag ? wv : 0.f;
+            const float below = in && !diag ? wv : 0.f;
+            ka[k][r] += below;
+            ra += static_cast<Acc>(u[r]) * below;
           }
-          ds[k] += vl;
-          if (pt == 0) mt.put4(lx, wave, jb, gl);
+          if (pt == 0) mt.put4(lx, wave, blk(k), gl);
         }
       }
-      const bool active = 16 * wave < cols;
-      // dx^T[p][j]: channels p0 + 16 wave + 4 g + r, tokens 16 blk + li; the state's part first
+      // dx^T[p][j]: channels 64 pt + 16 wave + 4 g + r, tokens 16 blk + li; the state's part first
       f32x4 xa[Q];
 #pragma unroll
       for (int k = 0; k < Q; ++k) xa[k] = zero4();
 #pragma unroll
       for (int nt0 = 0; nt0 < NT; nt0 += TW) {
-        if (nt0 >= ntiles) continue;
-        if (nt0 > 0) {
+        if (TW < NT && nt0 >= ntiles) continue;
+        if (nt0 > 0 && (use_h || use_dh)) {
           __syncthreads();  // (the last state tile's readers)
           put_states();
           __syncthreads();
@@ -287,72 +282,59 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
         } else if (h + 1 < h_hi) {
           fetch(h + 1, 0);
         }
-        if (active && use_dh) {
+        if (!use_h && !use_dh) continue;
 #pragma unroll
-          for (int ks = 0; ks < 2 * TW; ++ks) {
-            const Frag<NP> df = dt.get8(lw, wave, ks);
+        for (int ks = 0; ks < 2 * TW; ++ks) {
+          const Frag<NP> df = dt.get8(lw, wave, ks);
 #pragma unroll
-            for (int k = 0; k < Q; ++k) {
-              const Frag<NP> bf = LY::kBInLds
-                                      ? bt.get8(lw, blk(k), ks)
-                                      : brow.get8(16 * blk(k) + li, 64 * nt0 + 32 * ks + 8 * g).frag();
-              xa[k] = mm(df, bf, xa[k]);
-            }
+          for (int k = 0; k < Q; ++k) {
+            const int col = 64 * nt0 + 32 * ks + 8 * g;
+            const Frag<NP> bf = LY::kBInLds ? bt.get8(lw, blk(k), ks)
+                                            : brow.get8(16 * blk(k) + li, col, N - col, 0).frag();
+            xa[k] = mm(df, bf, xa[k]);
           }
         }
         // states 64 nt + 16 wave + ...: h^T dy and dh^T x
 #pragma unroll
         for (int tw = 0; tw < TW; ++tw) {
-          const int nt = nt0 + tw;
-          if (64 * nt + 16 * wave >= N) continue;
-          if (use_h) {
-            const Frag<NP> h0 = ht.tr8(lw, 0, 4 * tw + wave), h1 = ht.tr8(lw, 1, 4 * tw + wave);
+          const int nt = nt0 + tw, sc = 64 * nt + 16 * wave + 4 * g;
+          const Frag<NP> h0 = ht.tr8(lw, 0, 4 * tw + wave), h1 = ht.tr8(lw, 1, 4 * tw + wave);
 #pragma unroll
-            for (int k = 0; k < Q; ++k) {
-              const f32x4 v = mm(h1, yt.get8(lx, blk(k), 1), mm(h0, yt.get8(lx, blk(k), 0), zero4()));
-              const f32x4 cv = crow.get4(16 * blk(k) + li, 64 * nt + 16 * wave + 4 * g);
-              dCa[nt][k] += dec.e[16 * blk(k) + li] * v;
+          for (int k = 0; k < Q; ++k) {
+            const f32x4 v = mm(h1, yt.get8(lx, blk(k), 1), mm(h0, yt.get8(lx, blk(k), 0), zero4()));
+            const f32x4 cv = crow.get4(16 * blk(k) + li, sc, N - sc);
+            dCa[nt][k] += dec.e[16 * blk(k) + li] * v;
 #pragma unroll
-              for (int r = 0; r < 4; ++r) qa[k] += static_cast<Acc>(v[r]) * cv[r];
-            }
+            for (int r = 0; r < 4; ++r) qa[k] += static_cast<Acc>(v[r]) * cv[r];
           }
-          if (use_dh) {
-            const Frag<NP> d0 = dt.tr8(lw, 0, 4 * tw + wave), d1 = dt.tr8(lw, 1, 4 * tw + wave);
+          const Frag<NP> d0 = dt.tr8(lw, 0, 4 * tw + wave), d1 = dt.tr8(lw, 1, 4 * tw + wave);
 #pragma unroll
-            for (int k = 0; k < Q; ++k) {
-              const f32x4 v = mm(d1, xt.get8(lx, blk(k), 1), mm(d0, xt.get8(lx, blk(k), 0), zero4()));
-              dBa[nt][k] += (dec.f[16 * blk(k) + li] * dec.u[16 * blk(k) + li]) * v;
-            }
+          for (int k = 0; k < Q; ++k) {
+            const f32x4 v = mm(d1, xt.get8(lx, blk(k), 1), mm(d0, xt.get8(lx, blk(k), 0), zero4()));
+            dBa[nt][k] += dec.w[16 * blk(k) + li] * v;
           }
         }
       }
-      if (active && use_dh) {
+      settle();
 #pragma unroll
-        for (int k = 0; k < Q; ++k) {
-          const f32x4 xv = xt.get4(lx, blk(k), wave);
+      for (int k = 0; k < Q; ++k) {
+        const f32x4 xv = xt.get4(lx, blk(k), wave);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) ga[k] += static_cast<Acc>(xv[r]) * xa[k][r];
-          xa[k] *= dec.f[16 * blk(k) + li];
-        }
+        for (int r = 0; r < 4; ++r) ga[k] += static_cast<Acc>(xv[r]) * xa[k][r];
+        xa[k] *= dec.f[16 * blk(k) + li];
       }
       __syncthreads();  // M is whole
-      if (active) {
-        const Rows<DT, VEC> out(b.dx, (c.t0 * H + h) * P + p0, int64_t(H) * P, n, cols);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const Frag<NP> yf = yt.tr8(lx, ks, wave);
+      for (int ks = 0; ks < 2; ++ks) {
+        const Frag<NP> yf = yt.tr8(lx, ks, wave);
 #pragma unroll
-          for (int k = 0; k < Q; ++k)
-            if (32 * ks + 31 >= 16 * blk(k)) xa[k] = mm(yf, mt.tr8(lx, ks, blk(k)), xa[k]);
-        }
-        settle();
+        for (int k = 0; k < Q; ++k) xa[k] = mm(yf, mt.tr8(lx, ks, blk(k)), xa[k]);
+      }
 #pragma unroll
-        for (int k = 0; k < Q; ++k) {
-          const int j = 16 * blk(k) + li;
-          f32x4 v = dec.u[j] * xa[k];
-          if (a.p.D != nullptr) v += skip * yt.get4(lx, blk(k), wave);
-          out.put4(j, 16 * wave + 4 * g, v);
-        }
+      for (int k = 0; k < Q; ++k) {
+        const int col = 16 * wave + 4 * g;
+        const f32x4 v = dec.u[16 * blk(k) + li] * xa[k] + skip * yt.get4(lx, blk(k), wave);
+        orow.put4(16 * blk(k) + li, col, width(pt) - col, h * P + pt * kTile, v);
       }
     }
     // the head's sums over channels and states
@@ -377,7 +359,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
     if (lane == 0) zp[0][wid] = za, zp[1][wid] = xy;
     const float u = dec.u[lane], e = dec.e[lane], f = dec.f[lane], e_last = dec.e[kQ - 1];
     __syncthreads();  // the sums are whole, every tile and factor has been read
-    if (wid == 0) {
+    if (wid == (h & 7)) {  // (each head another wave's: the others go on)
       const int t = lane;
       auto four = [&](const Acc* p) { return (p[t] + p[kQ + t]) + (p[2 * kQ + t] + p[3 * kQ + t]); };
       const Acc K = four(Kp), q = e * four(qp), gt = f * four(gp);
@@ -410,41 +392,38 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   }
   // what the chunk's own tokens give of dB and dC, summed over the heads
 #pragma unroll
-  for (int k = 0; k < Q; ++k)
-    if (blk(k) <= wave) mt.put4(lx, wave, blk(k), ds[k]);
+  for (int k = 0; k < Q; ++k) mt.put4(lx, wave, blk(k), ds[k]);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     if (nt >= ntiles) continue;
     lx.refresh();
     __syncthreads();
-    sx.load(Rows<DT, VEC>(a.p.B, c.t0 * a.p.b_stride + gcol + 64 * nt, a.p.b_stride, n, N - 64 * nt));
-    sy.load(Rows<DT, VEC>(a.p.C, c.t0 * a.p.c_stride + gcol + 64 * nt, a.p.c_stride, n, N - 64 * nt));
+    sx.load(brow, kQ, N - 64 * nt, 64 * nt);
+    sy.load(crow, kQ, N - 64 * nt, 64 * nt);
     sx.put(xt);
     sy.put(yt);
     __syncthreads();
-    const int sc = 64 * nt + 16 * wave;
-    if (sc >= N) continue;
+    const int sc = 64 * nt + 16 * wave + 4 * g;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const Frag<NP> bf = xt.tr8(lx, ks, wave), cf = yt.tr8(lx, ks, wave);
 #pragma unroll
       for (int k = 0; k < Q; ++k) {
-        // dC_i: j <= i; dB_j: i >= j
-        if (32 * ks < 16 * blk(k) + 16) dCa[nt][k] = mm(bf, mt.get8(lx, blk(k), ks), dCa[nt][k]);
-        if (32 * ks + 31 >= 16 * blk(k)) dBa[nt][k] = mm(cf, mt.tr8(lx, ks, blk(k)), dBa[nt][k]);
+        dCa[nt][k] = mm(bf, mt.get8(lx, blk(k), ks), dCa[nt][k]);
+        dBa[nt][k] = mm(cf, mt.tr8(lx, ks, blk(k)), dBa[nt][k]);
       }
     }
-    settle();
     const int64_t at = (c.t0 * G + grp) * N, all = a.p.seq.n_tokens * int64_t(G) * N * sub;
+    settle();
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
       const int t = 16 * blk(k) + li;
       if (b.subs == 1) {
-        Rows<DT, VEC>(b.dB, at, int64_t(G) * N, n, N).put4(t, sc + 4 * g, dBa[nt][k]);
-        Rows<DT, VEC>(b.dC, at, int64_t(G) * N, n, N).put4(t, sc + 4 * g, dCa[nt][k]);
+        Span<DT, VEC>(b.dB, at, int64_t(G) * N, n).put4(t, sc, N - sc, 0, dBa[nt][k]);
+        Span<DT, VEC>(b.dC, at, int64_t(G) * N, n).put4(t, sc, N - sc, 0, dCa[nt][k]);
       } else {
-        Rows<DT_F32, VEC>(b.dB_part, all + at, int64_t(G) * N, n, N).put4(t, sc + 4 * g, dBa[nt][k]);
-        Rows<DT_F32, VEC>(b.dC_part, all + at, int64_t(G) * N, n, N).put4(t, sc + 4 * g, dCa[nt][k]);
+        Span<DT_F32, VEC>(b.dB_part, all + at, int64_t(G) * N, n).put4(t, sc, N - sc, 0, dBa[nt][k]);
+        Span<DT_F32, VEC>(b.dC_part, all + at, int64_t(G) * N, n).put4(t, sc, N - sc, 0, dCa[nt][k]);
       }
     }
   }
