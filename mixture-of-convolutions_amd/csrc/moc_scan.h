@@ -337,9 +337,12 @@ struct Span {
 
 // An LDS tile of bf16 planes, W = 64, 128 or 256 columns.  Blocks of 8 columns (16 bytes)
 // of a row are permuted by an exclusive or with f(row), so that both kinds of operand
-// reads meet every bank once: rows li = 0..15 at one block (get8: f takes 16 values, or 8
-// on the rows of one parity where two rows share the banks, W = 64), and rows {0..3, 8..11}
-// or {4..7, 12..15} at two neighbouring blocks (tr8: so do f's upper bits).
+// reads meet every bank once.  A 16-byte read serves 16 lanes at a time: rows 0-3 and 12-15
+// at block g with rows 4-11 at block g + 1, or the other way about (lanes 0-3, 12-15, 20-27,
+// then the rest of 32), and their blocks must all differ (for W = 64, where two rows share
+// the banks, those of rows of one parity).  A transposed read meets rows {0-3, 8-11} or
+// {4-7, 12-15} at pairs of blocks, which f's bits but the lowest must keep apart.  With r the
+// row's bits, (r2 ^ r3, r3) as f's low bits does both, r1 (and r0 for W > 64) above them.
 //
 // Offsets are (a lane's own) ^ (the column's part) + (the row block's part):
 //   nat   row li, block g           (8 elements: column 8 g)
@@ -349,8 +352,8 @@ template <int W>
 struct Lane {
   int nat, quad, tr;
   static __device__ __forceinline__ int f(int row) {
-    if (W == 64) return ((row >> 1 & 1) << 2) | ((row >> 3 & 1) << 1) | (row >> 2 & 1);
-    return ((row & 1) << 3) | ((row >> 1 & 1) << 2) | ((row >> 3 & 1) << 1) | (row >> 2 & 1);
+    const int low = (((row >> 2 ^ row >> 3) & 1) << 1) | (row >> 3 & 1);
+    return W == 64 ? ((row >> 1 & 1) << 2) | low : ((row & 1) << 3) | ((row >> 1 & 1) << 2) | low;
   }
   __device__ __forceinline__ Lane() {
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
@@ -424,10 +427,10 @@ struct Tile {
   // A transposed operand: entry k of lane (li, g) is element [32 ks + 8 g + k][16 cb + li].
   // Two ds_read_b64_tr_b16 a plane: lane i of a 16-lane group gets element i % 4 of the
   // 8-byte rows read by lanes i / 4 + {0, 4, 8, 12}, so lane L reads row L / 4 of four,
-  // columns 4 (L % 4)..; the next four rows differ in one bit of f.
+  // columns 4 (L % 4)..; the next four rows differ in one bit of f (two blocks).
   __device__ __forceinline__ Frag<NP> tr8(const Lane<W>& l, int ks, int cb) const {
     const int o = l.tr ^ (16 * cb);
-    const uint16_t *q = p + o + 32 * ks * W, *q2 = p + (o ^ 8) + (32 * ks + 4) * W;
+    const uint16_t *q = p + o + 32 * ks * W, *q2 = p + (o ^ 16) + (32 * ks + 4) * W;
     Frag<NP> r;
 #pragma unroll
     for (int k = 0; k < NP; ++k)
