@@ -456,6 +456,8 @@ struct Staged {
   // rows 0..rows of a span at `off`, `cols` columns of them
   __device__ __forceinline__ void load(const Span<DT, VEC>& src, int rows, int cols, int64_t off) {
     constexpr int kStep = THREADS / (W / 8);
+    // (without a resource's range check the span's own end is checked here, for every step)
+    if (!VEC && rows > src.n) rows = src.n;
 #pragma unroll
     for (int k = 0; k < kLoads; ++k)
       v[k] = src.get8(row(0), col(k), row(0) + k * kStep < rows ? cols - col(k) : 0, off + int64_t(k) * kStep * src.stride);

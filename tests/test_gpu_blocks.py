@@ -448,6 +448,29 @@ def test_scan_reads_slices_in_place(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("H, P, G, N", [(6, 33, 3, 100), (2, 40, 1, 128), (2, 72, 1, 130), (2, 80, 1, 256), (3, 5, 1, 7)])
+def test_scan_uses_nothing_behind_the_last_token(dtype, H, P, G, N):
+    """Whatever lies behind the last token of x, dt, B and C in memory (here NaN or 0) changes no bit."""
+    T = 130
+    ins = scan_inputs((1, T), H, P, G, N, dtype)
+    dy = rnd(1, T, H, P, seed=9, dtype=dtype)
+    results = []
+    for tail in (0.0, float("nan")):
+        leaves = {}
+        for q, t in ins.items():
+            if q in ("x", "dt", "B", "C"):
+                t = torch.cat([t, torch.full_like(t[:, :64], tail)], 1)
+            leaves[q] = dev(t).requires_grad_()
+        cut = {q: t[:, :T] if q in ("x", "dt", "B", "C") else t for q, t in leaves.items()}
+        y, fin = moc.selective_scan(**cut, output_final_state=True, dt_softplus=True)
+        dyt = torch.cat([dy, torch.full_like(dy[:, :64], tail)], 1)
+        g = torch.autograd.grad([y], list(leaves.values()), [dev(dyt)[:, :T]])
+        results.append((y, fin, *(t[:, :T] if t.ndim > 1 else t for t in g)))
+    for a, b in zip(*results):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("H, P, G, N", [(2, 64, 1, 128), (3, 5, 3, 7), (4, 80, 2, 16), (1, 128, 1, 256), (2, 16, 1, 1)])
 def test_scan_steps(dtype, H, P, G, N):
     ins = scan_inputs((3, 6), H, P, G, N, dtype)
