@@ -578,6 +578,7 @@ struct Args {
   int64_t seg;      // tokens of a segment
   float* u;         // [H][chunks][kQ] softplus(dt + bias), 0 behind a sequence's end
   double* s;        // [H][chunks][kQ] running sum of u A log2(e) within the chunk
+  float* par;       // [H][2] A and D (or 0)
   bool vec;         // 16-byte accesses of everything that the kernels load and store
 };
 

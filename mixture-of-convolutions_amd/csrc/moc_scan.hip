@@ -31,9 +31,14 @@ using Int = std::integral_constant<int, V>;
 // neighbours), heads for the loads.
 __global__ __launch_bounds__(kThreads) void prep_kernel(Args a) {
   __shared__ float raw[16][kQ + 1];
+  const int h0 = blockIdx.y * 16;
+  if (blockIdx.x == 0 && threadIdx.x < 16 && h0 + threadIdx.x < a.p.H) {
+    const int64_t h = h0 + threadIdx.x;
+    a.par[2 * h] = load_any(a.p.A, a.p.a_dt, h);
+    a.par[2 * h + 1] = a.p.D == nullptr ? 0.f : load_any(a.p.D, a.p.d_dt, h);
+  }
   Chunk c;
   if (!chunk_at(a, blockIdx.x, c)) return;
-  const int h0 = blockIdx.y * 16;
   for (int k = threadIdx.x; k < 16 * kQ; k += kThreads) {
     const int t = k >> 4, h = h0 + (k & 15);
     if (t < c.n && h < a.p.H) raw[k & 15][t] = load_any(a.p.dt, a.p.x_dt, (c.t0 + t) * a.p.dt_stride + h);
@@ -530,7 +535,7 @@ bool segmented(const Args& a) { return a.seg < (a.seqs.l.cu == nullptr ? a.seqs.
 size_t prep_bytes(const Scan& p) {
   Args a = make_args(p, nullptr);
   const size_t n = size_t(p.H) * a.chunks * kQ;
-  return up(n * 4) + up(n * 8);
+  return up(n * 4) + up(n * 8) + up(size_t(p.H) * 8);
 }
 
 // Segments: a walk's workgroups are heads x segments, and 768 of them are on the card at
@@ -564,6 +569,7 @@ Args make_args(const Scan& p, void* prep) {
   const size_t n = size_t(p.H) * a.chunks * kQ;
   a.u = static_cast<float*>(prep);
   a.s = reinterpret_cast<double*>(static_cast<char*>(prep) + up(n * 4));
+  a.par = reinterpret_cast<float*>(static_cast<char*>(prep) + up(n * 4) + up(n * 8));
   a.vec = p.P % 8 == 0 && p.N % 8 == 0 && aligned({p.x, p.B, p.C}, 16);
   // (a chunk's states lie under one buffer resource)
   a.vec = a.vec && p.H * p.P * p.N * 4 < int64_t(kNowhere) - 16;

@@ -94,12 +94,14 @@ __device__ __forceinline__ Acc dot(const Raw<DT_F32>& a, const Raw<DT_F32>& b) {
 template <int DT, int NT>
 struct Layout {
   static constexpr int NP = kPlanes<DT>;
-  // state tiles of 64 at a time: all of them and B's beside them (bf16), or one (three planes)
+  // state tiles of 64 at a time: all of them, with B's and C's beside them (bf16: loads return
+  // in order, so that one of B or C behind the next head's would wait for those, 296 -> 277 us
+  // at 16384 tokens, 32 heads, 64 x 128), or one (three planes, which leave no room for B and C)
   static constexpr int TW = DT == DT_BF16 ? NT : 1, W = 64 * TW;
-  static constexpr bool kBInLds = DT == DT_BF16;
+  static constexpr bool kInLds = DT == DT_BF16;
   using Acc = typename std::conditional<DT == DT_BF16, float, double>::type;
   static constexpr int kSums = (4 + 2 + 4 + 4 + 1) * kQ;  // Acc values
-  static constexpr int kBytes = 3 * Tile<NP, 64>::kBytes + (kBInLds ? 3 : 2) * Tile<NP, W>::kBytes + Decays::kBytes +
+  static constexpr int kBytes = 3 * Tile<NP, 64>::kBytes + (kInLds ? 4 : 2) * Tile<NP, W>::kBytes + Decays::kBytes +
                                 kSums * static_cast<int>(sizeof(Acc));
   // waves a SIMD: two workgroups of 8 waves a CU where LDS holds them
   static constexpr int kWaves = 2;
@@ -122,8 +124,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   const Tile<NP, 64> xt{reinterpret_cast<uint16_t*>(smem)}, yt{reinterpret_cast<uint16_t*>(smem + kT)},
       mt{reinterpret_cast<uint16_t*>(smem + 2 * kT)};
   const Tile<NP, W> ht{reinterpret_cast<uint16_t*>(smem + 3 * kT)}, dt{reinterpret_cast<uint16_t*>(smem + 3 * kT + kS)},
-      bt{reinterpret_cast<uint16_t*>(smem + 3 * kT + 2 * kS)};
-  char* rest = smem + 3 * kT + (LY::kBInLds ? 3 : 2) * kS;
+      bt{reinterpret_cast<uint16_t*>(smem + 3 * kT + 2 * kS)}, ct{reinterpret_cast<uint16_t*>(smem + 3 * kT + 3 * kS)};
+  char* rest = smem + 3 * kT + (LY::kInLds ? 4 : 2) * kS;
   const Decays dec(rest);
   Acc* Kp = reinterpret_cast<Acc*>(rest + Decays::kBytes);  // [4][64] column sums by row block
   Acc* Rv = Kp + 4 * kQ;                                    // [2][64] row sums by half
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   Staged<DT, VEC, 64, kBack> sx, sy;
   Staged<DT, VEC, W, kBack> sh, sd;
   double sv = 0.0;
-  float uv = 0.f;
+  float uv = 0.f, rate_v = 0.f, skip_v = 0.f;
   auto width = [&](int pt) { return P - pt * kTile < kTile ? P - pt * kTile : kTile; };
   auto fetch_states = [&](int h, int pt, int nt) {
     const int64_t off = (int64_t(h) * P + pt * kTile) * N + nt * 64;
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
     sy.load(yrow, kQ, width(pt), off);
     fetch_states(h, pt, 0);
     const int64_t at = (int64_t(h) * a.chunks + c.id) * kQ + lane;
-    if (pt == 0) sv = a.s[at], uv = a.u[at];
+    if (pt == 0) sv = a.s[at], uv = a.u[at], rate_v = a.par[2 * h], skip_v = a.par[2 * h + 1];
   };
   fetch(h_lo, 0);
 
@@ -185,10 +187,12 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   f32x4 gm[Q], ds[Q];
 #pragma unroll
   for (int k = 0; k < Q; ++k) gm[k] = ds[k] = zero4();
-  if (LY::kBInLds) {
+  if (LY::kInLds) {
     Staged<DT, VEC, W, kBack> sb;
     sb.load(brow, kQ, N, 0);
     sb.put(bt);
+    sb.load(crow, kQ, N, 0);
+    sb.put(ct);
   }
 #pragma unroll
   for (int ks = 0; ks < 2 * NT; ++ks) {
@@ -206,7 +210,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 
 #pragma unroll 1
   for (int h = h_lo; h < h_hi; ++h) {
-    const float skip = a.p.D == nullptr ? 0.f : load_any(a.p.D, a.p.d_dt, h);
+    const float rate = rate_v, skip = skip_v;
     Acc qa[Q], ga[Q], ka[Q][4], ra = 0, da = 0, za = 0, xy = 0;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
@@ -217,6 +221,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 #pragma unroll 1
     for (int pt = 0; pt < ptiles; ++pt) {
       lx.refresh(), lw.refresh();
+      int rel = i - 4 * g - 16 * half;
+      asm volatile("" : "+v"(rel));  // (its comparisons are made anew: kept, they fill scalar registers)
       if (pt > 0) __syncthreads();  // (the last tile's readers; a head's last barrier is behind them too)
 #pragma unroll
       for (int k = 0; k < sx.kLoads; ++k) xy += dot<Acc>(sx.v[k], sy.v[k]);
@@ -250,7 +256,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
           f32x4 gl;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const bool in = j0 + r <= i, diag = j0 + r == i;
+            const bool in = rel >= 16 * kHalves * k + r, diag = rel == 16 * kHalves * k + r;
             const float L = __builtin_amdgcn_exp2f(static_cast<float>(si - dec.s[j0 + r]));
             const float gv = gm[k][r] * L, vv = vm[k][r] * (L * u[r]), wv = gv * vm[k][r];
             gl[r] = in ? gv : 0.f;
@@ -289,7 +295,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 #pragma unroll
           for (int k = 0; k < Q; ++k) {
             const int col = 64 * nt0 + 32 * ks + 8 * g;
-            const Frag<NP> bf = LY::kBInLds ? bt.get8(lw, blk(k), ks)
+            const Frag<NP> bf = LY::kInLds ? bt.get8(lw, blk(k), ks)
                                             : brow.get8(16 * blk(k) + li, col, N - col, 0).frag();
             xa[k] = mm(df, bf, xa[k]);
           }
@@ -302,7 +308,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 #pragma unroll
           for (int k = 0; k < Q; ++k) {
             const f32x4 v = mm(h1, yt.get8(lx, blk(k), 1), mm(h0, yt.get8(lx, blk(k), 0), zero4()));
-            const f32x4 cv = crow.get4(16 * blk(k) + li, sc, N - sc);
+            const f32x4 cv = LY::kInLds ? ct.get4(lw, blk(k), 4 * tw + wave)
+                                        : crow.get4(16 * blk(k) + li, sc, N - sc);
             dCa[nt][k] += dec.e[16 * blk(k) + li] * v;
 #pragma unroll
             for (int r = 0; r < 4; ++r) qa[k] += static_cast<Acc>(v[r]) * cv[r];
@@ -377,7 +384,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
         if (t >= d) pre += o2;
       }
       const double dat = suf + (pre - own) + static_cast<double>(z) * e_last;
-      double du = K + dg[t] + gt + load_any(a.p.A, a.p.a_dt, h) * dat;
+      double du = K + dg[t] + gt + rate * dat;
       if (a.p.softplus) du *= -expm1f(-u);
       const bool real = t < n;
       if (real) store_any(b.ddt, DT, (c.t0 + t) * H + h, static_cast<float>(du));
