@@ -237,16 +237,18 @@ struct Rows {
     }
     return v;
   }
-  __device__ __forceinline__ void put4(int row, int col, f32x4 v) const {
+  // (row + more, col), `more` the same for every lane
+  __device__ __forceinline__ void put4(int row, int col, f32x4 v, int more = 0) const {
     if constexpr (VEC) {
-      const int o = off(row, col);
+      const int o = off(row, col), s = more * static_cast<int>(stride) * E;
       if constexpr (DT == DT_BF16) {
         const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
-        __builtin_amdgcn_raw_buffer_store_b64(w, rsrc(), o, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b64(w, rsrc(), o, s, 0);
       } else {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rsrc(), o, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rsrc(), o, s, 0);
       }
     } else {
+      row += more;
       const int have = row < n ? cols - col : 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -501,7 +503,8 @@ struct Decays {
   }
   // every wave: lane t with token t's u and s; wave w makes a part of them
   __device__ __forceinline__ void put(int wave, double sv, float uv) const {
-    const int t = threadIdx.x & 63;
+    int t = threadIdx.x & 63;
+    asm volatile("" : "+v"(t));  // (no address of these is kept over a walk)
     auto ex = [](double d) { return __builtin_amdgcn_exp2f(static_cast<float>(d)); };
     if (wave == 0) {
       const double before = __shfl(sv, (t & 48) > 0 ? (t & 48) - 1 : 0);
@@ -526,6 +529,16 @@ struct Decays {
     return v;
   }
 };
+
+// a[at + lane] for the uniform place `at` of an array (no 64-bit address a lane)
+__device__ __forceinline__ double lane_of(const double* a, int64_t at, int lane) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<double*>(a + at), 0, kQ * 8, 0x00020000);
+  return __builtin_bit_cast(double, __builtin_amdgcn_raw_buffer_load_b64(r, lane * 8, 0, 0));
+}
+__device__ __forceinline__ float lane_of(const float* a, int64_t at, int lane) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a + at), 0, kQ * 4, 0x00020000);
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, 0, 0));
+}
 
 // Sequences as [edge(m), edge(m + 1)), m < count: the batch's rows, or the packed axis
 // cut at 0, every cu entry and n_tokens (what lies outside the cu entries is a sequence

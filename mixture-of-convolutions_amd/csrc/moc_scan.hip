@@ -75,7 +75,10 @@ __device__ __forceinline__ void load_state(const Rows<DT, VEC>& src, int row, f3
 }
 template <int NB, int DT, bool VEC>
 __device__ __forceinline__ void store_state(const Rows<DT, VEC>& dst, int row, const f32x4 (&acc)[NB]) {
-  const int n0 = 4 * ((threadIdx.x & 63) >> 4);
+  int n0 = 4 * ((threadIdx.x & 63) >> 4);
+  // (the blocks' offsets are formed here each time: kept over a walk, they push others to
+  // memory, whose reloads wait for every load ahead)
+  asm volatile("" : "+v"(n0));
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) dst.put4(row, 16 * nb + n0, acc[nb]);
 }
@@ -179,8 +182,8 @@ __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 :
     const int n = s.n - i * kQ < kQ ? s.n - i * kQ : kQ;
     sx.load(Rows<DT, VEC>(w.x, t * w.x_stride + xcol, w.x_stride, n, cols));
     sb.load(Rows<DT, VEC>(w.b, t * w.b_stride + bcol, w.b_stride, n, N));
-    sv = a.s[at + i * kQ + lane];
-    if (!REV) uv = a.u[at + i * kQ + lane];
+    sv = lane_of(a.s, at + i * kQ, lane);
+    if (!REV) uv = lane_of(a.u, at + i * kQ, lane);
   };
   double total = 0.0;
   fetch(REV ? s.chunks - 1 : 0);
@@ -255,7 +258,8 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
   int* odd = reinterpret_cast<int*>(reinterpret_cast<char*>(dec.s) + Decays::kBytes);  // [2], by chunk parity
   Lane<W> lw;
   Lane<64> lx;
-  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63;
+  int li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int P = static_cast<int>(a.p.P), N = static_cast<int>(a.p.N);
   const int ptiles = (P + kTile - 1) / kTile;
@@ -291,14 +295,15 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
     sx.load(Rows<DT, VEC>(a.p.x, t * a.p.x_stride + xcol, a.p.x_stride, tokens(k), cols));
     sb.load(Rows<DT, VEC>(a.p.B, t * a.p.b_stride + bcol, a.p.b_stride, tokens(k), N));
     if (kCInLds) sc.load(c_rows(k));
-    sv = a.s[at + k * kQ + lane];
-    uv = a.u[at + k * kQ + lane];
+    sv = lane_of(a.s, at + k * kQ, lane);
+    uv = lane_of(a.u, at + k * kQ, lane);
   };
   fetch(0);
   __syncthreads();  // odd is 0
 #pragma unroll 1
   for (int k = 0; k < s.chunks; ++k) {
     lw.refresh(), lx.refresh();
+    asm volatile("" : "+v"(li), "+v"(g));  // (nor are addresses in the factors kept from chunk to chunk)
     const int n = tokens(k);
     sx.put(xt);
     sb.put(bt);
@@ -406,7 +411,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
         // (without D skip is 0: no branch between a product and the first use of its result,
         // whose wait states the compiler has been seen to leave out on the path around a body)
         ya[ib] += skip * xt.get4(lx, ib, wave);
-        yrow.put4(16 * ib + li, 16 * wave + 4 * g, ya[ib]);
+        yrow.put4(li, 16 * wave + 4 * g, ya[ib], 16 * ib);
       }
       if (bad) {
 #pragma unroll 1
