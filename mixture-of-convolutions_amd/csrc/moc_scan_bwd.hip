@@ -135,7 +135,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   __shared__ Acc zp[2][4 * kHalves];                        // z, <x, dy> by wave
   Lane<64> lx;
   Lane<W> lw;
-  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63;
+  int li = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wid & 3, half = wid >> 2;
   const int H = static_cast<int>(a.p.H), P = static_cast<int>(a.p.P), G = static_cast<int>(a.p.G),
             N = static_cast<int>(a.p.N);
@@ -159,7 +160,6 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   const Span<DT, VEC> orow(b.dx, c.t0 * H * P, int64_t(H) * P, n);
   const Span<DT, VEC> hrow(b.h, c.id * H * P * N, N, int64_t(H) * P);
   const Span<DT, VEC> drow(b.dh, c.id * H * P * N, N, int64_t(H) * P);
-  const int i = 16 * wave + li;  // this lane's row i of G, V (result column)
   auto blk = [&](int k) { return k * kHalves + half; };  // this wave's column blocks
 
   // the loads of a head's (and channel tile's) tensors, ahead of their use
@@ -173,13 +173,21 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
     sh.load(hrow, use_h ? width(pt) : 0, N - nt * 64, off);
     sd.load(drow, use_dh ? width(pt) : 0, N - nt * 64, off);
   };
+  // (one place in the code with no branch in it, or the compiler loads to other registers and
+  // waits to move the values over; behind the last head nothing is loaded)
   auto fetch = [&](int h, int pt) {
-    const int off = h * P + pt * kTile;
-    sx.load(xrow, kQ, width(pt), off);
-    sy.load(yrow, kQ, width(pt), off);
-    fetch_states(h, pt, 0);
-    const int64_t at = (int64_t(h) * a.chunks + c.id) * kQ + lane;
-    if (pt == 0) sv = a.s[at], uv = a.u[at], rate_v = a.par[2 * h], skip_v = a.par[2 * h + 1];
+    const bool more = h < h_hi;
+    const int at = more ? h : h_lo, off = at * P + pt * kTile, w = more ? width(pt) : 0;
+    sx.load(xrow, kQ, w, off);
+    sy.load(yrow, kQ, w, off);
+    const int64_t soff = int64_t(off) * N;
+    sh.load(hrow, use_h ? w : 0, N, soff);
+    sd.load(drow, use_dh ? w : 0, N, soff);
+    const int64_t tok = (int64_t(at) * a.chunks + c.id) * kQ;
+    sv = lane_of(a.s, tok, lane);
+    uv = lane_of(a.u, tok, lane);
+    rate_v = lane_of(a.par, 2 * at, 0);
+    skip_v = lane_of(a.par, 2 * at, 1);
   };
   fetch(h_lo, 0);
 
@@ -197,7 +205,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 #pragma unroll
   for (int ks = 0; ks < 2 * NT; ++ks) {
     const int col = 32 * ks + 8 * g;
-    const Frag<NP> cf = crow.get8(i, col, N - col, 0).frag();
+    const Frag<NP> cf = crow.get8(16 * wave + li, col, N - col, 0).frag();
 #pragma unroll
     for (int k = 0; k < Q; ++k) gm[k] = mm(brow.get8(16 * blk(k) + li, col, N - col, 0).frag(), cf, gm[k]);
   }
@@ -221,8 +229,10 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 #pragma unroll 1
     for (int pt = 0; pt < ptiles; ++pt) {
       lx.refresh(), lw.refresh();
-      int rel = i - 4 * g - 16 * half;
-      asm volatile("" : "+v"(rel));  // (its comparisons are made anew: kept, they fill scalar registers)
+      // (lane masks and addresses are formed anew: kept over the heads, they fill the registers
+      // and spill, and a reload waits for every load ahead)
+      asm volatile("" : "+v"(li), "+v"(g));
+      const int i = 16 * wave + li, rel = i - 4 * g - 16 * half;  // this lane's row i of G, V (result column)
       if (pt > 0) __syncthreads();  // (the last tile's readers; a head's last barrier is behind them too)
 #pragma unroll
       for (int k = 0; k < sx.kLoads; ++k) xy += dot<Acc>(sx.v[k], sy.v[k]);
@@ -281,12 +291,11 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
           put_states();
           __syncthreads();
         }
-        if (nt0 + TW < ntiles) {
+        if (TW < NT && nt0 + TW < ntiles) {
           fetch_states(h, pt, nt0 + TW);
-        } else if (pt + 1 < ptiles) {
-          fetch(h, pt + 1);
-        } else if (h + 1 < h_hi) {
-          fetch(h + 1, 0);
+        } else {
+          const bool same = pt + 1 < ptiles;
+          fetch(same ? h : h + 1, same ? pt + 1 : 0);
         }
         if (!use_h && !use_dh) continue;
 #pragma unroll
@@ -345,6 +354,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
       }
     }
     // the head's sums over channels and states
+    asm volatile("" : "+v"(li), "+v"(g));
+    const int i = 16 * wave + li;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
 #pragma unroll
@@ -367,7 +378,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
     const float u = dec.u[lane], e = dec.e[lane], f = dec.f[lane], e_last = dec.e[kQ - 1];
     __syncthreads();  // the sums are whole, every tile and factor has been read
     if (wid == (h & 7)) {  // (each head another wave's: the others go on)
-      const int t = lane;
+      int t = lane;
+      asm volatile("" : "+v"(t));
       auto four = [&](const Acc* p) { return (p[t] + p[kQ + t]) + (p[2 * kQ + t] + p[3 * kQ + t]); };
       const Acc K = four(Kp), q = e * four(qp), gt = f * four(gp);
       Acc z = 0, xd = 0;
