@@ -255,7 +255,22 @@ struct Rows {
         if (k < have) store_any(const_cast<char*>(base), DT, row * stride + col + k, v[k]);
     }
   }
+  // 8 elements, all or none of which are there
+  __device__ __forceinline__ void put8(int row, int col, f32x4 lo, f32x4 hi) const {
+    if constexpr (VEC && DT == DT_BF16) {
+      const u32x4 w{pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(hi[0], hi[1]), pack2(hi[2], hi[3])};
+      __builtin_amdgcn_raw_buffer_store_b128(w, rsrc(), off(row, col), 0, 0);
+    } else {
+      put4(row, col, lo);
+      put4(row, col + 4, hi);
+    }
+  }
 };
+
+// States kept for the backward pass: [channels][kept_cols(N)], a row's states in the order
+// in which the walks' lanes hold them: the 4 states of lane group g in the lower and the
+// upper block of 16 of 32 states next to each other, so that a lane stores 8 at a time.
+__host__ __device__ constexpr int64_t kept_cols(int64_t N) { return (N + 31) / 32 * 32; }
 
 // Rows at a place that moves by a uniform offset (a head's columns of a token, a head's rows
 // of the states) under one buffer resource: `off` elements from base, row by row `stride`.
@@ -380,6 +395,16 @@ struct Tile {
 #pragma unroll
     for (int k = 0; k < NP; ++k) *reinterpret_cast<s16x8*>(q + k * kPlane) = r.v[k];
   }
+  // 8 kept states (block `col` / 8 of a row): lower and upper four
+  __device__ __forceinline__ void put44(int row, int col, const Frag<NP>& r) const {
+    const int c = (col & ~31) + ((col & 31) >> 1), x = Lane<W>::f(row) << 3;
+    uint16_t *q = p + row * W + (c ^ x), *q2 = p + row * W + ((c + 16) ^ x);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      *reinterpret_cast<s16x4*>(q + k * kPlane) = __builtin_shufflevector(r.v[k], r.v[k], 0, 1, 2, 3);
+      *reinterpret_cast<s16x4*>(q2 + k * kPlane) = __builtin_shufflevector(r.v[k], r.v[k], 4, 5, 6, 7);
+    }
+  }
   // row 16 rb + li, columns 32 ks + 8 g..
   __device__ __forceinline__ Frag<NP> get8(const Lane<W>& l, int rb, int ks) const {
     const uint16_t* q = p + (l.nat ^ (32 * ks)) + 16 * rb * W;
@@ -468,6 +493,11 @@ struct Staged {
   __device__ __forceinline__ void put(const Tile<NP, W>& t) const {
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) t.put8(row(k), col(k), v[k].frag());
+  }
+  template <int NP>
+  __device__ __forceinline__ void put_kept(const Tile<NP, W>& t) const {
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) t.put44(row(k), col(k), v[k].frag());
   }
   __device__ __forceinline__ uint32_t odd() const {
     uint32_t r = 0;

@@ -83,6 +83,15 @@ __device__ __forceinline__ void store_state(const Rows<DT, VEC>& dst, int row, c
   for (int nb = 0; nb < NB; ++nb) dst.put4(row, 16 * nb + n0, acc[nb]);
 }
 
+// acc to a row of kept states (rounded to x's type: operands of the backward's products)
+template <int NB, int DT, bool VEC>
+__device__ __forceinline__ void keep_state(const Rows<DT, VEC>& dst, int row, const f32x4 (&acc)[NB]) {
+  int g8 = 8 * ((threadIdx.x & 63) >> 4);
+  asm volatile("" : "+v"(g8));
+#pragma unroll
+  for (int nb = 0; nb < NB; nb += 2) dst.put8(row, 16 * nb + g8, acc[nb], acc[nb + 1]);
+}
+
 // 8 products of a transposed x operand and the tokens' weights w[0..8) as three planes
 template <int NP>
 __device__ __forceinline__ Frag<3> weighted(const Frag<NP>& x, const float* w) {
@@ -154,7 +163,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 :
   Lane<W> lw;
   Lane<64> lx;
   const int lane = threadIdx.x & 63, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int P = static_cast<int>(a.p.P), N = static_cast<int>(a.p.N);
+  const int P = static_cast<int>(a.p.P), N = static_cast<int>(a.p.N), NK = static_cast<int>(kept_cols(N));
   const int ptiles = (P + kTile - 1) / kTile;
   const int h = blockIdx.y / ptiles, p0 = (blockIdx.y % ptiles) * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
   Segment s;
@@ -192,7 +201,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 :
     lw.refresh(), lx.refresh();
     const int i = REV ? s.chunks - 1 - k : k;
     if (!LOCAL && w.kept != nullptr && !(k == 0 && from == nullptr))
-      store_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + i) * a.p.H + h) * P + p0) * N, N, cols, N), row, acc);
+      keep_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + i) * a.p.H + h) * P + p0) * NK, NK, cols, NK), row, acc);
     sx.put(xt);
     sb.put(bt);
     const double last = __shfl(sv, 63);
@@ -261,7 +270,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
   const int lane = threadIdx.x & 63;
   int li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int P = static_cast<int>(a.p.P), N = static_cast<int>(a.p.N);
+  const int P = static_cast<int>(a.p.P), N = static_cast<int>(a.p.N), NK = static_cast<int>(kept_cols(N));
   const int ptiles = (P + kTile - 1) / kTile;
   const int h = blockIdx.y / ptiles, p0 = (blockIdx.y % ptiles) * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
   Segment s;
@@ -357,7 +366,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
     else if (wave == 2) m_blocks(Int<8>{}, Int<9>{}, Int<10>{});
     else m_blocks(Int<13>{}, Int<14>{}, Int<15>{});
     if (w.kept != nullptr && !(k == 0 && from == nullptr))
-      store_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + k) * a.p.H + h) * P + p0) * N, N, cols, N), row, acc);
+      keep_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + k) * a.p.H + h) * P + p0) * NK, NK, cols, NK), row, acc);
     if (k + 1 < s.chunks) fetch(k + 1);
     f32x4 ya[4];
 #pragma unroll
@@ -577,7 +586,7 @@ Args make_args(const Scan& p, void* prep) {
   a.par = reinterpret_cast<float*>(static_cast<char*>(prep) + up(n * 4) + up(n * 8));
   a.vec = p.P % 8 == 0 && p.N % 8 == 0 && aligned({p.x, p.B, p.C}, 16);
   // (a chunk's states lie under one buffer resource)
-  a.vec = a.vec && p.H * p.P * p.N * 4 < int64_t(kNowhere) - 16;
+  a.vec = a.vec && p.H * p.P * kept_cols(p.N) * 4 < int64_t(kNowhere) - 16;
   for (int64_t st : {p.x_stride, p.b_stride, p.c_stride, p.H * p.P, p.G * p.N}) a.vec = a.vec && st % 8 == 0 && st < kMaxStride;
   return a;
 }
@@ -622,7 +631,7 @@ using namespace scan;
 
 size_t scan_saved_bytes(const Scan& p) {
   const Args a = make_args(p, nullptr);
-  return prep_bytes(p) + size_t(a.chunks) * p.H * p.P * p.N * (p.x_dt == DT_BF16 ? 2 : 4);
+  return prep_bytes(p) + size_t(a.chunks) * p.H * p.P * kept_cols(p.N) * (p.x_dt == DT_BF16 ? 2 : 4);
 }
 
 size_t scan_forward_workspace(const Scan& p, bool saved) {

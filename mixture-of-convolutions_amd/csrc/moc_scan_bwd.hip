@@ -32,7 +32,7 @@ constexpr int kThreads = 256;
 
 struct Back {
   const void* dy;       // [tokens][H][P] contiguous
-  const void* h;        // [chunks][H][P][N], x dtype: state before each chunk
+  const void* h;        // [chunks][H][P][kept_cols(N)], x dtype: state before each chunk
   const void* dh;       // the same: gradient of the state behind each chunk
   bool has_init, has_dfin;
   void *dx, *ddt, *dB, *dC;
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   int li = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wid & 3, half = wid >> 2;
   const int H = static_cast<int>(a.p.H), P = static_cast<int>(a.p.P), G = static_cast<int>(a.p.G),
-            N = static_cast<int>(a.p.N);
+            N = static_cast<int>(a.p.N), NK = static_cast<int>(kept_cols(N));
   const int grp = blockIdx.y / b.subs, sub = blockIdx.y % b.subs, hpg = H / G;
   const int h_lo = grp * hpg + sub * b.per_sub;
   const int h_hi = (sub + 1) * b.per_sub < hpg ? h_lo + b.per_sub : (grp + 1) * hpg;
@@ -158,8 +158,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   const Span<DT, VEC> xrow(a.p.x, c.t0 * a.p.x_stride, a.p.x_stride, n);
   const Span<DT, VEC> yrow(b.dy, c.t0 * H * P, int64_t(H) * P, n);
   const Span<DT, VEC> orow(b.dx, c.t0 * H * P, int64_t(H) * P, n);
-  const Span<DT, VEC> hrow(b.h, c.id * H * P * N, N, int64_t(H) * P);
-  const Span<DT, VEC> drow(b.dh, c.id * H * P * N, N, int64_t(H) * P);
+  const Span<DT, VEC> hrow(b.h, c.id * H * P * NK, NK, int64_t(H) * P);
+  const Span<DT, VEC> drow(b.dh, c.id * H * P * NK, NK, int64_t(H) * P);
   auto blk = [&](int k) { return k * kHalves + half; };  // this wave's column blocks
 
   // the loads of a head's (and channel tile's) tensors, ahead of their use
@@ -169,9 +169,9 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   float uv = 0.f, rate_v = 0.f, skip_v = 0.f;
   auto width = [&](int pt) { return P - pt * kTile < kTile ? P - pt * kTile : kTile; };
   auto fetch_states = [&](int h, int pt, int nt) {
-    const int64_t off = (int64_t(h) * P + pt * kTile) * N + nt * 64;
-    sh.load(hrow, use_h ? width(pt) : 0, N - nt * 64, off);
-    sd.load(drow, use_dh ? width(pt) : 0, N - nt * 64, off);
+    const int64_t off = (int64_t(h) * P + pt * kTile) * NK + nt * 64;
+    sh.load(hrow, use_h ? width(pt) : 0, NK - nt * 64, off);
+    sd.load(drow, use_dh ? width(pt) : 0, NK - nt * 64, off);
   };
   // (one place in the code with no branch in it, or the compiler loads to other registers and
   // waits to move the values over; behind the last head nothing is loaded)
@@ -180,9 +180,9 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
     const int at = more ? h : h_lo, off = at * P + pt * kTile, w = more ? width(pt) : 0;
     sx.load(xrow, kQ, w, off);
     sy.load(yrow, kQ, w, off);
-    const int64_t soff = int64_t(off) * N;
-    sh.load(hrow, use_h ? w : 0, N, soff);
-    sd.load(drow, use_dh ? w : 0, N, soff);
+    const int64_t soff = int64_t(off) * NK;
+    sh.load(hrow, use_h ? w : 0, NK, soff);
+    sd.load(drow, use_dh ? w : 0, NK, soff);
     const int64_t tok = (int64_t(at) * a.chunks + c.id) * kQ;
     sv = lane_of(a.s, tok, lane);
     uv = lane_of(a.u, tok, lane);
@@ -242,8 +242,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
       auto put_states = [&]() {
 #pragma unroll
         for (int k = 0; k < sh.kLoads; ++k) za += dot<Acc>(sh.v[k], sd.v[k]);
-        sh.put(ht);
-        sd.put(dt);
+        sh.put_kept(ht);
+        sd.put_kept(dt);
       };
       if (use_h || use_dh) put_states();
       __syncthreads();
@@ -478,7 +478,7 @@ struct Bytes {
 Bytes bytes_of(const Args& a) {
   Bytes r;
   r.walk = walk_bytes(a);
-  r.dh = up(size_t(a.chunks) * a.p.H * a.p.P * a.p.N * (a.p.x_dt == DT_BF16 ? 2 : 4));
+  r.dh = up(size_t(a.chunks) * a.p.H * a.p.P * kept_cols(a.p.N) * (a.p.x_dt == DT_BF16 ? 2 : 4));
   r.part = up(size_t(a.chunks) * 3 * a.p.H * 4);
   const int64_t s = subs_of(a);
   r.sub = s == 1 ? 0 : up(size_t(s) * a.p.seq.n_tokens * a.p.G * a.p.N * 4);
