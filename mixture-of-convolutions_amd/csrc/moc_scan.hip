@@ -25,27 +25,38 @@ constexpr int kThreads = 256;
 template <int V>
 using Int = std::integral_constant<int, V>;
 
+constexpr int kPrepHeads = 8;  // of a workgroup: two a wave
+
+// v of the lane N below in its group of 16 (0 where there is none)
+template <int N>
+__device__ __forceinline__ double row_below(double v) {
+  const uint64_t w = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(w), 0x110 + N, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(w >> 32), 0x110 + N, 0xf, 0xf, true);
+  return __longlong_as_double((static_cast<uint64_t>(hi) << 32) | lo);
+}
+
 // ---------------------------------------------------------------------------
 // u and s of every chunk and head.  Lanes are tokens for the running sum (in 64 bits:
 // s_i - s_j is formed from it, where a 32-bit sum of tens would lose the differences of
 // neighbours), heads for the loads.
 __global__ __launch_bounds__(kThreads) void prep_kernel(Args a) {
-  __shared__ float raw[16][kQ + 1];
-  const int h0 = blockIdx.y * 16;
-  if (blockIdx.x == 0 && threadIdx.x < 16 && h0 + threadIdx.x < a.p.H) {
+  __shared__ float raw[kPrepHeads][kQ + 1];
+  const int h0 = blockIdx.y * kPrepHeads;
+  if (blockIdx.x == 0 && threadIdx.x < kPrepHeads && h0 + threadIdx.x < a.p.H) {
     const int64_t h = h0 + threadIdx.x;
     a.par[2 * h] = load_any(a.p.A, a.p.a_dt, h);
     a.par[2 * h + 1] = a.p.D == nullptr ? 0.f : load_any(a.p.D, a.p.d_dt, h);
   }
   Chunk c;
   if (!chunk_at(a, blockIdx.x, c)) return;
-  for (int k = threadIdx.x; k < 16 * kQ; k += kThreads) {
-    const int t = k >> 4, h = h0 + (k & 15);
-    if (t < c.n && h < a.p.H) raw[k & 15][t] = load_any(a.p.dt, a.p.x_dt, (c.t0 + t) * a.p.dt_stride + h);
+  for (int k = threadIdx.x; k < kPrepHeads * kQ; k += kThreads) {
+    const int t = k / kPrepHeads, q = k % kPrepHeads;
+    if (t < c.n && h0 + q < a.p.H) raw[q][t] = load_any(a.p.dt, a.p.x_dt, (c.t0 + t) * a.p.dt_stride + h0 + q);
   }
   __syncthreads();
   const int t = threadIdx.x & 63;
-  for (int k = threadIdx.x >> 6; k < 16 && h0 + k < a.p.H; k += 4) {
+  for (int k = threadIdx.x >> 6; k < kPrepHeads && h0 + k < a.p.H; k += 4) {
     const int h = h0 + k;
     float u = 0.f;
     if (t < c.n) {
@@ -54,11 +65,14 @@ __global__ __launch_bounds__(kThreads) void prep_kernel(Args a) {
     }
     double s = static_cast<double>(u) * load_any(a.p.A, a.p.a_dt, h) * 1.4426950408889634074;
     if (t >= c.n) s = 0.0;  // (also where A is not finite)
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double o = __shfl_up(s, d);
-      if (t >= d) s += o;
-    }
+    // running sum: within groups of 16 lanes by row operations, then the groups before
+    s += row_below<1>(s);
+    s += row_below<2>(s);
+    s += row_below<4>(s);
+    s += row_below<8>(s);
+    const double e0 = __shfl(s, 15), e1 = __shfl(s, 31), e2 = __shfl(s, 47);
+    const int g = t >> 4;
+    s += g == 0 ? 0.0 : (g == 1 ? e0 : (g == 2 ? e0 + e1 : (e0 + e1) + e2));
     const int64_t at = (int64_t(h) * a.chunks + c.id) * kQ + t;
     a.u[at] = u;
     a.s[at] = s;
@@ -592,7 +606,7 @@ Args make_args(const Scan& p, void* prep) {
 }
 
 void launch_prep(const Args& a, hipStream_t st) {
-  hipLaunchKernelGGL(prep_kernel, dim3(static_cast<unsigned>(a.chunks), static_cast<unsigned>((a.p.H + 15) / 16)),
+  hipLaunchKernelGGL(prep_kernel, dim3(static_cast<unsigned>(a.chunks), static_cast<unsigned>((a.p.H + kPrepHeads - 1) / kPrepHeads)),
                      dim3(kThreads), 0, st, a);
 }
 
