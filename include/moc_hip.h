@@ -457,8 +457,8 @@ int moc_conv_update(const void* x, const void* weight, const void* bias, void* c
  *   u = softplus(dt + dt_bias) (or dt + dt_bias), h_t = exp(u_t a) h_{t-1} + u_t x_t (x) b_t,
  *   y_t = h_t c_t + d x_t.
  * x [n_tokens, heads, head_dim], dt [n_tokens, heads], b and c [n_tokens, groups,
- * state_dim] in x_dtype (bf16 or f32), tokens *_stride elements apart, a token's own
- * values contiguous; heads h of group h / (heads / groups) share b and c.  a, d (or NULL),
+ * state_dim] in x_dtype (bf16 or f32), tokens *_stride elements apart (below 2^31; not
+ * read for a single token), a token's own values contiguous; heads h of group h / (heads / groups) share b and c.  a, d (or NULL),
  * dt_bias (or NULL) [heads] in any dtype.  head_dim <= 128, state_dim <= 256.  States
  * [n_seqs, heads, head_dim, state_dim] f32, fixed length only.
  */

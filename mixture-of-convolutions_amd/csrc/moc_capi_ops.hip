@@ -15,6 +15,7 @@ bool any_dt(int dt) { return dt == MOC_DT_F32 || dt == MOC_DT_BF16 || dt == MOC_
 bool x_dt_ok(int dt) { return dt == MOC_DT_F32 || dt == MOC_DT_BF16; }
 
 constexpr int64_t kMaxTokens = int64_t(1) << 31;
+constexpr int64_t kMaxStride = int64_t(1) << 31;  // elements between tokens
 constexpr int64_t kMaxWorkgroups = int64_t(1) << 24;  // of 256 threads: a grid counts threads in 32 bits
 
 int launched(const char* what) {
@@ -92,6 +93,9 @@ int check_scan(const MocScan* s, bool step) {
   const int64_t xs = s->heads * s->head_dim, bs = s->groups * s->state_dim;
   if (s->n_tokens > 1 && (s->x_stride < xs || s->dt_stride < s->heads || s->b_stride < bs || s->c_stride < bs))
     return fail(MOC_ERR_ARG, "token strides must hold a token's values");
+  if (s->n_tokens > 1 && (s->x_stride >= kMaxStride || s->dt_stride >= kMaxStride || s->b_stride >= kMaxStride ||
+                          s->c_stride >= kMaxStride))
+    return fail(MOC_ERR_ARG, "token strides must be below 2^31 elements");
   if (int rc = check_seq(s->cu_seqlens, s->n_seqs, s->n_tokens, s->seq_len)) return rc;
   if (step) {
     if (s->cu_seqlens != nullptr || s->seq_len != 1) return fail(MOC_ERR_ARG, "a step has one token per sequence");
@@ -117,10 +121,12 @@ moc::Scan problem(const MocScan* s) {
   p.C = s->c;
   p.D = s->d;
   p.bias = s->dt_bias;
-  p.x_stride = s->x_stride;
-  p.dt_stride = s->dt_stride;
-  p.b_stride = s->b_stride;
-  p.c_stride = s->c_stride;
+  // (a single token's strides say nothing)
+  const bool one = s->n_tokens == 1;
+  p.x_stride = one ? s->heads * s->head_dim : s->x_stride;
+  p.dt_stride = one ? s->heads : s->dt_stride;
+  p.b_stride = one ? s->groups * s->state_dim : s->b_stride;
+  p.c_stride = one ? s->groups * s->state_dim : s->c_stride;
   p.x_dt = s->x_dtype;
   p.a_dt = s->a_dtype;
   p.d_dt = s->d_dtype;

@@ -560,7 +560,7 @@ std::optional<std::tuple<Tensor, OptTensor>> conv(const Tensor& x, const Tensor&
 // --- selective scan
 
 // ops.token_rows: t itself where a token's `inner` dimensions are contiguous and tokens
-// evenly apart, a copy otherwise
+// evenly apart (below 2^31 elements), a copy otherwise
 Tensor token_rows(const Tensor& t, int64_t inner, int64_t& step) {
   const int64_t lead = t.dim() - inner;
   int64_t n = 1;
@@ -577,7 +577,7 @@ Tensor token_rows(const Tensor& t, int64_t inner, int64_t& step) {
     else ok = ok && t.stride(i) == t.size(lead - 1) * step;
     any = true;
   }
-  if (ok && step >= n) return t;
+  if (ok && step >= n && step < int64_t(1) << 31) return t;
   step = n;
   return t.contiguous();
 }

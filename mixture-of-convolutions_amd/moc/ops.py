@@ -769,7 +769,7 @@ def token_rows(t: torch.Tensor, inner: int) -> tuple[torch.Tensor, int]:
     """(tensor, elements between tokens) of a tensor whose last ``inner`` dimensions
     are a token's values and whose leading ones ([B, T] or [N]) are tokens: as it
     is where a token's values are contiguous and tokens evenly apart (a slice of a
-    wider projection), a contiguous copy otherwise."""
+    wider projection) and fewer than 2**31 elements, a contiguous copy otherwise."""
     lead, n = t.shape[:t.ndim - inner], 1
     dense = True
     for size, stride in zip(reversed(t.shape[t.ndim - inner:]),
@@ -780,7 +780,7 @@ def token_rows(t: torch.Tensor, inner: int) -> tuple[torch.Tensor, int]:
     if dense and len(strides) == 2:
         dense = strides[0] == lead[1] * strides[1]
     step = strides[-1] if strides else n
-    if not dense or step < n:
+    if not dense or step < n or step >= 2**31:
         return t.contiguous(), n
     return t, step
 

@@ -269,6 +269,8 @@ def _table(**kw):
     (dict(x=None), ERR_ARG), (dict(heads=0), ERR_ARG), (dict(groups=3), ERR_ARG), (dict(head_dim=129), ERR_ARG),
     (dict(state_dim=257), ERR_ARG), (dict(heads=40000, groups=1), ERR_ARG), (dict(x_dtype=2), ERR_DTYPE),
     (dict(a_dtype=7), ERR_DTYPE), (dict(dt_softplus=2), ERR_ARG), (dict(x_stride=31), ERR_ARG),
+    (dict(x_stride=1 << 31), ERR_ARG), (dict(dt_stride=1 << 31), ERR_ARG), (dict(b_stride=1 << 31), ERR_ARG),
+    (dict(c_stride=1 << 40), ERR_ARG),
     (dict(seq_len=4), ERR_ARG), (dict(n_tokens=0), ERR_ARG), (dict(cu_seqlens=FAKE, n_seqs=0), ERR_ARG),
     (dict(cu_seqlens=FAKE, n_seqs=2), ERR_ARG),
 ])

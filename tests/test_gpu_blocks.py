@@ -706,6 +706,32 @@ def test_library_refuses_what_python_would():
     assert _lib.lib().moc_last_error()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scan_strides_of_a_single_token_are_not_read(dtype):
+    H, P, G, N = 2, 64, 1, 64
+    ins = {q: dev(t) for q, t in scan_inputs((1, 1), H, P, G, N, dtype).items()}
+    order = [ins[q] for q in ("x", "dt", "A", "B", "C", "D", "dt_bias")]
+    dy = dev(rnd(1, 1, H, P, seed=9, dtype=dtype))
+    plain = moc.ops._scan_table
+
+    def run():
+        y, fin, saved = moc.ops.launch_scan_forward(*order, None, softplus=True, final_state=True, keep=True)
+        return y, fin, *moc.ops.launch_scan_backward(*order, dy, None, saved, softplus=True, has_init=False,
+                                                     need_init=False)
+
+    def zero_strides(*args):
+        table, held = plain(*args)
+        table.x_stride = table.dt_stride = table.b_stride = table.c_stride = 0
+        return table, held
+
+    want = run()
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(moc.ops, "_scan_table", zero_strides)
+        got = run()
+    assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
+    assert want[0].abs().sum() > 0
+
+
 def test_python_functions_are_the_host_modules(monkeypatch):
     """Without the host module the Python functions make the same calls."""
     def everything():
