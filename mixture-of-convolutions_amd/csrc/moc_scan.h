@@ -28,7 +28,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kQ = 64;        // tokens of a chunk
 constexpr int kTile = 64;     // channels of a head (P) and states (N) of a tile
-constexpr float kLog2e = 1.4426950408889634f;
 
 // One operand of a 16 x 16 x 32 product: 8 consecutive contraction entries of a
 // row, in NP planes.
