@@ -429,7 +429,7 @@ int moc_norm_backward(const void* x, const void* weight, const void* dy, const f
  * weight [kernel_size, dim], 1 <= kernel_size <= 16, bias [dim] or NULL, any dtypes.
  * Fixed length only: cache [n_seqs, dim, kernel_size] in the x dtype (newest slot last) or
  * NULL (zeros before a sequence), final_state the same or NULL: the last kernel_size
- * inputs.  Tokens outside every [cu_seqlens[j], cu_seqlens[j+1]) start their own history.
+ * inputs, in another tensor than cache.  Tokens outside every [cu_seqlens[j], cu_seqlens[j+1]) start their own history.
  */
 int moc_conv_forward(const void* x, const void* weight, const void* bias, const void* cache, void* y,
                      void* final_state, const void* cu_seqlens, int cu_seqlens_i64, int64_t n_seqs, int64_t n_tokens,
@@ -506,8 +506,9 @@ int moc_scan_forward(const MocScan* scan, void* y, const float* initial_state, f
 size_t moc_scan_backward_workspace_bytes(const MocScan* scan);
 
 /* Gradients for dy (contiguous, x dtype) and dfinal_state (or NULL) on the inputs and the
- * `saved` of moc_scan_forward; has_initial_state: whether that call had one.  Sums over
- * tokens and heads are formed in a fixed order. */
+ * `saved` of moc_scan_forward; has_initial_state: whether that call had one.
+ * dinitial_state may not be dfinal_state.  Sums over tokens and heads are formed in a fixed
+ * order. */
 int moc_scan_backward(const MocScan* scan, const void* dy, int has_initial_state, const float* dfinal_state,
                       const void* saved, size_t saved_bytes, const MocScanGrads* grads, void* workspace,
                       size_t workspace_bytes, void* stream);

@@ -138,6 +138,8 @@ moc::Scan problem(const MocScan* s) {
 int check_states(const MocScan* s, const void* a, const void* b) {
   if ((a != nullptr || b != nullptr) && s->cu_seqlens != nullptr)
     return fail(MOC_ERR_ARG, "states are only supported for fixed-length inputs");
+  // (one workgroup reads the first while another writes the last)
+  if (a != nullptr && a == b) return fail(MOC_ERR_ARG, "the state read and the state written must not be the same tensor");
   return MOC_OK;
 }
 
@@ -183,6 +185,8 @@ int moc_conv_forward(const void* x, const void* weight, const void* bias, const 
   if (!x || !weight || !y) return fail(MOC_ERR_ARG, "null tensor pointer");
   if ((cache != nullptr || final_state != nullptr) && cu_seqlens != nullptr)
     return fail(MOC_ERR_ARG, "states are only supported for fixed-length inputs");
+  if (cache != nullptr && cache == final_state)
+    return fail(MOC_ERR_ARG, "the cache read and the final state written must not be the same tensor");
   const moc::Conv p{layout(cu_seqlens, cu_seqlens_i64, n_seqs, n_tokens, seq_len), dim, kernel_size, x_dtype,
                     weight_dtype, bias_dtype, activation};
   moc::conv_forward(p, x, weight, bias, cache, y, final_state, static_cast<hipStream_t>(stream));

@@ -285,6 +285,16 @@ def test_capi_scan_arguments(kw, code):
         assert L.moc_scan_saved_bytes(ref) == 0 and L.moc_last_error()
 
 
+def test_capi_states_read_and_written_are_two_tensors():
+    L = _lib.lib()
+    ref = ctypes.byref(_table())
+    assert L.moc_scan_forward(ref, FAKE, FAKE, FAKE, FAKE, 1 << 40, FAKE, 1 << 40, None) == ERR_ARG
+    grads = _lib.MocScanGrads(*[FAKE] * 8)
+    assert L.moc_scan_backward(ref, FAKE, 0, FAKE, FAKE, 1 << 40, ctypes.byref(grads), FAKE, 1 << 40, None) == ERR_ARG
+    assert L.moc_conv_forward(FAKE, FAKE, None, FAKE, FAKE, FAKE, None, 0, 0, 8, 4, 16, 4, 1, 1, 1, 0, None) == ERR_ARG
+    assert b"same tensor" in L.moc_last_error()
+
+
 def test_capi_scan_workspaces():
     L = _lib.lib()
     t = _table()
