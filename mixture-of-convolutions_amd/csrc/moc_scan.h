@@ -47,6 +47,9 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
 // c + a . b.  The products of the lower planes are summed by themselves and added
 // once: each addition to c costs a rounding at c's size.
 __device__ __forceinline__ f32x4 mm(const Frag<1>& a, const Frag<1>& b, f32x4 c) { return mfma(a.v[0], b.v[0], c); }
+__device__ __forceinline__ f32x4 mm(const Frag<1>& a, const Frag<2>& b, f32x4 c) {
+  return mfma(a.v[0], b.v[0], mfma(a.v[0], b.v[1], c));
+}
 __device__ __forceinline__ f32x4 mm(const Frag<3>& a, const Frag<3>& b, f32x4 c) {
   f32x4 t = mfma(a.v[0], b.v[2], f32x4{0.f, 0.f, 0.f, 0.f});
   t = mfma(a.v[1], b.v[1], t);

@@ -20,8 +20,8 @@
 // heads through memory would move N fp32 values a token and head, more than x).  h and
 // dh come from memory in the x dtype (2 P N / kQ elements a token and head: at 64 x 128
 // four times x).  For bf16 that is one rounding of a matrix operand, as B's and C's is.
-// The gradient in which it shows is dA, a sum of products of random sign of h and dh: 0.001
-// relative beside the 0.0017 of its own rounding to bf16, more where decays are slow.
+// The gradient in which it shows is dA, a sum of products of random sign of h and dh: about
+// 0.001 relative beside the 0.0017 of its own rounding to bf16, more where decays are slow.
 //
 // 16384 bf16 tokens, 32 heads of 64 x 128: 235 us for 470 MB (2 TB/s; 302 us where the next
 // head's loads were waited for early, by reloads of spilled addresses, by loads of A, C and
@@ -416,9 +416,11 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
       }
     }
   }
-  // what the chunk's own tokens give of dB and dC, summed over the heads
+  // what the chunk's own tokens give of dB and dC, summed over the heads: once a workgroup,
+  // so that bf16 takes two planes of it (behind M's tile, where the states were)
+  const Tile<NP == 1 ? 2 : NP, 64> st{mt.p};
 #pragma unroll
-  for (int k = 0; k < Q; ++k) mt.put4(lx, wave, blk(k), ds[k]);
+  for (int k = 0; k < Q; ++k) st.put4(lx, wave, blk(k), ds[k]);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     if (nt >= ntiles) continue;
@@ -435,8 +437,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
       const Frag<NP> bf = xt.tr8(lx, ks, wave), cf = yt.tr8(lx, ks, wave);
 #pragma unroll
       for (int k = 0; k < Q; ++k) {
-        dCa[nt][k] = mm(bf, mt.get8(lx, blk(k), ks), dCa[nt][k]);
-        dBa[nt][k] = mm(cf, mt.tr8(lx, ks, blk(k)), dBa[nt][k]);
+        dCa[nt][k] = mm(bf, st.get8(lx, blk(k), ks), dCa[nt][k]);
+        dBa[nt][k] = mm(cf, st.tr8(lx, ks, blk(k)), dBa[nt][k]);
       }
     }
     const int64_t at = (c.t0 * G + grp) * N, all = a.p.seq.n_tokens * int64_t(G) * N * sub;
