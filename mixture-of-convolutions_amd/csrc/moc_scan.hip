@@ -576,24 +576,38 @@ size_t prep_bytes(const Scan& p) {
 }
 
 // Segments: a walk's workgroups are heads x segments, and 768 of them are on the card at
-// a time (three a CU, what registers and LDS allow): one round of them, as a second one
-// would run with the card part empty.  A segment has 256 tokens at least, as every one but
-// the last is walked twice.
+// a time (three a CU, what registers and LDS allow): at most one round of them where
+// sequences are cut, as a second one would run with the card part empty (16384 tokens, 32
+// heads of 64 x 128, forward and backward: 496 us with 768, 523 with 512, 538 with 1024).
+//
+// Cutting halves a walk's length at the price of a second walk, without output, and the
+// joining.  In units of one workgroup's time for a chunk, alone on its CU (3 us for bf16, 7
+// to 11 for fp32), a walk of q chunks takes q f, f = 1/4 + 3/4 of the workgroups a CU (at
+// least 1), the first walk half of that, and launches and joining 4 (bf16) or 1.3 (fp32).
+// The least of whole sequences, segments from 256 and segments from 128 tokens on is taken
+// (us, whole / 256 / 128: bf16 8 x 777 tokens, 24 heads of 64 x 64: 41 / 50 / 50; 16 x 1000, 8
+// heads of 64 x 128: 60 / 52 / 54; fp32 8 x 600, 12 heads of 64 x 64: 77 / 64 / 46).
 int64_t segment(const Scan& p) {
   const int64_t n = p.seq.n_tokens, heads = p.H * ((p.P + kTile - 1) / kTile);
-  const int64_t longest = p.seq.cu == nullptr ? p.seq.seq_len : n;
+  const bool packed = p.seq.cu != nullptr;
+  const int64_t longest = packed ? n : p.seq.seq_len, seqs = packed ? 1 : n / longest;
+  const int64_t whole = (longest + kQ - 1) / kQ * kQ;
   int64_t want = 768 / heads;  // segments of the whole token axis
   if (want < 1) want = 1;
-  if (p.seq.cu == nullptr) {  // the same number in every sequence
-    want /= n / longest;
-    if (want < 1) want = 1;
-    want *= n / longest;
+  if (!packed) want = want < seqs ? seqs : want / seqs * seqs;  // the same number in every sequence
+  const int64_t even = ((n + want - 1) / want + kQ - 1) / kQ * kQ;
+  auto cost = [&](int64_t seg) {
+    const double wgs = static_cast<double>(heads * seqs * ((longest + seg - 1) / seg));
+    const double f = 0.25 + 0.75 * wgs / 256.0;
+    const double walk = static_cast<double>(seg / kQ) * (f < 1.0 ? 1.0 : f);
+    return seg >= whole ? walk : 1.5 * walk + (p.x_dt == DT_BF16 ? 4.0 : 1.3);
+  };
+  int64_t best = whole;
+  for (int64_t least : {256, 128}) {
+    const int64_t seg = even < least ? least : even;
+    if (seg < whole && cost(seg) < cost(best)) best = seg;
   }
-  int64_t seg = (n + want - 1) / want;
-  seg = (seg + kQ - 1) / kQ * kQ;
-  if (seg < 256) seg = 256;
-  const int64_t whole = (longest + kQ - 1) / kQ * kQ;
-  return seg < whole ? seg : whole;
+  return best;
 }
 
 Args make_args(const Scan& p, void* prep) {
