@@ -15,6 +15,9 @@
 // of the fp32 matrix instructions.
 #pragma once
 
+#include <initializer_list>
+#include <type_traits>
+
 #include "moc_kernels.h"
 #include "moc_rows.h"
 
@@ -163,15 +166,32 @@ struct Raw<DT_F32> {
 
 // Rows (tokens, or channels of a state) of a tensor from one of them on: element
 // (row, col) lies at base + row * stride + col; rows from n on and columns from `cols` on
-// read as 0 and are not written.  VEC: column counts and strides are multiples of 8 and
-// base is aligned to 16 bytes: accesses go through a buffer resource that ends behind row
-// n - 1, whose range check makes the zeros without a branch (a lane whose columns are not
-// there has an offset that no range reaches), and a lane's offset is the same for every
-// chunk of a walk.
+// read as 0 and are not written.  VEC: column counts and strides are multiples of it (8 for
+// bf16, or 4; 0: any) and base is aligned to as many elements (16 bytes at most): accesses
+// go through a buffer resource that ends behind row n - 1, whose range check makes the zeros
+// without a branch (a lane whose columns are not there has an offset that no range reaches),
+// and a lane's offset is the same for every chunk of a walk.
 constexpr uint32_t kNowhere = 0x80000000u;
 constexpr int64_t kMaxStride = int64_t(1) << 22;  // VEC: 64 rows stay below kNowhere
 
-template <int DT, bool VEC>
+// 8 elements: all there or not (VEC 8, bf16), or two fours with a place of their own each
+template <int VEC>
+__device__ __forceinline__ void load8(Raw<DT_BF16>& v, __amdgpu_buffer_rsrc_t r, int lo, int hi, int s) {
+  if constexpr (VEC == 8) {
+    v.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lo, s, 0));
+  } else {
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, lo, s, 0));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, hi, s, 0));
+    v.w = u32x4{a[0], a[1], b[0], b[1]};
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void load8(Raw<DT_F32>& v, __amdgpu_buffer_rsrc_t r, int lo, int hi, int s) {
+  v.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lo, s, 0));
+  v.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, hi, s, 0));
+}
+
+template <int DT, int VEC>
 struct Rows {
   static constexpr int E = DT == DT_BF16 ? 2 : 4;
   const char* base;
@@ -190,15 +210,10 @@ struct Rows {
   // (row + more, col), `more` the same for every lane
   __device__ __forceinline__ Raw<DT> get8(int row, int col, int more = 0) const {
     Raw<DT> v;
-    if constexpr (VEC) {
+    if constexpr (VEC != 0) {
       const int o = off(row, col), s = more * static_cast<int>(stride) * E;
       const auto r = rsrc();
-      if constexpr (DT == DT_BF16) {
-        v.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, s, 0));
-      } else {
-        v.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, s, 0));
-        v.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o + 16, s, 0));
-      }
+      load8<VEC>(v, r, o, col + 4 < cols ? o + 4 * E : static_cast<int>(kNowhere), s);
     } else {
       row += more;
       const int have = row < n ? cols - col : 0;
@@ -224,7 +239,7 @@ struct Rows {
   // 4 elements as fp32
   __device__ __forceinline__ f32x4 get4(int row, int col) const {
     f32x4 v;
-    if constexpr (VEC) {
+    if constexpr (VEC != 0) {
       const int o = off(row, col);
       if constexpr (DT == DT_BF16) {
         const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc(), o, 0, 0));
@@ -241,7 +256,7 @@ struct Rows {
   }
   // (row + more, col), `more` the same for every lane
   __device__ __forceinline__ void put4(int row, int col, f32x4 v, int more = 0) const {
-    if constexpr (VEC) {
+    if constexpr (VEC != 0) {
       const int o = off(row, col), s = more * static_cast<int>(stride) * E;
       if constexpr (DT == DT_BF16) {
         const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
@@ -259,7 +274,7 @@ struct Rows {
   }
   // 8 elements, all or none of which are there
   __device__ __forceinline__ void put8(int row, int col, f32x4 lo, f32x4 hi) const {
-    if constexpr (VEC && DT == DT_BF16) {
+    if constexpr (VEC != 0 && DT == DT_BF16) {
       const u32x4 w{pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(hi[0], hi[1]), pack2(hi[2], hi[3])};
       __builtin_amdgcn_raw_buffer_store_b128(w, rsrc(), off(row, col), 0, 0);
     } else {
@@ -277,7 +292,7 @@ __host__ __device__ constexpr int64_t kept_cols(int64_t N) { return (N + 31) / 3
 // Rows at a place that moves by a uniform offset (a head's columns of a token, a head's rows
 // of the states) under one buffer resource: `off` elements from base, row by row `stride`.
 // `have`: how many of the elements asked for are there (at most 0: none).  VEC as in Rows.
-template <int DT, bool VEC>
+template <int DT, int VEC>
 struct Span {
   static constexpr int E = DT == DT_BF16 ? 2 : 4;
   const char* base;
@@ -289,15 +304,10 @@ struct Span {
   }
   __device__ __forceinline__ Raw<DT> get8(int row, int col, int have, int64_t off) const {
     Raw<DT> v;
-    if constexpr (VEC) {
+    if constexpr (VEC != 0) {
       const int o = have > 0 ? (row * stride + col) * E : static_cast<int>(kNowhere);
       const int s = static_cast<int>(off) * E;
-      if constexpr (DT == DT_BF16) {
-        v.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), o, s, 0));
-      } else {
-        v.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), o, s, 0));
-        v.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), o + 16, s, 0));
-      }
+      load8<VEC>(v, rsrc(), o, have > 4 ? o + 4 * E : static_cast<int>(kNowhere), s);
     } else {
       if (row >= n) have = 0;
       const int64_t at = int64_t(row) * stride + col + off;
@@ -321,7 +331,7 @@ struct Span {
   }
   __device__ __forceinline__ f32x4 get4(int row, int col, int have) const {
     f32x4 v;
-    if constexpr (VEC) {
+    if constexpr (VEC != 0) {
       const int o = have > 0 ? (row * stride + col) * E : static_cast<int>(kNowhere);
       if constexpr (DT == DT_BF16) {
         const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc(), o, 0, 0));
@@ -336,7 +346,7 @@ struct Span {
     return v;
   }
   __device__ __forceinline__ void put4(int row, int col, int have, int64_t off, f32x4 v) const {
-    if constexpr (VEC) {
+    if constexpr (VEC != 0) {
       const int o = have > 0 ? (row * stride + col) * E : static_cast<int>(kNowhere);
       const int s = static_cast<int>(off) * E;
       if constexpr (DT == DT_BF16) {
@@ -474,7 +484,7 @@ struct Tile {
 
 // 64 rows of a tensor on their way to an LDS tile of W columns: loads first (all in
 // flight), the tile once the last chunk's readers are done.
-template <int DT, bool VEC, int W, int THREADS>
+template <int DT, int VEC, int W, int THREADS>
 struct Staged {
   static constexpr int kLoads = 8 * W / THREADS;  // vectors of 8 of a thread
   Raw<DT> v[kLoads];
@@ -486,7 +496,7 @@ struct Staged {
   __device__ __forceinline__ void load(const Span<DT, VEC>& src, int rows, int cols, int64_t off) {
     constexpr int kStep = THREADS / (W / 8);
     // (without a resource's range check the span's own end is checked here, for every step)
-    if (!VEC && rows > src.n) rows = src.n;
+    if (VEC == 0 && rows > src.n) rows = src.n;
 #pragma unroll
     for (int k = 0; k < kLoads; ++k)
       v[k] = src.get8(row(0), col(k), row(0) + k * kStep < rows ? cols - col(k) : 0, off + int64_t(k) * kStep * src.stride);
@@ -624,7 +634,7 @@ struct Args {
   float* u;         // [H][chunks][kQ] softplus(dt + bias), 0 behind a sequence's end
   double* s;        // [H][chunks][kQ] running sum of u A log2(e) within the chunk
   float* par;       // [H][2] A and D (or 0)
-  bool vec;         // 16-byte accesses of everything that the kernels load and store
+  int vec;          // VEC of everything that the kernels load and store
 };
 
 // Chunk `id`: false where there is none.
@@ -646,6 +656,16 @@ __device__ __forceinline__ bool chunk_at(const Args& a, int64_t id, Chunk& c) {
 }
 
 Args make_args(const Scan& p, void* prep);
+void align(Args& a, std::initializer_list<const void*> of_x, std::initializer_list<const void*> others);
+// f with a.vec as a constant
+template <int DT, typename F>
+void with_vec(const Args& a, F&& f) {
+  if constexpr (DT == DT_BF16) {
+    if (a.vec == 8) return f(std::integral_constant<int, 8>{});
+  }
+  if (a.vec == 4) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 0>{});
+}
 size_t prep_bytes(const Scan& p);
 // tokens of a segment: see moc_scan.hip
 int64_t segment(const Scan& p);
@@ -661,7 +681,7 @@ struct Walk {
   float* end;           // the same or null: state at its end
   float* seg_state;     // [segments][H][P][N]: state at each segment's start
   double* seg_decay;    // [segments][H]: log2 of a segment's decay
-  void* kept;           // [chunks][H][P][N] in the x dtype or null: state before each chunk
+  void* kept;           // [chunks][H][P][kept_cols(N)] in the x dtype or null: state before each chunk
 };
 size_t walk_bytes(const Args& a);   // seg_state and seg_decay
 void carve_walk(const Args& a, void* workspace, Walk& w);

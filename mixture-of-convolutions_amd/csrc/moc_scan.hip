@@ -88,13 +88,13 @@ __global__ __launch_bounds__(kThreads) void prep_kernel(Args a) {
 
 // ---------------------------------------------------------------------------
 // acc: states 16 nb + 4 g + r of one channel, from / to a [P][N] state's rows
-template <int NB, int DT, bool VEC>
+template <int NB, int DT, int VEC>
 __device__ __forceinline__ void load_state(const Rows<DT, VEC>& src, int row, f32x4 (&acc)[NB]) {
   const int n0 = 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) acc[nb] = src.get4(row, 16 * nb + n0);
 }
-template <int NB, int DT, bool VEC>
+template <int NB, int DT, int VEC>
 __device__ __forceinline__ void store_state(const Rows<DT, VEC>& dst, int row, const f32x4 (&acc)[NB]) {
   int n0 = 4 * ((threadIdx.x & 63) >> 4);
   // (the blocks' offsets are formed here each time: kept over a walk, they push others to
@@ -105,7 +105,7 @@ __device__ __forceinline__ void store_state(const Rows<DT, VEC>& dst, int row, c
 }
 
 // acc to a row of kept states (rounded to x's type: operands of the backward's products)
-template <int NB, int DT, bool VEC>
+template <int NB, int DT, int VEC>
 __device__ __forceinline__ void keep_state(const Rows<DT, VEC>& dst, int row, const f32x4 (&acc)[NB]) {
   int g8 = 8 * ((threadIdx.x & 63) >> 4);
   asm volatile("" : "+v"(g8));
@@ -174,7 +174,7 @@ constexpr int kForwardLds =
 // The state over one segment's chunks, forwards (REV false) or backwards.  LOCAL: from
 // zero, for segments that another one follows, to seg_state and seg_decay; else from the
 // state that enters the segment, kept before each chunk.
-template <int DT, int NT, bool VEC, bool REV, bool LOCAL>
+template <int DT, int NT, int VEC, bool REV, bool LOCAL>
 __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 : (NT == 2 ? 3 : 2))) void state_walk(Args a, Walk w) {
   constexpr int NP = kPlanes<DT>, NB = 4 * NT, W = 64 * NT;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(kThreads) void join_segments(Args a, Walk w) {
 }
 
 // ---------------------------------------------------------------------------
-template <int DT, int NT, bool VEC>
+template <int DT, int NT, int VEC>
 __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void forward_walk(Args a, Walk w, void* y) {
   constexpr int NP = kPlanes<DT>, NB = 4 * NT, W = 64 * NT;
   constexpr bool kCInLds = DT == DT_BF16;  // (three planes of it beside B's would not fit)
@@ -534,8 +534,7 @@ void with_types(const Args& a, F&& f) {
   const int nt = n_tiles(a.p.N);
 #define MOC_SCAN_CASE(DT, NT) \
   if (a.p.x_dt == DT && nt == NT) { \
-    if (a.vec) f(std::integral_constant<int, DT>{}, std::integral_constant<int, NT>{}, std::true_type{}); \
-    else f(std::integral_constant<int, DT>{}, std::integral_constant<int, NT>{}, std::false_type{}); \
+    with_vec<DT>(a, [&](auto VEC) { f(Int<DT>{}, Int<NT>{}, VEC); }); \
     return; \
   }
   MOC_SCAN_CASE(DT_BF16, 1) MOC_SCAN_CASE(DT_BF16, 2) MOC_SCAN_CASE(DT_BF16, 4)
@@ -610,6 +609,13 @@ int64_t segment(const Scan& p) {
   return best;
 }
 
+// a.vec for tensors of the x type and others (16 bytes) at these addresses
+void align(Args& a, std::initializer_list<const void*> of_x, std::initializer_list<const void*> others) {
+  const int size = a.p.x_dt == DT_BF16 ? 2 : 4;
+  if (a.vec == 8 && !aligned(of_x, 8 * size)) a.vec = 4;
+  if (!aligned(of_x, 4 * size) || !aligned(others, 16)) a.vec = 0;
+}
+
 Args make_args(const Scan& p, void* prep) {
   Args a{};
   a.p = p;
@@ -621,10 +627,15 @@ Args make_args(const Scan& p, void* prep) {
   a.u = static_cast<float*>(prep);
   a.s = reinterpret_cast<double*>(static_cast<char*>(prep) + up(n * 4));
   a.par = reinterpret_cast<float*>(static_cast<char*>(prep) + up(n * 4) + up(n * 8));
-  a.vec = p.P % 8 == 0 && p.N % 8 == 0 && aligned({p.x, p.B, p.C}, 16);
   // (a chunk's states lie under one buffer resource)
-  a.vec = a.vec && p.H * p.P * kept_cols(p.N) * 4 < int64_t(kNowhere) - 16;
-  for (int64_t st : {p.x_stride, p.b_stride, p.c_stride, p.H * p.P, p.G * p.N}) a.vec = a.vec && st % 8 == 0 && st < kMaxStride;
+  const bool small = p.H * p.P * kept_cols(p.N) * 4 < int64_t(kNowhere) - 16;
+  for (int v : {8, 4}) {
+    bool ok = small && a.vec == 0 && (v == 4 || p.x_dt == DT_BF16);
+    for (int64_t k : {p.P, p.N}) ok = ok && k % v == 0;
+    for (int64_t st : {p.x_stride, p.b_stride, p.c_stride, p.H * p.P, p.G * p.N}) ok = ok && st % v == 0 && st < kMaxStride;
+    if (ok) a.vec = v;
+  }
+  align(a, {p.x, p.B, p.C}, {});
   return a;
 }
 
@@ -679,7 +690,7 @@ void scan_forward(const Scan& p, void* y, const float* init, float* fin, void* s
                   hipStream_t st) {
   char* ws = static_cast<char*>(workspace);
   Args a = make_args(p, saved != nullptr ? saved : ws);
-  a.vec = a.vec && aligned({y, init, fin, saved, workspace}, 16);
+  align(a, {y}, {init, fin, saved, workspace});
   Walk w{};
   w.x = p.x;
   w.b = p.B;

@@ -121,7 +121,7 @@ constexpr int kBack = 256 * kHalves;  // threads of backward_chunk
 // 16 q.., 16 jb..) those of parity w / 4.  For fp32 the sums that da is formed from are
 // kept in 64 bits (Acc): da is one number for a whole chunk to a large part (z, and the
 // sums over the tokens behind), so that its rounding does not average out over tokens.
-template <int DT, int NT, bool VEC>
+template <int DT, int NT, int VEC>
 __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chunk(Args a, Back b) {
   using LY = Layout<DT, NT>;
   using Acc = typename LY::Acc;
@@ -506,7 +506,7 @@ void scan_backward(const Scan& p, const void* dy, bool has_init, const float* df
   Args a = make_args(p, const_cast<void*>(saved));
   const Bytes n = bytes_of(a);
   char* ws = static_cast<char*>(workspace);
-  a.vec = a.vec && aligned({dy, dfin, saved, workspace, g.dx, g.dB, g.dC, g.dinit}, 16);
+  align(a, {dy, g.dx, g.dB, g.dC}, {dfin, saved, workspace, g.dinit});
   Walk w{};
   w.x = dy;
   w.b = p.C;
@@ -547,10 +547,7 @@ void scan_backward(const Scan& p, const void* dy, bool has_init, const float* df
   using BF = std::integral_constant<int, DT_BF16>;
   using F = std::integral_constant<int, DT_F32>;
   auto nt = [&](auto DT) {
-    auto with = [&](auto NT) {
-      if (a.vec) go(DT, NT, std::true_type{});
-      else go(DT, NT, std::false_type{});
-    };
+    auto with = [&](auto NT) { with_vec<DT.value>(a, [&](auto VEC) { go(DT, NT, VEC); }); };
     if (p.N <= 64) with(std::integral_constant<int, 1>{});
     else if (p.N <= 128) with(std::integral_constant<int, 2>{});
     else with(std::integral_constant<int, 4>{});

@@ -448,6 +448,13 @@ def test_scan_reads_slices_in_place(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B, T, H, P, G, N", [
+    (2, 130, 4, 36, 2, 100), (1, 200, 2, 20, 1, 12), (1, 77, 2, 68, 1, 132), (3, 65, 2, 64, 1, 4), (1, 70, 1, 4, 1, 252)])
+def test_scan_of_multiples_of_four(dtype, B, T, H, P, G, N):
+    check_scan(scan_inputs((B, T), H, P, G, N, dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("H, P, G, N", [(6, 33, 3, 100), (2, 40, 1, 128), (2, 72, 1, 130), (2, 80, 1, 256), (3, 5, 1, 7)])
 def test_scan_uses_nothing_behind_the_last_token(dtype, H, P, G, N):
     """Whatever lies behind the last token of x, dt, B and C in memory (here NaN or 0) changes no bit."""
