@@ -470,14 +470,26 @@ __global__ __launch_bounds__(kThreads) void sum_subs(const float* __restrict__ p
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
-// Parts of a group's heads: about 1024 workgroups (four a CU) where the heads give
-// them; each part adds 8 N bytes a token and group to the traffic.
+// Parts of a group's heads.  A CU holds one workgroup, so that the time goes with the rounds
+// of 256 of them: each takes a part's heads and, measured in heads (6.4 us for bf16 at 64 x
+// 128, more for fp32), 1.25 (fp32: 0.75) for what is done once a workgroup.  More than one
+// part also costs the launch that adds them and their way through memory.  16384 bf16 tokens,
+// 32 heads of one group: 1 part 213 us, 2 parts 222 + 9, 4 parts 236 + 15; forward and
+// backward of 8000 bf16 tokens, 40 heads of 4 groups, 1 part 323 us, 2 parts 391.
 int64_t subs_of(const Args& a) {
   const int64_t wgs = a.chunks * a.p.G, hpg = a.p.H / a.p.G;
-  int64_t s = (1024 + wgs - 1) / wgs;
-  if (s > hpg) s = hpg;
-  const int64_t per = (hpg + s - 1) / s;
-  return (hpg + per - 1) / per;
+  const bool bf = a.p.x_dt == DT_BF16;
+  const double once = bf ? 1.25 : 0.75, launch = bf ? 0.5 : 0.3, way = (bf ? 1.8e-5 : 0.8e-5) * a.p.N;
+  int64_t best = 1;
+  double least = 0.0;
+  for (int64_t s = 1; s <= hpg && s <= 64; ++s) {
+    const int64_t per = (hpg + s - 1) / s, parts = (hpg + per - 1) / per;
+    if (parts != s) continue;
+    const double cost = static_cast<double>((wgs * s + 255) / 256) * (static_cast<double>(per) + once) +
+                        (s > 1 ? launch + way * static_cast<double>(wgs * s) : 0.0);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
 }
 
 struct Bytes {
