@@ -23,7 +23,7 @@
 // The gradient in which it shows is dA, a sum of products of random sign of h and dh: about
 // 0.001 relative beside the 0.0017 of its own rounding to bf16, more where decays are slow.
 //
-// 16384 bf16 tokens, 32 heads of 64 x 128: 235 us for 470 MB (2 TB/s; 302 us where the next
+// 16384 bf16 tokens, 32 heads of 64 x 128: 214 us for 470 MB (2.2 TB/s; 67 us more where the next
 // head's loads were waited for early, by reloads of spilled addresses, by loads of A, C and
 // D behind them and by moves of their registers).  One workgroup of 8 waves fits a CU (230
 // registers, 93 KB), and the phases of a head, parted by three barriers, overlap little:
