@@ -33,12 +33,10 @@ _DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
 _Q = 64  # tokens of a chunk of the plain scan
 
 
-_PKG = str(Path(__file__).resolve().parents[1] / "mixture-of-convolutions_amd")
-if _PKG not in sys.path:
-    sys.path.insert(0, _PKG)
-
-
 def _moc():
+    pkg = str(Path(__file__).resolve().parents[1] / "mixture-of-convolutions_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
     import moc
     return moc
 
