@@ -12,7 +12,9 @@
 // Matrix operands are bf16 planes: a bf16 tensor is one plane, an fp32 value three
 // (v = p0 + p1 + p2 exactly: 24 bits of significand in three times 8), whose six
 // products of at least 2^-16 relative weight give fp32's accuracy at 6/16 of the cost
-// of the fp32 matrix instructions.
+// of the fp32 matrix instructions.  What the kernels form themselves (the decay-weighted
+// tile, the state) enters a product with bf16 inputs in two planes: 2^-16 of it at most is
+// lost, a 256th of what the result's own rounding loses.
 #pragma once
 
 #include <initializer_list>
@@ -41,6 +43,9 @@ struct Frag {
 
 template <int DT>
 constexpr int kPlanes = DT == DT_BF16 ? 1 : 3;
+// planes of an operand that a kernel formed, beside inputs of NP planes
+template <int NP>
+constexpr int kFormed = NP == 1 ? 2 : NP;
 
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
@@ -52,6 +57,9 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mm(const Frag<1>& a, const Frag<1>& b, f32x4 c) { return mfma(a.v[0], b.v[0], c); }
 __device__ __forceinline__ f32x4 mm(const Frag<1>& a, const Frag<2>& b, f32x4 c) {
   return mfma(a.v[0], b.v[0], mfma(a.v[0], b.v[1], c));
+}
+__device__ __forceinline__ f32x4 mm(const Frag<2>& a, const Frag<1>& b, f32x4 c) {
+  return mfma(a.v[0], b.v[0], mfma(a.v[1], b.v[0], c));
 }
 __device__ __forceinline__ f32x4 mm(const Frag<3>& a, const Frag<3>& b, f32x4 c) {
   f32x4 t = mfma(a.v[0], b.v[2], f32x4{0.f, 0.f, 0.f, 0.f});
@@ -479,6 +487,51 @@ struct Tile {
   static __device__ __forceinline__ s16x4 tr(const uint16_t* q) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         (__attribute__((address_space(3))) s16x4*)(const_cast<uint16_t*>(q)));
+  }
+};
+
+// The blocks of 16 x 16 on and below the diagonal of a 64 x 64 tile, row by row of blocks, a
+// block's rows 32 bytes each: 10 KB for two planes, where a whole tile's 16 would leave room
+// for two workgroups a CU in place of three.  (A 16-byte read's 16 lanes, see Lane, meet rows
+// 0-3 and 12-15 of one half of a block's columns and 4-11 of the other: every bank once.)
+template <int NP>
+struct Lower {
+  static constexpr int kPlane = 10 * 256;  // elements
+  static constexpr int kBytes = NP * kPlane * 2;
+  uint16_t* p;
+  static __device__ __forceinline__ constexpr int block(int ib, int jb) { return (ib * (ib + 1) / 2 + jb) * 256; }
+  // row 16 ib + li, columns 16 jb + 4 g..
+  __device__ __forceinline__ void put4(int li, int g, int ib, int jb, f32x4 v) const {
+    uint16_t* q = p + block(ib, jb) + 16 * li + 4 * g;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
+      *reinterpret_cast<u32x2*>(q + k * kPlane) = w;
+      if (k + 1 < NP) v -= f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
+    }
+  }
+  // row 16 ib + li, columns 32 ks + 8 g.. (2 ks <= ib; 0 right of the diagonal's block)
+  __device__ __forceinline__ Frag<NP> get8(int li, int g, int ib, int ks) const {
+    const uint16_t* q = p + block(ib, 2 * ks) + 16 * li + 8 * (g & 1) + 256 * (g >> 1);
+    Frag<NP> r;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      u32x4 w = *reinterpret_cast<const u32x4*>(q + k * kPlane);
+      if (2 * ks == ib) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = g < 2 ? w[e] : 0u;
+      }
+      r.v[k] = __builtin_bit_cast(s16x8, w);
+    }
+    return r;
+  }
+  // element (i, j), j <= i, as fp32
+  __device__ __forceinline__ float at(int i, int j) const {
+    const uint16_t* q = p + block(i >> 4, j >> 4) + 16 * (i & 15) + (j & 15);
+    float v = 0.f;
+#pragma unroll
+    for (int k = NP - 1; k >= 0; --k) v += bf16_to_f32(q[k * kPlane]);
+    return v;
   }
 };
 

@@ -169,7 +169,8 @@ constexpr int kWalkLds = kPlanes<DT> * kQ * (64 * NT + 64) * 2 + kQ * 4;
 // (B, and C where it is staged)
 template <int DT, int NT>
 constexpr int kForwardLds =
-    kPlanes<DT> * kQ * ((DT == DT_BF16 ? 2 : 1) * 64 * NT + 128) * 2 + Decays::kBytes + 16;
+    kPlanes<DT> * kQ * ((DT == DT_BF16 ? 2 : 1) * 64 * NT + 64) * 2 + Lower<kFormed<kPlanes<DT>>>::kBytes +
+    Decays::kBytes + 16;
 
 // The state over one segment's chunks, forwards (REV false) or backwards.  LOCAL: from
 // zero, for segments that another one follows, to seg_state and seg_decay; else from the
@@ -278,13 +279,13 @@ __global__ __launch_bounds__(kThreads) void join_segments(Args a, Walk w) {
 // ---------------------------------------------------------------------------
 template <int DT, int NT, int VEC>
 __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void forward_walk(Args a, Walk w, void* y) {
-  constexpr int NP = kPlanes<DT>, NB = 4 * NT, W = 64 * NT;
+  constexpr int NP = kPlanes<DT>, MP = kFormed<NP>, NB = 4 * NT, W = 64 * NT;
   constexpr bool kCInLds = DT == DT_BF16;  // (three planes of it beside B's would not fit)
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const Tile<NP, W> bt{reinterpret_cast<uint16_t*>(smem)};
   const Tile<NP, W> ct{reinterpret_cast<uint16_t*>(smem + bt.kBytes)};
   const Tile<NP, 64> xt{reinterpret_cast<uint16_t*>(smem + (kCInLds ? 2 : 1) * bt.kBytes)};
-  const Tile<NP, 64> mt{xt.p + xt.kBytes / 2};
+  const Lower<MP> mt{xt.p + xt.kBytes / 2};
   const Decays dec(reinterpret_cast<char*>(mt.p + mt.kBytes / 2));
   int* odd = reinterpret_cast<int*>(reinterpret_cast<char*>(dec.s) + Decays::kBytes);  // [2], by chunk parity
   Lane<W> lw;
@@ -308,8 +309,6 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
   for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float* from = s.first ? w.start : w.seg_state;
   if (from != nullptr) load_state<NB>(state(from, s.first ? s.m : int64_t(blockIdx.x)), row, acc);
-  // the block right of the diagonal that a 32-token product step reads (no wave writes it)
-  if ((wave & 1) == 0) mt.put4(lx, wave, wave + 1, f32x4{0.f, 0.f, 0.f, 0.f});
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   const int64_t at = (int64_t(h) * a.chunks + s.c0) * kQ;
   const int64_t xcol = int64_t(h) * P + p0, bcol = int64_t(h / (a.p.H / a.p.G)) * N;
@@ -379,7 +378,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
             v[r] = 4 * g + r <= li ? m : 0.f;
           }
         }
-        mt.put4(lx, ib[q], jb[q], v);
+        mt.put4(li, g, ib[q], jb[q], v);
       }
     };
     // (a pair is 4 i + j, in blocks)
@@ -401,7 +400,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
         float f[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = acc[2 * ks + e / 4][e % 4];
-        const Frag<NP> hf = split<NP>(f);
+        const Frag<MP> hf = split<MP>(f);
 #pragma unroll
         for (int ib = 0; ib < 4; ++ib) {
           Frag<NP> cf;
@@ -437,8 +436,8 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
       const Rows<DT, VEC> yrow(y, ((s.t0 + int64_t(k) * kQ) * a.p.H + h) * P + p0, a.p.H * P, n, cols);
 #pragma unroll
       for (int ib = 0; ib < 4; ++ib) {
-        ya[ib] = mm(xm[0], mt.get8(lx, ib, 0), ya[ib]);
-        if (ib >= 2) ya[ib] = mm(xm[1], mt.get8(lx, ib, 1), ya[ib]);
+        ya[ib] = mm(xm[0], mt.get8(li, g, ib, 0), ya[ib]);
+        if (ib >= 2) ya[ib] = mm(xm[1], mt.get8(li, g, ib, 1), ya[ib]);
         // (without D skip is 0: no branch between a product and the first use of its result,
         // whose wait states the compiler has been seen to leave out on the path around a body)
         ya[ib] += skip * xt.get4(lx, ib, wave);
