@@ -280,22 +280,30 @@ struct Rows {
         if (k < have) store_any(const_cast<char*>(base), DT, row * stride + col + k, v[k]);
     }
   }
-  // 8 elements, all or none of which are there
-  __device__ __forceinline__ void put8(int row, int col, f32x4 lo, f32x4 hi) const {
-    if constexpr (VEC != 0 && DT == DT_BF16) {
-      const u32x4 w{pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(hi[0], hi[1]), pack2(hi[2], hi[3])};
+  // 8 bf16 elements as they are, all or none of which are there
+  __device__ __forceinline__ void put8(int row, int col, s16x8 v) const {
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+    if constexpr (VEC != 0) {
       __builtin_amdgcn_raw_buffer_store_b128(w, rsrc(), off(row, col), 0, 0);
-    } else {
-      put4(row, col, lo);
-      put4(row, col + 4, hi);
+    } else if (row < n && col < cols) {
+      uint16_t* p = reinterpret_cast<uint16_t*>(const_cast<char*>(base)) + row * stride + col;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        p[2 * k] = static_cast<uint16_t>(w[k]);
+        p[2 * k + 1] = static_cast<uint16_t>(w[k] >> 16);
+      }
     }
   }
 };
 
-// States kept for the backward pass: [channels][kept_cols(N)], a row's states in the order
+// States kept for the backward pass: [channels][kept_planes][kept_cols(N)] in the x dtype
+// (fp32 as they are, for bf16 in the two planes in which they enter its products: 4 bytes a
+// state in both), a row's states in the order
 // in which the walks' lanes hold them: the 4 states of lane group g in the lower and the
 // upper block of 16 of 32 states next to each other, so that a lane stores 8 at a time.
 __host__ __device__ constexpr int64_t kept_cols(int64_t N) { return (N + 31) / 32 * 32; }
+template <int DT>
+constexpr int kKeptPlanes = DT == DT_BF16 ? 2 : 1;
 
 // Rows at a place that moves by a uniform offset (a head's columns of a token, a head's rows
 // of the states) under one buffer resource: `off` elements from base, row by row `stride`.
@@ -559,11 +567,6 @@ struct Staged {
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) t.put8(row(k), col(k), v[k].frag());
   }
-  template <int NP>
-  __device__ __forceinline__ void put_kept(const Tile<NP, W>& t) const {
-#pragma unroll
-    for (int k = 0; k < kLoads; ++k) t.put44(row(k), col(k), v[k].frag());
-  }
   __device__ __forceinline__ uint32_t odd() const {
     uint32_t r = 0;
 #pragma unroll
@@ -572,6 +575,38 @@ struct Staged {
   }
   static __device__ __forceinline__ int row(int k) { return threadIdx.x / (W / 8) + k * (THREADS / (W / 8)); }
   static __device__ __forceinline__ int col(int) { return threadIdx.x % (W / 8) * 8; }
+};
+
+// 64 rows of kept states on their way to an LDS tile of W columns.
+template <int DT, int VEC, int W, int THREADS>
+struct KeptStates {
+  static constexpr int PL = kKeptPlanes<DT>, NP = kFormed<kPlanes<DT>>;
+  Staged<DT, VEC, W, THREADS> s[PL];
+  static constexpr int kLoads = Staged<DT, VEC, W, THREADS>::kLoads;
+  // `rows` rows of a span at `off`, `cols` columns of a plane's NK
+  __device__ __forceinline__ void load(const Span<DT, VEC>& src, int rows, int cols, int64_t off, int NK) {
+#pragma unroll
+    for (int p = 0; p < PL; ++p) s[p].load(src, rows, cols, off + p * NK);
+  }
+  __device__ __forceinline__ Frag<NP> frag(int k) const {
+    if constexpr (PL == 1) {
+      return s[0].v[k].frag();
+    } else {
+      return Frag<2>{{s[0].v[k].frag().v[0], s[1].v[k].frag().v[0]}};
+    }
+  }
+  __device__ __forceinline__ void get(int k, float (&f)[8]) const {
+    if constexpr (PL == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = s[0].v[k].lo[e], f[4 + e] = s[0].v[k].hi[e];
+    } else {
+      join(frag(k), f);
+    }
+  }
+  __device__ __forceinline__ void put(const Tile<NP, W>& t) const {
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) t.put44(s[0].row(k), s[0].col(k), frag(k));
+  }
 };
 
 // The factors of a chunk's decays.  For tokens of two blocks of 16, i's after j's,
@@ -734,7 +769,7 @@ struct Walk {
   float* end;           // the same or null: state at its end
   float* seg_state;     // [segments][H][P][N]: state at each segment's start
   double* seg_decay;    // [segments][H]: log2 of a segment's decay
-  void* kept;           // [chunks][H][P][kept_cols(N)] in the x dtype or null: state before each chunk
+  void* kept;           // [chunks][H][P] rows of kept states or null: state before each chunk
 };
 size_t walk_bytes(const Args& a);   // seg_state and seg_decay
 void carve_walk(const Args& a, void* workspace, Walk& w);

@@ -104,13 +104,32 @@ __device__ __forceinline__ void store_state(const Rows<DT, VEC>& dst, int row, c
   for (int nb = 0; nb < NB; ++nb) dst.put4(row, 16 * nb + n0, acc[nb]);
 }
 
-// acc to a row of kept states (rounded to x's type: operands of the backward's products)
+// The kept states of one head's channels from p0 on, `cols` of them, of chunk `id`.
+template <int DT, int VEC>
+__device__ __forceinline__ Rows<DT, VEC> kept_rows(const Args& a, void* kept, int64_t id, int h, int p0, int cols, int NK) {
+  const int row = kKeptPlanes<DT> * NK;
+  return Rows<DT, VEC>(kept, ((id * a.p.H + h) * a.p.P + p0) * row, row, cols, row);
+}
+// acc to a row of them
 template <int NB, int DT, int VEC>
-__device__ __forceinline__ void keep_state(const Rows<DT, VEC>& dst, int row, const f32x4 (&acc)[NB]) {
+__device__ __forceinline__ void keep_state(const Rows<DT, VEC>& dst, int row, int NK, const f32x4 (&acc)[NB]) {
   int g8 = 8 * ((threadIdx.x & 63) >> 4);
   asm volatile("" : "+v"(g8));
 #pragma unroll
-  for (int nb = 0; nb < NB; nb += 2) dst.put8(row, 16 * nb + g8, acc[nb], acc[nb + 1]);
+  for (int nb = 0; nb < NB; nb += 2) {
+    const int col = 16 * nb + g8;
+    if constexpr (DT == DT_BF16) {
+      const float f[8] = {acc[nb][0],     acc[nb][1],     acc[nb][2],     acc[nb][3],
+                          acc[nb + 1][0], acc[nb + 1][1], acc[nb + 1][2], acc[nb + 1][3]};
+      const Frag<2> v = split<2>(f);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (16 * nb < NK) dst.put8(row, col + p * NK, v.v[p]);
+    } else {
+      dst.put4(row, col, acc[nb]);
+      dst.put4(row, col + 4, acc[nb + 1]);
+    }
+  }
 }
 
 // 8 products of a transposed x operand and the tokens' weights w[0..8) as three planes
@@ -223,7 +242,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 :
     lw.refresh(), lx.refresh();
     const int i = REV ? s.chunks - 1 - k : k;
     if (!LOCAL && w.kept != nullptr && !(k == 0 && from == nullptr))
-      keep_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + i) * a.p.H + h) * P + p0) * NK, NK, cols, NK), row, acc);
+      keep_state<NB>(kept_rows<DT, VEC>(a, w.kept, s.c0 + i, h, p0, cols, NK), row, NK, acc);
     sx.put(xt);
     sb.put(bt);
     const double last = __shfl(sv, 63);
@@ -387,7 +406,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
     else if (wave == 2) m_blocks(Int<8>{}, Int<9>{}, Int<10>{});
     else m_blocks(Int<13>{}, Int<14>{}, Int<15>{});
     if (w.kept != nullptr && !(k == 0 && from == nullptr))
-      keep_state<NB>(Rows<DT, VEC>(w.kept, (((s.c0 + k) * a.p.H + h) * P + p0) * NK, NK, cols, NK), row, acc);
+      keep_state<NB>(kept_rows<DT, VEC>(a, w.kept, s.c0 + k, h, p0, cols, NK), row, NK, acc);
     if (k + 1 < s.chunks) fetch(k + 1);
     f32x4 ya[4];
 #pragma unroll
@@ -678,7 +697,7 @@ using namespace scan;
 
 size_t scan_saved_bytes(const Scan& p) {
   const Args a = make_args(p, nullptr);
-  return prep_bytes(p) + size_t(a.chunks) * p.H * p.P * kept_cols(p.N) * (p.x_dt == DT_BF16 ? 2 : 4);
+  return prep_bytes(p) + size_t(a.chunks) * p.H * p.P * kept_cols(p.N) * 4;
 }
 
 size_t scan_forward_workspace(const Scan& p, bool saved) {

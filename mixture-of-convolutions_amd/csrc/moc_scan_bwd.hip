@@ -18,10 +18,9 @@
 // One workgroup takes a chunk, a group and some of the group's heads: G is formed
 // once for all of them, and dB, dC stay in its registers over its heads (a sum over
 // heads through memory would move N fp32 values a token and head, more than x).  h and
-// dh come from memory in the x dtype (2 P N / kQ elements a token and head: at 64 x 128
-// four times x).  For bf16 that is one rounding of a matrix operand, as B's and C's is.
-// The gradient in which it shows is dA, a sum of products of random sign of h and dh: about
-// 0.001 relative beside the 0.0017 of its own rounding to bf16, more where decays are slow.
+// dh come from memory in 4 bytes a state (2 P N / kQ states a token and head: at 64 x 128
+// eight times a bf16 x), for bf16 in two planes: in one they would move half as much, but each
+// pair's product in dA, a sum over all tokens, would be off by 0.001 and more.
 //
 // 16384 bf16 tokens, 32 heads of 64 x 128: 214 us for 470 MB (2.2 TB/s; 67 us more where the next
 // head's loads were waited for early, by reloads of spilled addresses, by loads of A, C and
@@ -40,7 +39,7 @@ constexpr int kThreads = 256;
 
 struct Back {
   const void* dy;       // [tokens][H][P] contiguous
-  const void* h;        // [chunks][H][P][kept_cols(N)], x dtype: state before each chunk
+  const void* h;        // [chunks][H][P] rows of kept states: state before each chunk
   const void* dh;       // the same: gradient of the state behind each chunk
   bool has_init, has_dfin;
   void *dx, *ddt, *dB, *dC;
@@ -91,6 +90,13 @@ __device__ __forceinline__ Acc dot(const Raw<DT_BF16>& a, const Raw<DT_BF16>& b)
   return s;
 }
 template <typename Acc>
+__device__ __forceinline__ Acc dot(const float (&a)[8], const float (&b)[8]) {
+  Acc s = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s += static_cast<Acc>(a[k]) * b[k];
+  return s;
+}
+template <typename Acc>
 __device__ __forceinline__ Acc dot(const Raw<DT_F32>& a, const Raw<DT_F32>& b) {
   Acc s = 0;
 #pragma unroll
@@ -98,21 +104,31 @@ __device__ __forceinline__ Acc dot(const Raw<DT_F32>& a, const Raw<DT_F32>& b) {
   return s;
 }
 
-// LDS of backward_chunk, at most 158 KB (bf16, N over 128).
+// LDS of backward_chunk, at most 135 KB.
 template <int DT, int NT>
 struct Layout {
-  static constexpr int NP = kPlanes<DT>;
-  // state tiles of 64 at a time: all of them, with B's and C's beside them (bf16: loads return
-  // in order, so that one of B or C behind the next head's would wait for those, 296 -> 277 us
-  // at 16384 tokens, 32 heads, 64 x 128), or one (three planes, which leave no room for B and C)
-  static constexpr int TW = DT == DT_BF16 ? NT : 1, W = 64 * TW;
+  static constexpr int NP = kPlanes<DT>, MP = kFormed<NP>;
+  // B and C whole in LDS (bf16: loads return in order, so that one of B or C behind the next
+  // head's would wait for those, 296 -> 277 us at 16384 tokens, 32 heads, 64 x 128; three
+  // planes leave no room)
   static constexpr bool kInLds = DT == DT_BF16;
+  static constexpr int WB = 64 * NT;
+  // state tiles of 64 at a time: two where B and C leave room for them, or one
+  static constexpr int TW = DT == DT_BF16 && NT <= 2 ? NT : 1, W = 64 * TW;
   using Acc = typename std::conditional<DT == DT_BF16, float, double>::type;
   static constexpr int kSums = (4 + 2 + 4 + 4 + 1) * kQ;  // Acc values
-  static constexpr int kBytes = 3 * Tile<NP, 64>::kBytes + (kInLds ? 4 : 2) * Tile<NP, W>::kBytes + Decays::kBytes +
+  static constexpr int kBytes = 2 * Tile<NP, 64>::kBytes + Tile<MP, 64>::kBytes + 2 * Tile<MP, W>::kBytes +
+                                (kInLds ? 2 * Tile<NP, WB>::kBytes : 0) + Decays::kBytes +
                                 kSums * static_cast<int>(sizeof(Acc));
   static constexpr int kWaves = 2;  // a SIMD: one workgroup a CU (with more, registers spill)
 };
+
+// (the lanes' offsets in tiles of two widths: the same object where the widths are one)
+template <bool SAME, typename T, typename U>
+__device__ __forceinline__ decltype(auto) same_or_own(U& u) {
+  if constexpr (SAME) return (u);
+  else return T();
+}
 
 constexpr int kHalves = 2;
 constexpr int kBack = 256 * kHalves;  // threads of backward_chunk
@@ -125,14 +141,16 @@ template <int DT, int NT, int VEC>
 __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chunk(Args a, Back b) {
   using LY = Layout<DT, NT>;
   using Acc = typename LY::Acc;
-  constexpr int NP = LY::NP, TW = LY::TW, W = LY::W, Q = 4 / kHalves;
+  constexpr int NP = LY::NP, MP = LY::MP, TW = LY::TW, W = LY::W, WB = LY::WB, Q = 4 / kHalves;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int kT = Tile<NP, 64>::kBytes, kS = Tile<NP, W>::kBytes;
-  const Tile<NP, 64> xt{reinterpret_cast<uint16_t*>(smem)}, yt{reinterpret_cast<uint16_t*>(smem + kT)},
-      mt{reinterpret_cast<uint16_t*>(smem + 2 * kT)};
-  const Tile<NP, W> ht{reinterpret_cast<uint16_t*>(smem + 3 * kT)}, dt{reinterpret_cast<uint16_t*>(smem + 3 * kT + kS)},
-      bt{reinterpret_cast<uint16_t*>(smem + 3 * kT + 2 * kS)}, ct{reinterpret_cast<uint16_t*>(smem + 3 * kT + 3 * kS)};
-  char* rest = smem + 3 * kT + (LY::kInLds ? 4 : 2) * kS;
+  const Tile<NP, 64> xt{reinterpret_cast<uint16_t*>(smem)}, yt{reinterpret_cast<uint16_t*>(smem + xt.kBytes)};
+  char* rest = smem + 2 * xt.kBytes;
+  const Tile<MP, 64> mt{reinterpret_cast<uint16_t*>(rest)};
+  rest += mt.kBytes;
+  const Tile<MP, W> ht{reinterpret_cast<uint16_t*>(rest)}, dt{reinterpret_cast<uint16_t*>(rest + ht.kBytes)};
+  rest += 2 * ht.kBytes;
+  const Tile<NP, WB> bt{reinterpret_cast<uint16_t*>(rest)}, ct{reinterpret_cast<uint16_t*>(rest + bt.kBytes)};
+  rest += LY::kInLds ? 2 * bt.kBytes : 0;
   const Decays dec(rest);
   Acc* Kp = reinterpret_cast<Acc*>(rest + Decays::kBytes);  // [4][64] column sums by row block
   Acc* Rv = Kp + 4 * kQ;                                    // [2][64] row sums by half
@@ -142,11 +160,12 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   __shared__ Acc zp[2][4 * kHalves];                        // z, <x, dy> by wave
   Lane<64> lx;
   Lane<W> lw;
+  typename std::conditional<W == WB, Lane<W>&, Lane<WB>>::type lb(same_or_own<W == WB, Lane<WB>>(lw));
   const int lane = threadIdx.x & 63;
   int li = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wid & 3, half = wid >> 2;
   const int H = static_cast<int>(a.p.H), P = static_cast<int>(a.p.P), G = static_cast<int>(a.p.G),
-            N = static_cast<int>(a.p.N), NK = static_cast<int>(kept_cols(N));
+            N = static_cast<int>(a.p.N), NK = static_cast<int>(kept_cols(N)), NR = kKeptPlanes<DT> * NK;
   const int grp = blockIdx.y / b.subs, sub = blockIdx.y % b.subs, hpg = H / G;
   const int h_lo = grp * hpg + sub * b.per_sub;
   const int h_hi = (sub + 1) * b.per_sub < hpg ? h_lo + b.per_sub : (grp + 1) * hpg;
@@ -165,20 +184,20 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   const Span<DT, VEC> xrow(a.p.x, c.t0 * a.p.x_stride, a.p.x_stride, n);
   const Span<DT, VEC> yrow(b.dy, c.t0 * H * P, int64_t(H) * P, n);
   const Span<DT, VEC> orow(b.dx, c.t0 * H * P, int64_t(H) * P, n);
-  const Span<DT, VEC> hrow(b.h, c.id * H * P * NK, NK, int64_t(H) * P);
-  const Span<DT, VEC> drow(b.dh, c.id * H * P * NK, NK, int64_t(H) * P);
+  const Span<DT, VEC> hrow(b.h, c.id * H * P * NR, NR, int64_t(H) * P);
+  const Span<DT, VEC> drow(b.dh, c.id * H * P * NR, NR, int64_t(H) * P);
   auto blk = [&](int k) { return k * kHalves + half; };  // this wave's column blocks
 
   // the loads of a head's (and channel tile's) tensors, ahead of their use
   Staged<DT, VEC, 64, kBack> sx, sy;
-  Staged<DT, VEC, W, kBack> sh, sd;
+  KeptStates<DT, VEC, W, kBack> sh, sd;
   double sv = 0.0;
   float uv = 0.f, rate_v = 0.f, skip_v = 0.f;
   auto width = [&](int pt) { return P - pt * kTile < kTile ? P - pt * kTile : kTile; };
   auto fetch_states = [&](int h, int pt, int nt) {
-    const int64_t off = (int64_t(h) * P + pt * kTile) * NK + nt * 64;
-    sh.load(hrow, use_h ? width(pt) : 0, NK - nt * 64, off);
-    sd.load(drow, use_dh ? width(pt) : 0, NK - nt * 64, off);
+    const int64_t off = (int64_t(h) * P + pt * kTile) * NR + nt * 64;
+    sh.load(hrow, use_h ? width(pt) : 0, NK - nt * 64, off, NK);
+    sd.load(drow, use_dh ? width(pt) : 0, NK - nt * 64, off, NK);
   };
   // (one place in the code with no branch in it, or the compiler loads to other registers and
   // waits to move the values over; behind the last head nothing is loaded)
@@ -187,9 +206,9 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
     const int at = more ? h : h_lo, off = at * P + pt * kTile, w = more ? width(pt) : 0;
     sx.load(xrow, kQ, w, off);
     sy.load(yrow, kQ, w, off);
-    const int64_t soff = int64_t(off) * NK;
-    sh.load(hrow, use_h ? w : 0, NK, soff);
-    sd.load(drow, use_dh ? w : 0, NK, soff);
+    const int64_t soff = int64_t(off) * NR;
+    sh.load(hrow, use_h ? w : 0, NK, soff, NK);
+    sd.load(drow, use_dh ? w : 0, NK, soff, NK);
     const int64_t tok = (int64_t(at) * a.chunks + c.id) * kQ;
     sv = lane_of(a.s, tok, lane);
     uv = lane_of(a.u, tok, lane);
@@ -203,7 +222,7 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 #pragma unroll
   for (int k = 0; k < Q; ++k) gm[k] = ds[k] = zero4();
   if (LY::kInLds) {
-    Staged<DT, VEC, W, kBack> sb;
+    Staged<DT, VEC, WB, kBack> sb;
     sb.load(brow, kQ, N, 0);
     sb.put(bt);
     sb.load(crow, kQ, N, 0);
@@ -248,9 +267,14 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
       sy.put(yt);
       auto put_states = [&]() {
 #pragma unroll
-        for (int k = 0; k < sh.kLoads; ++k) za += dot<Acc>(sh.v[k], sd.v[k]);
-        sh.put_kept(ht);
-        sd.put_kept(dt);
+        for (int k = 0; k < sh.kLoads; ++k) {
+          float hv[8], dv[8];
+          sh.get(k, hv);
+          sd.get(k, dv);
+          za += dot<Acc>(hv, dv);
+        }
+        sh.put(ht);
+        sd.put(dt);
       };
       if (use_h || use_dh) put_states();
       __syncthreads();
@@ -307,11 +331,11 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
         if (!use_h && !use_dh) continue;
 #pragma unroll
         for (int ks = 0; ks < 2 * TW; ++ks) {
-          const Frag<NP> df = dt.get8(lw, wave, ks);
+          const Frag<MP> df = dt.get8(lw, wave, ks);
 #pragma unroll
           for (int k = 0; k < Q; ++k) {
             const int col = 64 * nt0 + 32 * ks + 8 * g;
-            const Frag<NP> bf = LY::kInLds ? bt.get8(lw, blk(k), ks)
+            const Frag<NP> bf = LY::kInLds ? bt.get8(lb, blk(k), 2 * nt0 + ks)
                                             : brow.get8(16 * blk(k) + li, col, N - col, 0).frag();
             xa[k] = mm(df, bf, xa[k]);
           }
@@ -320,17 +344,17 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
 #pragma unroll
         for (int tw = 0; tw < TW; ++tw) {
           const int nt = nt0 + tw, sc = 64 * nt + 16 * wave + 4 * g;
-          const Frag<NP> h0 = ht.tr8(lw, 0, 4 * tw + wave), h1 = ht.tr8(lw, 1, 4 * tw + wave);
+          const Frag<MP> h0 = ht.tr8(lw, 0, 4 * tw + wave), h1 = ht.tr8(lw, 1, 4 * tw + wave);
 #pragma unroll
           for (int k = 0; k < Q; ++k) {
             const f32x4 v = mm(h1, yt.get8(lx, blk(k), 1), mm(h0, yt.get8(lx, blk(k), 0), zero4()));
-            const f32x4 cv = LY::kInLds ? ct.get4(lw, blk(k), 4 * tw + wave)
+            const f32x4 cv = LY::kInLds ? ct.get4(lb, blk(k), 4 * nt + wave)
                                         : crow.get4(16 * blk(k) + li, sc, N - sc);
             dCa[nt][k] += dec.e[16 * blk(k) + li] * v;
 #pragma unroll
             for (int r = 0; r < 4; ++r) qa[k] += static_cast<Acc>(v[r]) * cv[r];
           }
-          const Frag<NP> d0 = dt.tr8(lw, 0, 4 * tw + wave), d1 = dt.tr8(lw, 1, 4 * tw + wave);
+          const Frag<MP> d0 = dt.tr8(lw, 0, 4 * tw + wave), d1 = dt.tr8(lw, 1, 4 * tw + wave);
 #pragma unroll
           for (int k = 0; k < Q; ++k) {
             const f32x4 v = mm(d1, xt.get8(lx, blk(k), 1), mm(d0, xt.get8(lx, blk(k), 0), zero4()));
@@ -416,9 +440,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
       }
     }
   }
-  // what the chunk's own tokens give of dB and dC, summed over the heads: once a workgroup,
-  // so that bf16 takes two planes of it (behind M's tile, where the states were)
-  const Tile<NP == 1 ? 2 : NP, 64> st{mt.p};
+  // what the chunk's own tokens give of dB and dC, summed over the heads, where M was
+  const Tile<MP, 64>& st = mt;
 #pragma unroll
   for (int k = 0; k < Q; ++k) st.put4(lx, wave, blk(k), ds[k]);
 #pragma unroll
@@ -499,7 +522,7 @@ struct Bytes {
 Bytes bytes_of(const Args& a) {
   Bytes r;
   r.walk = walk_bytes(a);
-  r.dh = up(size_t(a.chunks) * a.p.H * a.p.P * kept_cols(a.p.N) * (a.p.x_dt == DT_BF16 ? 2 : 4));
+  r.dh = up(size_t(a.chunks) * a.p.H * a.p.P * kept_cols(a.p.N) * 4);
   r.part = up(size_t(a.chunks) * 3 * a.p.H * 4);
   const int64_t s = subs_of(a);
   r.sub = s == 1 ? 0 : up(size_t(s) * a.p.seq.n_tokens * a.p.G * a.p.N * 4);

@@ -5,7 +5,12 @@ form themselves enters a product with at most 2^-16 of it lost, and sums are fp3
 result is off by its own rounding, whose norm is that of round(want) - want (about 2^-9.3 of
 the result's), and by what its factors lost: two of them, 2^-15 of the result, so that the
 norm of the whole is at most 1 + 2^-15 / 2^-9.3 = 1.02 times that of the rounding; 1.05 is
-asked for.  One rounding of one factor to bf16 (2^-9.3 of it) would make it 1.4."""
+asked for.  One rounding of one factor to bf16 (2^-9.3 of it) would make it 1.4.
+
+Gradients of fp32 parameters are sums of such products over tokens, of random sign, rounded
+in fp32 only: each product is off by at most 2^-15 of itself (two factors), and the sum of
+their errors grows as the sum itself does.  2^-11 of the norm over the heads, sixteen times as
+much, leaves room for heads whose sum happens to be small."""
 from __future__ import annotations
 
 import pytest
@@ -49,3 +54,26 @@ def test_outputs(lead, H, P, G, N):
     y, got_fin = moc.selective_scan(**{k: dev(v) for k, v in ins.items()}, cache=dev(init), output_final_state=True)
     assert off(y.flatten(0, 1), want) <= 1.05 * own_rounding(want, BF16)
     assert off(got_fin, fin) <= 2.0 ** -16 * fin.norm()
+
+
+@pytest.mark.parametrize("lead, H, P, G, N", SHAPES)
+def test_gradients(lead, H, P, G, N):
+    ins = slow_inputs(lead, H, P, G, N, F32)
+    init, dfin = rnd(lead[0], H, P, N, seed=20, scale=0.3), rnd(lead[0], H, P, N, seed=21)
+    dy = rnd(*lead, H, P, seed=50, dtype=BF16)
+    flat = {k: (v.flatten(0, 1) if v.ndim > 1 else v) for k, v in ins.items()}
+    u = O.step_lengths(flat["dt"], flat["dt_bias"], True)
+    seqs = O.spans(lead[0] * lead[1], lead[1], None)
+    _, (dx, du, dA, dB, dC, dD, dinit, _) = O.scan(flat["x"], u, flat["A"], flat["B"], flat["C"], flat["D"], seqs,
+                                                   init=init, dy=dy.flatten(0, 1), dfin=dfin)
+    ddt = du * O.sigmoid_of(u, True)
+    leaves = {k: dev(v).requires_grad_() for k, v in ins.items()}
+    cache = dev(init).requires_grad_()
+    y, fin = moc.selective_scan(**leaves, cache=cache, output_final_state=True)
+    names = ["x", "dt", "B", "C", "A", "D", "dt_bias"]
+    got = torch.autograd.grad([y, fin], [*(leaves[k] for k in names), cache], [dev(dy), dev(dfin)])
+    for name, g, want in zip(names, got[:4], (dx, ddt, dB, dC)):
+        assert off(g.flatten(0, 1), want) <= 1.05 * own_rounding(want, BF16), name
+    for name, g, want in zip(names[4:], got[4:], (dA, dD, ddt.sum(0))):
+        assert g.dtype == F32 and off(g, want) <= 2.0 ** -11 * want.norm(), name
+    assert off(got[7], dinit) <= 2.0 ** -16 * dinit.norm()
