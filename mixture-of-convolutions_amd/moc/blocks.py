@@ -12,6 +12,9 @@ sequence the decode step, in place on the cache and not differentiable.
 All run as hand-written HIP kernels of libmoc_hip.so, forward, backward and step;
 there is no fallback.  Calls go through the host module (csrc/moc_host.cpp) where they
 are ones that it takes; the Python functions below are the same calls for all others.
+Every launch below stands in an autograd function, also where no gradient is asked for, so
+that a tracer records it and an input with a tangent is refused (a launch by itself is seen
+by neither).
 """
 from __future__ import annotations
 
@@ -95,9 +98,10 @@ def _written(cache: torch.Tensor) -> None:
 
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = ops.launch_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+    def forward(ctx, x, weight, bias, eps, keep):
+        y, mean, rstd = ops.launch_norm_forward(x, weight, bias, eps, keep)
+        if keep:
+            ctx.save_for_backward(x, weight, bias, mean, rstd)
         return y
 
     @staticmethod
@@ -105,7 +109,8 @@ class _LayerNormFunction(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, mean, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*ops.launch_norm_backward(x, weight, bias, dy, mean, rstd, need[0], need[1], need[2]), None)
+        return (*ops.launch_norm_backward(x, weight, bias, dy, mean, rstd, need[0], need[1], need[2]),
+                None, None)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
@@ -124,9 +129,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
         if t is not None and tuple(t.shape) != (x.shape[-1],):
             raise ValueError(f"{name} must have shape {(x.shape[-1],)}, got {tuple(t.shape)}")
     x, weight, bias = x.contiguous(), _operand(weight), _operand(bias)
-    if _wants_grad(x, weight, bias):
-        return _LayerNormFunction.apply(x, weight, bias, float(eps))
-    return ops.launch_norm_forward(x, weight, bias, float(eps), False)[0]
+    return _LayerNormFunction.apply(x, weight, bias, float(eps), _wants_grad(x, weight, bias))
 
 
 class LayerNorm(nn.Module):
@@ -147,6 +150,8 @@ class LayerNorm(nn.Module):
 # causal convolution
 
 class _CausalConvFunction(torch.autograd.Function):
+    """Differentiable in x, weight and bias, without a cache."""
+
     @staticmethod
     def forward(ctx, x, weight, bias, act, cu_seqlens):
         y, _ = ops.launch_conv_forward(x, weight, bias, None, activation_flag=act, cu_seqlens=cu_seqlens)
@@ -163,10 +168,20 @@ class _CausalConvFunction(torch.autograd.Function):
                                           need_w=need[1], need_b=need[2], cu_seqlens=cu_seqlens), None, None)
 
 
-def _conv(x, weight, bias, act, cu_seqlens=None):
-    if _wants_grad(x, weight, bias):
-        return _CausalConvFunction.apply(x, weight, bias, act, cu_seqlens)
-    return ops.launch_conv_forward(x, weight, bias, None, activation_flag=act, cu_seqlens=cu_seqlens)[0]
+class _CausalConvPromptFunction(torch.autograd.Function):
+    """Returns (y, final state or None); applied where no gradient is asked for."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, cache, act, want_state):
+        return ops.launch_conv_forward(x, weight, bias, cache, activation_flag=act, final_state=want_state)
+
+
+class _CausalConvStepFunction(torch.autograd.Function):
+    """In place on the cache; applied without gradients."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, cache, act):
+        return ops.launch_conv_update(x, weight, bias, cache, activation_flag=act)
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -207,26 +222,27 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
         raise ValueError(f"kernel_size must be at most {_lib.CONV_MAX_KERNEL}, got {S}")
     x, weight, bias = x.contiguous(), _operand(weight), _operand(bias)
     if cu_seqlens is not None:
-        y = _conv(x, weight, bias, act, cu_seqlens.contiguous())
+        y = _CausalConvFunction.apply(x, weight, bias, act, cu_seqlens.contiguous())
         return (y[None] if restore else y), None
     B, T, _ = x.shape
     if cache is not None:
         _check_state(cache, (B, D, S), x.dtype, x, T == 1)
         if T == 1:
-            y = ops.launch_conv_update(x[:, 0], weight, bias, cache, activation_flag=act)
+            with torch.no_grad():
+                y = _CausalConvStepFunction.apply(x[:, 0], weight, bias, cache, act)
             _written(cache)
             return y[:, None], (cache if output_final_state else None)
     if _wants_grad(x, weight, bias, cache):
         if cache is None:
-            y = _conv(x, weight, bias, act)
+            y = _CausalConvFunction.apply(x, weight, bias, act, None)
         else:
             # the S - 1 newest cached inputs, then the tokens themselves
-            y = _conv(torch.cat((cache.transpose(1, 2)[:, 1:], x), 1), weight, bias, act)[:, S - 1:]
+            every = torch.cat((cache.transpose(1, 2)[:, 1:], x), 1)
+            y = _CausalConvFunction.apply(every, weight, bias, act, None)[:, S - 1:]
         return y, (_final_state(x, cache, S) if output_final_state else None)
     if cache is not None:
         cache = cache.contiguous()
-    return ops.launch_conv_forward(x, weight, bias, cache, activation_flag=act,
-                                   final_state=output_final_state)
+    return _CausalConvPromptFunction.apply(x, weight, bias, cache, act, bool(output_final_state))
 
 
 class CausalConv(nn.Module):
@@ -273,9 +289,11 @@ class _SelectiveScanFunction(torch.autograd.Function):
     """Returns (y, final state or None)."""
 
     @staticmethod
-    def forward(ctx, x, dt, A, B, C, D, dt_bias, cache, softplus, want_state, cu_seqlens):
+    def forward(ctx, x, dt, A, B, C, D, dt_bias, cache, softplus, want_state, cu_seqlens, keep):
         y, fin, saved = ops.launch_scan_forward(x, dt, A, B, C, D, dt_bias, cache, softplus=softplus,
-                                                final_state=want_state, keep=True, cu_seqlens=cu_seqlens)
+                                                final_state=want_state, keep=keep, cu_seqlens=cu_seqlens)
+        if not keep:
+            return y, fin
         ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, saved, cu_seqlens)
         ctx.softplus = softplus
         ctx.has_init = cache is not None
@@ -288,14 +306,26 @@ class _SelectiveScanFunction(torch.autograd.Function):
         *ins, saved, cu_seqlens = ctx.saved_tensors
         if dy is None:
             if dfin is None:
-                return (None,) * 11
+                return (None,) * 12
             dy = torch.zeros_like(ins[0])
         if dfin is not None:
             dfin = dfin.float().contiguous()
         grads = ops.launch_scan_backward(*ins, dy, dfin, saved, softplus=ctx.softplus,
                                          has_init=ctx.has_init, need_init=ctx.needs_input_grad[7],
                                          cu_seqlens=cu_seqlens)
-        return (*[g if need else None for g, need in zip(grads, ctx.needs_input_grad)], None, None, None)
+        return (*[g if need else None for g, need in zip(grads, ctx.needs_input_grad)], None, None, None, None)
+
+
+class _SelectiveScanStepFunction(torch.autograd.Function):
+    """In place on the cache; applied without gradients."""
+
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, dt_bias, cache, softplus):
+        state = cache.contiguous()
+        y = ops.launch_scan_update(x, dt, A, B, C, D, dt_bias, state, softplus=softplus)
+        if state is not cache:
+            cache.copy_(state)
+        return y
 
 
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
@@ -364,22 +394,14 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         step = tokens[1] == 1
         _check_state(cache, (tokens[0], H, P, N), torch.float32, x, step)
         if step:
-            state = cache.detach().contiguous()
-            y = ops.launch_scan_update(*(t if t is None else t.detach() for t in (x, dt, A, B, C, D, dt_bias)),
-                                       state, softplus=softplus)
-            if state.data_ptr() != cache.data_ptr():
-                with torch.no_grad():
-                    cache.copy_(state)
-            else:
-                _written(cache)
+            with torch.no_grad():
+                y = _SelectiveScanStepFunction.apply(x, dt, A, B, C, D, dt_bias, cache, softplus)
+            _written(cache)
             return y, (cache if output_final_state else None)
         cache = cache.contiguous()
     want = bool(output_final_state)
-    if _wants_grad(x, dt, A, B, C, D, dt_bias, cache):
-        y, fin = _SelectiveScanFunction.apply(x, dt, A, B, C, D, dt_bias, cache, softplus, want, cu_seqlens)
-    else:
-        y, fin, _ = ops.launch_scan_forward(x, dt, A, B, C, D, dt_bias, cache, softplus=softplus,
-                                            final_state=want, keep=False, cu_seqlens=cu_seqlens)
+    y, fin = _SelectiveScanFunction.apply(x, dt, A, B, C, D, dt_bias, cache, softplus, want, cu_seqlens,
+                                          _wants_grad(x, dt, A, B, C, D, dt_bias, cache))
     return (y[None] if restore else y), fin
 
 
