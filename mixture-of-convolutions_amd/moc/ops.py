@@ -672,6 +672,11 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape, dtype, device and type (a subclass's too)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def launch_norm_forward(x, weight, bias, eps: float, keep: bool):
     """(y, mean, rstd) of layer norm over the last axis of a contiguous x; mean and
     rstd are None unless ``keep``."""
@@ -819,9 +824,9 @@ def launch_scan_forward(x, dt, A, B, C, D, dt_bias, init, *, softplus: bool, fin
     L = _lib.lib()
     table, held = _scan_table(x, dt, A, B, C, D, dt_bias, softplus, cu_seqlens)
     ref = ctypes.byref(table)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     H, P, N = x.shape[-2], x.shape[-1], B.shape[-1]
-    fin = torch.empty(x.shape[0], H, P, N, dtype=torch.float32, device=x.device) if final_state else None
+    fin = x.new_empty(x.shape[0], H, P, N, dtype=torch.float32) if final_state else None
     with _lib.device_guard(x.device):
         saved = _workspace(_query(L.moc_scan_saved_bytes(ref), "moc_scan_forward"), x.device) if keep else None
         ws = _workspace(_query(L.moc_scan_forward_workspace_bytes(ref, int(keep)), "moc_scan_forward"),
@@ -841,11 +846,10 @@ def launch_scan_backward(x, dt, A, B, C, D, dt_bias, dy, dfinal, saved, *, softp
     table, held = _scan_table(x, dt, A, B, C, D, dt_bias, softplus, cu_seqlens)
     ref = ctypes.byref(table)
     dy = dy.to(x.dtype).contiguous()
-    like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-    outs = [like(t) for t in (x, dt, A, B, C, D, dt_bias)]
+    outs = [None if t is None else _dense_like(t) for t in (x, dt, A, B, C, D, dt_bias)]
     dinit = None
     if need_init:
-        dinit = torch.empty(x.shape[0], *x.shape[-2:], B.shape[-1], dtype=torch.float32, device=x.device)
+        dinit = x.new_empty(x.shape[0], *x.shape[-2:], B.shape[-1], dtype=torch.float32)
     grads = _lib.MocScanGrads(*[_ptr(t) for t in (*outs, dinit)])
     with _lib.device_guard(x.device):
         ws = _workspace(_query(L.moc_scan_backward_workspace_bytes(ref), "moc_scan_backward"), x.device)
@@ -861,7 +865,7 @@ def launch_scan_update(x, dt, A, B, C, D, dt_bias, state, *, softplus: bool) -> 
     """One token per sequence ([B, 1, ..] inputs), in place on the contiguous fp32
     ``state``."""
     table, held = _scan_table(x, dt, A, B, C, D, dt_bias, softplus, None)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     with _lib.device_guard(x.device):
         rc = _lib.lib().moc_scan_update(ctypes.byref(table), state.data_ptr(), y.data_ptr(),
                                         _lib.stream_ptr(x.device))
