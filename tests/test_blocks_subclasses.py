@@ -43,7 +43,8 @@ def test_subclasses_keep_their_type():
     ins = {k: dev(v) for k, v in scan_inputs((2, 20), 2, 16, 1, 8, BF16).items()}
     tag = lambda t: t.as_subclass(Tagged)  # noqa: E731
     H, s = _lib.host(), dict(ins)
-    assert H.norm(tag(x), w, b, 1e-5) is None and H.norm(x, tag(w), b, 1e-5) is None
+    assert H.norm(x, b, b, 1e-5) is not None
+    assert H.norm(tag(x), b, b, 1e-5) is None and H.norm(x, tag(b), b, 1e-5) is None
     assert H.conv(tag(x), w, b, None, 0, False, None) is None
     assert H.conv(x, w, tag(b), None, 0, False, None) is None
     assert H.scan(tag(s["x"]), s["dt"], s["A"], s["B"], s["C"], None, None, None, True, False, None) is None
@@ -54,7 +55,7 @@ def test_subclasses_keep_their_type():
             pairs = []
             for t, i in ((tag(x), dict(ins, x=tag(ins["x"]))), (x, ins)):
                 cc, sc = torch.zeros(2, 32, 4, dtype=BF16, device=DEV), torch.zeros(2, 2, 16, 8, device=DEV)
-                pairs.append((moc.layer_norm(t, w, b), moc.causal_conv(t, w, b, "silu")[0],
+                pairs.append((moc.layer_norm(t, b, b), moc.causal_conv(t, w, b, "silu")[0],
                               moc.causal_conv(t, w, cache=cc)[0], moc.causal_conv(t[:, :1], w, cache=cc)[0],
                               *moc.selective_scan(**i, output_final_state=True),
                               moc.selective_scan(**cut(i, 1), cache=sc)[0]))
