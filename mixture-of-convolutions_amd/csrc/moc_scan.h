@@ -103,9 +103,17 @@ __device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+// What the first of several planes of v is rounded from: values from 3.396e38 on, finite but
+// an infinity in bf16, take bf16's largest, and the next plane the rest (so does an infinity:
+// its second plane is the infinity).
+__device__ __forceinline__ float below_top(float v) {
+  constexpr float kTop = 0x1.fep127f;
+  return __builtin_amdgcn_fmed3f(v, -kTop, kTop);
+}
+
 // Planes of 8 fp32 values: each plane is what the ones before it left, rounded to bf16
 // (the differences are exact; those of an infinity are NaN, so what an infinity enters
-// comes out as NaN where there are several planes).
+// comes out as NaN where there are three planes).
 template <int NP>
 __device__ __forceinline__ Frag<NP> split(const float (&f)[8]) {
   u32x4 w[NP];
@@ -114,7 +122,7 @@ __device__ __forceinline__ Frag<NP> split(const float (&f)[8]) {
     float a = f[2 * k], b = f[2 * k + 1];
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const uint32_t v = pack2(a, b);
+      const uint32_t v = p == 0 && NP > 1 ? pack2(below_top(a), below_top(b)) : pack2(a, b);
       w[p][k] = v;
       if (p + 1 < NP) a -= lo_f(v), b -= hi_f(v);
     }
@@ -123,6 +131,19 @@ __device__ __forceinline__ Frag<NP> split(const float (&f)[8]) {
 #pragma unroll
   for (int p = 0; p < NP; ++p) r.v[p] = __builtin_bit_cast(s16x8, w[p]);
   return r;
+}
+
+// 4 fp32 values in planes `apart` elements from each other
+template <int NP>
+__device__ __forceinline__ void put_planes(uint16_t* q, int apart, f32x4 v) {
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    f32x4 c = v;
+    if (k == 0 && NP > 1) c = f32x4{below_top(v[0]), below_top(v[1]), below_top(v[2]), below_top(v[3])};
+    const u32x2 w{pack2(c[0], c[1]), pack2(c[2], c[3])};
+    *reinterpret_cast<u32x2*>(q + k * apart) = w;
+    if (k + 1 < NP) v -= f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
+  }
 }
 
 template <int NP>
@@ -454,12 +475,7 @@ struct Tile {
   // row 16 rb + li, columns 16 cb + 4 g..: 4 fp32 values split over the planes
   __device__ __forceinline__ void put4(const Lane<W>& l, int rb, int cb, f32x4 v) const {
     uint16_t* q = p + (l.quad ^ (16 * cb)) + 16 * rb * W;
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
-      *reinterpret_cast<u32x2*>(q + k * kPlane) = w;
-      if (k + 1 < NP) v -= f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
-    }
+    put_planes<NP>(q, kPlane, v);
   }
   __device__ __forceinline__ f32x4 get4(const Lane<W>& l, int rb, int cb) const {
     const uint16_t* q = p + (l.quad ^ (16 * cb)) + 16 * rb * W;
@@ -511,12 +527,7 @@ struct Lower {
   // row 16 ib + li, columns 16 jb + 4 g..
   __device__ __forceinline__ void put4(int li, int g, int ib, int jb, f32x4 v) const {
     uint16_t* q = p + block(ib, jb) + 16 * li + 4 * g;
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      const u32x2 w{pack2(v[0], v[1]), pack2(v[2], v[3])};
-      *reinterpret_cast<u32x2*>(q + k * kPlane) = w;
-      if (k + 1 < NP) v -= f32x4{lo_f(w[0]), hi_f(w[0]), lo_f(w[1]), hi_f(w[1])};
-    }
+    put_planes<NP>(q, kPlane, v);
   }
   // row 16 ib + li, columns 32 ks + 8 g.. (2 ks <= ib; 0 right of the diagonal's block)
   __device__ __forceinline__ Frag<NP> get8(int li, int g, int ib, int ks) const {

@@ -448,7 +448,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if ((xf[ks].v[0][e] & 0x7f80) == 0x7f80)
+            if ((xf[ks].v[NP - 1][e] & 0x7f80) == 0x7f80)  // (of the last plane: see below_top)
 #pragma unroll
               for (int q = 0; q < NP; ++q) xm[ks].v[q][e] = 0;
       }
