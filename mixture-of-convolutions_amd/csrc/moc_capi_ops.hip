@@ -263,6 +263,8 @@ int moc_scan_backward(const MocScan* s, const void* dy, int has_initial_state, c
   if (!dy || !saved || !grads || !grads->dx || !grads->ddt || !grads->da || !grads->db || !grads->dc)
     return fail(MOC_ERR_ARG, "null tensor pointer");
   if (int rc = check_states(s, dfinal_state, grads->dinitial_state)) return rc;
+  if (has_initial_state != 0 && s->cu_seqlens != nullptr)
+    return fail(MOC_ERR_ARG, "states are only supported for fixed-length inputs");
   const moc::Scan p = problem(s);
   if (int rc = check_space(moc::scan_saved_bytes(p), saved, saved_bytes)) return rc;
   if (int rc = check_space(moc::scan_backward_workspace(p), workspace, workspace_bytes)) return rc;
