@@ -689,6 +689,12 @@ __device__ __forceinline__ float lane_of(const float* a, int64_t at, int lane) {
 // one sequence are consecutive, those of two never meet (a sequence of n tokens has
 // ceil(n / kQ) chunks, and floor((e + n) / kQ) + 1 >= floor(e / kQ) + ceil(n / kQ)), and
 // no table has to be made on the device.  Segments (a multiple of kQ tokens) likewise.
+//
+// States are kept under numbers of their own, which do not grow with the sequences.  What
+// enters piece k of a sequence that began without a state has the slot floor(edge / q) + k - 1
+// (k >= 1; in reverse floor(edge / q) + k, k before the last): ceil(n / q) - 1 of them a
+// sequence, and floor((e + n) / q) >= floor(e / q) + ceil(n / q) - 1, so that they are
+// distinct and below floor(n_tokens / q).
 struct Seqs {
   SeqLayout l;
   int64_t count;
@@ -720,6 +726,10 @@ struct Seqs {
     return k >= 0 && edge(a) + k * q < edge(a + 1);
   }
 };
+// what piece k's slot is
+__device__ __forceinline__ int64_t slot_of(const Seqs& s, int64_t m, int64_t k, int64_t q, bool rev) {
+  return s.edge(m) / q + k - (rev ? 0 : 1);
+}
 inline int64_t pieces(const Seqs& s, int64_t q) {
   return s.l.cu == nullptr ? s.count * ((s.l.seq_len + q - 1) / q) : s.l.n_tokens / q + s.count;
 }
@@ -739,14 +749,23 @@ struct Args {
 // Chunk `id`: false where there is none.
 struct Chunk {
   int64_t m, t0, id;
+  int64_t h, dh;   // places of the kept state before it and of the gradient behind it
   int n;           // tokens
   bool first, last;
 };
+// The same of any chunk.  A fixed-length sequence may begin and end with a state, so its chunks
+// keep one each, under their own numbers.
+__device__ __forceinline__ int64_t kept_at(const Args& a, int64_t m, int64_t k, int64_t id, bool rev) {
+  return a.seqs.l.cu == nullptr ? id : slot_of(a.seqs, m, k, kQ, rev);
+}
+inline int64_t kept_states(const Args& a) { return a.seqs.l.cu == nullptr ? a.chunks : a.p.seq.n_tokens / kQ; }
 __device__ __forceinline__ bool chunk_at(const Args& a, int64_t id, Chunk& c) {
   int64_t k;
   if (!a.seqs.find(id, kQ, c.m, k)) return false;
   const int64_t lo = a.seqs.edge(c.m), hi = a.seqs.edge(c.m + 1);
   c.id = id;
+  c.h = kept_at(a, c.m, k, id, false);
+  c.dh = kept_at(a, c.m, k, id, true);
   c.t0 = lo + k * kQ;
   c.n = static_cast<int>(hi - c.t0 < kQ ? hi - c.t0 : kQ);
   c.first = k == 0;
@@ -778,9 +797,9 @@ struct Walk {
   int64_t x_stride, b_stride;
   const float* start;   // [sequences][H][P][N] or null: state at the walk's start
   float* end;           // the same or null: state at its end
-  float* seg_state;     // [segments][H][P][N]: state at each segment's start
-  double* seg_decay;    // [segments][H]: log2 of a segment's decay
-  void* kept;           // [chunks][H][P] rows of kept states or null: state before each chunk
+  float* seg_state;     // [n_tokens / seg][H][P][N]: state that enters each segment but a first one
+  double* seg_decay;    // [n_tokens / seg][H]: log2 of the decay of the segment before it
+  void* kept;           // [kept_states][H][P] rows of kept states or null: state before each chunk
 };
 size_t walk_bytes(const Args& a);   // seg_state and seg_decay
 void carve_walk(const Args& a, void* workspace, Walk& w);

@@ -104,11 +104,11 @@ __device__ __forceinline__ void store_state(const Rows<DT, VEC>& dst, int row, c
   for (int nb = 0; nb < NB; ++nb) dst.put4(row, 16 * nb + n0, acc[nb]);
 }
 
-// The kept states of one head's channels from p0 on, `cols` of them, of chunk `id`.
+// The kept states of one head's channels from p0 on, `cols` of them, at place `at`.
 template <int DT, int VEC>
-__device__ __forceinline__ Rows<DT, VEC> kept_rows(const Args& a, void* kept, int64_t id, int h, int p0, int cols, int NK) {
+__device__ __forceinline__ Rows<DT, VEC> kept_rows(const Args& a, void* kept, int64_t at, int h, int p0, int cols, int NK) {
   const int row = kKeptPlanes<DT> * NK;
-  return Rows<DT, VEC>(kept, ((id * a.p.H + h) * a.p.P + p0) * row, row, cols, row);
+  return Rows<DT, VEC>(kept, ((at * a.p.H + h) * a.p.P + p0) * row, row, cols, row);
 }
 // acc to a row of them
 template <int NB, int DT, int VEC>
@@ -163,9 +163,12 @@ __device__ __forceinline__ void update_state(const Tile<NP, W>& bt, const Lane<W
 // The segment of a walk's workgroup.
 struct Segment {
   int64_t m, t0, c0;   // sequence, first token, first chunk
+  int64_t kept;        // place of its first chunk's kept state (in reverse: gradient)
+  int64_t enters;      // slot of the state that enters it (in reverse: from behind)
   int n, chunks;       // tokens, chunks
   bool first, last;    // of its sequence
 };
+template <bool REV>
 __device__ __forceinline__ bool segment_at(const Args& a, int64_t id, Segment& s) {
   int64_t j;
   if (!a.seqs.find(id, a.seg, s.m, j)) return false;
@@ -173,7 +176,10 @@ __device__ __forceinline__ bool segment_at(const Args& a, int64_t id, Segment& s
   s.t0 = lo + j * a.seg;
   s.n = static_cast<int>(hi - s.t0 < a.seg ? hi - s.t0 : a.seg);
   s.chunks = (s.n + kQ - 1) / kQ;
-  s.c0 = a.seqs.base(s.m, kQ) + j * (a.seg / kQ);
+  const int64_t k = j * (a.seg / kQ);
+  s.c0 = a.seqs.base(s.m, kQ) + k;
+  s.kept = kept_at(a, s.m, k, s.c0, REV);
+  s.enters = slot_of(a.seqs, s.m, j, a.seg, REV);
   s.first = j == 0;
   s.last = s.t0 + s.n == hi;
   return true;
@@ -192,8 +198,8 @@ constexpr int kForwardLds =
     Decays::kBytes + 16;
 
 // The state over one segment's chunks, forwards (REV false) or backwards.  LOCAL: from
-// zero, for segments that another one follows, to seg_state and seg_decay; else from the
-// state that enters the segment, kept before each chunk.
+// zero, for segments that another one follows, to that one's seg_state and seg_decay; else from
+// the state that enters the segment, kept before each chunk.
 template <int DT, int NT, int VEC, bool REV, bool LOCAL>
 __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 : (NT == 2 ? 3 : 2))) void state_walk(Args a, Walk w) {
   constexpr int NP = kPlanes<DT>, NB = 4 * NT, W = 64 * NT;
@@ -208,7 +214,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 :
   const int ptiles = (P + kTile - 1) / kTile;
   const int h = blockIdx.y / ptiles, p0 = (blockIdx.y % ptiles) * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
   Segment s;
-  if (!segment_at(a, blockIdx.x, s)) return;
+  if (!segment_at<REV>(a, blockIdx.x, s)) return;
   const bool at_start = REV ? s.last : s.first, at_end = REV ? s.first : s.last;
   if (LOCAL && at_end) return;
   const int row = 16 * wave + (lane & 15);  // this lane's channel, from p0 on
@@ -220,7 +226,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 :
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float* from = LOCAL ? nullptr : (at_start ? w.start : w.seg_state);
-  if (from != nullptr) load_state<NB>(state(from, at_start ? s.m : int64_t(blockIdx.x)), row, acc);
+  if (from != nullptr) load_state<NB>(state(from, at_start ? s.m : s.enters), row, acc);
   const int64_t at = (int64_t(h) * a.chunks + s.c0) * kQ;
   const int64_t xcol = int64_t(h) * P + p0, bcol = int64_t(h / (a.p.H / a.p.G)) * N;
   Staged<DT, VEC, 64, kThreads> sx;
@@ -242,7 +248,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 :
     lw.refresh(), lx.refresh();
     const int i = REV ? s.chunks - 1 - k : k;
     if (!LOCAL && w.kept != nullptr && !(k == 0 && from == nullptr))
-      keep_state<NB>(kept_rows<DT, VEC>(a, w.kept, s.c0 + i, h, p0, cols, NK), row, NK, acc);
+      keep_state<NB>(kept_rows<DT, VEC>(a, w.kept, s.kept + i, h, p0, cols, NK), row, NK, acc);
     sx.put(xt);
     sb.put(bt);
     const double last = __shfl(sv, 63);
@@ -261,15 +267,16 @@ __global__ __launch_bounds__(kThreads, waves_for(kWalkLds<DT, NT>, NT == 1 ? 4 :
     __syncthreads();
   }
   if (LOCAL) {
-    store_state<NB>(state(w.seg_state, blockIdx.x), row, acc);
-    if (threadIdx.x == 0 && p0 == 0) w.seg_decay[int64_t(blockIdx.x) * a.p.H + h] = total;
+    const int64_t next = REV ? s.enters - 1 : s.enters + 1;
+    store_state<NB>(state(w.seg_state, next), row, acc);
+    if (threadIdx.x == 0 && p0 == 0) w.seg_decay[next * a.p.H + h] = total;
   } else if (at_end && w.end != nullptr) {
     store_state<NB>(state(w.end, s.m), row, acc);
   }
 }
 
-// seg_state: from each segment's own state to the state that enters it, one element a
-// thread.  Bound by memory (24 segments of 32 heads, 64 x 128: 50 MB in 13 us).
+// seg_state: from what the segment before leaves by itself to the state that enters, one
+// element a thread.  Bound by memory (24 segments of 32 heads, 64 x 128: 50 MB in 13 us).
 template <bool REV>
 __global__ __launch_bounds__(kThreads) void join_segments(Args a, Walk w) {
   const int64_t pn = a.p.P * a.p.N, per = a.p.H * pn;
@@ -279,18 +286,13 @@ __global__ __launch_bounds__(kThreads) void join_segments(Args a, Walk w) {
   for (int64_t m = blockIdx.y; m < a.seqs.count; m += gridDim.y) {
     const int64_t n = (a.seqs.edge(m + 1) - a.seqs.edge(m) + a.seg - 1) / a.seg;
     if (n <= 1) continue;
-    const int64_t s0 = a.seqs.base(m, a.seg);
+    const int64_t s0 = a.seqs.edge(m) / a.seg;
     float cur = w.start == nullptr ? 0.f : w.start[m * per + e];
-    for (int64_t k = 0; k < n; ++k) {
-      const int64_t id = s0 + (REV ? n - 1 - k : k);
-      if (k + 1 < n) {
-        const float own = w.seg_state[id * per + e];
-        const float decay = __builtin_amdgcn_exp2f(static_cast<float>(w.seg_decay[id * a.p.H + h]));
-        w.seg_state[id * per + e] = cur;
-        cur = decay * cur + own;
-      } else {
-        w.seg_state[id * per + e] = cur;
-      }
+    for (int64_t k = 0; k + 1 < n; ++k) {
+      const int64_t at = s0 + (REV ? n - 2 - k : k);
+      const float decay = __builtin_amdgcn_exp2f(static_cast<float>(w.seg_decay[at * a.p.H + h]));
+      cur = decay * cur + w.seg_state[at * per + e];
+      w.seg_state[at * per + e] = cur;
     }
   }
 }
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
   const int ptiles = (P + kTile - 1) / kTile;
   const int h = blockIdx.y / ptiles, p0 = (blockIdx.y % ptiles) * kTile, cols = P - p0 < kTile ? P - p0 : kTile;
   Segment s;
-  if (!segment_at(a, blockIdx.x, s)) return;
+  if (!segment_at<false>(a, blockIdx.x, s)) return;
   const int row = 16 * wave + li;  // this lane's channel of the state, from p0 on
   const bool active = 16 * wave < cols;
   const float skip = a.p.D == nullptr ? 0.f : load_any(a.p.D, a.p.d_dt, h);
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float* from = s.first ? w.start : w.seg_state;
-  if (from != nullptr) load_state<NB>(state(from, s.first ? s.m : int64_t(blockIdx.x)), row, acc);
+  if (from != nullptr) load_state<NB>(state(from, s.first ? s.m : s.enters), row, acc);
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   const int64_t at = (int64_t(h) * a.chunks + s.c0) * kQ;
   const int64_t xcol = int64_t(h) * P + p0, bcol = int64_t(h / (a.p.H / a.p.G)) * N;
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
     else if (wave == 2) m_blocks(Int<8>{}, Int<9>{}, Int<10>{});
     else m_blocks(Int<13>{}, Int<14>{}, Int<15>{});
     if (w.kept != nullptr && !(k == 0 && from == nullptr))
-      keep_state<NB>(kept_rows<DT, VEC>(a, w.kept, s.c0 + k, h, p0, cols, NK), row, NK, acc);
+      keep_state<NB>(kept_rows<DT, VEC>(a, w.kept, s.kept + k, h, p0, cols, NK), row, NK, acc);
     if (k + 1 < s.chunks) fetch(k + 1);
     f32x4 ya[4];
 #pragma unroll
@@ -664,13 +666,13 @@ void launch_prep(const Args& a, hipStream_t st) {
 
 size_t walk_bytes(const Args& a) {
   if (!segmented(a)) return 0;
-  const size_t n = size_t(pieces(a.seqs, a.seg)) * a.p.H;
+  const size_t n = size_t(a.p.seq.n_tokens / a.seg) * a.p.H;
   return up(n * a.p.P * a.p.N * 4) + up(n * 8);
 }
 
 void carve_walk(const Args& a, void* workspace, Walk& w) {
   if (!segmented(a)) return;
-  const size_t n = size_t(pieces(a.seqs, a.seg)) * a.p.H;
+  const size_t n = size_t(a.p.seq.n_tokens / a.seg) * a.p.H;
   w.seg_state = static_cast<float*>(workspace);
   w.seg_decay = reinterpret_cast<double*>(static_cast<char*>(workspace) + up(n * a.p.P * a.p.N * 4));
 }
@@ -697,7 +699,7 @@ using namespace scan;
 
 size_t scan_saved_bytes(const Scan& p) {
   const Args a = make_args(p, nullptr);
-  return prep_bytes(p) + size_t(a.chunks) * p.H * p.P * kept_cols(p.N) * 4;
+  return prep_bytes(p) + size_t(kept_states(a)) * p.H * p.P * kept_cols(p.N) * 4;
 }
 
 size_t scan_forward_workspace(const Scan& p, bool saved) {

@@ -39,7 +39,7 @@ constexpr int kThreads = 256;
 
 struct Back {
   const void* dy;       // [tokens][H][P] contiguous
-  const void* h;        // [chunks][H][P] rows of kept states: state before each chunk
+  const void* h;        // [kept_states][H][P] rows of kept states: state before each chunk
   const void* dh;       // the same: gradient of the state behind each chunk
   bool has_init, has_dfin;
   void *dx, *ddt, *dB, *dC;
@@ -184,8 +184,8 @@ __global__ __launch_bounds__(kBack, (Layout<DT, NT>::kWaves)) void backward_chun
   const Span<DT, VEC> xrow(a.p.x, c.t0 * a.p.x_stride, a.p.x_stride, n);
   const Span<DT, VEC> yrow(b.dy, c.t0 * H * P, int64_t(H) * P, n);
   const Span<DT, VEC> orow(b.dx, c.t0 * H * P, int64_t(H) * P, n);
-  const Span<DT, VEC> hrow(b.h, c.id * H * P * NR, NR, int64_t(H) * P);
-  const Span<DT, VEC> drow(b.dh, c.id * H * P * NR, NR, int64_t(H) * P);
+  const Span<DT, VEC> hrow(b.h, c.h * H * P * NR, NR, int64_t(H) * P);
+  const Span<DT, VEC> drow(b.dh, c.dh * H * P * NR, NR, int64_t(H) * P);
   auto blk = [&](int k) { return k * kHalves + half; };  // this wave's column blocks
 
   // the loads of a head's (and channel tile's) tensors, ahead of their use
@@ -522,7 +522,7 @@ struct Bytes {
 Bytes bytes_of(const Args& a) {
   Bytes r;
   r.walk = walk_bytes(a);
-  r.dh = up(size_t(a.chunks) * a.p.H * a.p.P * kept_cols(a.p.N) * 4);
+  r.dh = up(size_t(kept_states(a)) * a.p.H * a.p.P * kept_cols(a.p.N) * 4);
   r.part = up(size_t(a.chunks) * 3 * a.p.H * 4);
   const int64_t s = subs_of(a);
   r.sub = s == 1 ? 0 : up(size_t(s) * a.p.seq.n_tokens * a.p.G * a.p.N * 4);
