@@ -16,7 +16,9 @@ bool x_dt_ok(int dt) { return dt == MOC_DT_F32 || dt == MOC_DT_BF16; }
 
 constexpr int64_t kMaxTokens = int64_t(1) << 31;
 constexpr int64_t kMaxStride = int64_t(1) << 31;  // elements between tokens
-constexpr int64_t kMaxWorkgroups = int64_t(1) << 24;  // of 256 threads: a grid counts threads in 32 bits
+// a grid counts threads in 32 bits: workgroups of 256 threads, and chunks of a scan that is
+// differentiated, whose backward has workgroups of 512
+constexpr int64_t kMaxWorkgroups = int64_t(1) << 24, kMaxSavedChunks = int64_t(1) << 23;
 
 int launched(const char* what) {
   const hipError_t e = hipGetLastError();
@@ -74,7 +76,8 @@ int check_conv(int64_t dim, int64_t ks, int x_dt, int w_dt, int b_dt, int activa
 }
 
 // ---------------------------------------------------------------------------
-int check_scan(const MocScan* s, bool step) {
+enum class Use { kStep, kForward, kSaved };  // (kSaved: the forward for a backward, and that)
+int check_scan(const MocScan* s, Use use) {
   if (s == nullptr) return fail(MOC_ERR_ARG, "null scan");
   if (!s->x || !s->dt || !s->a || !s->b || !s->c) return fail(MOC_ERR_ARG, "null tensor pointer");
   if (s->heads <= 0 || s->head_dim <= 0 || s->groups <= 0 || s->state_dim <= 0 || s->heads % s->groups != 0)
@@ -97,11 +100,11 @@ int check_scan(const MocScan* s, bool step) {
                           s->c_stride >= kMaxStride))
     return fail(MOC_ERR_ARG, "token strides must be below 2^31 elements");
   if (int rc = check_seq(s->cu_seqlens, s->n_seqs, s->n_tokens, s->seq_len)) return rc;
-  if (step) {
+  if (use == Use::kStep) {
     if (s->cu_seqlens != nullptr || s->seq_len != 1) return fail(MOC_ERR_ARG, "a step has one token per sequence");
     if (s->n_tokens * s->heads >= kMaxWorkgroups) return fail(MOC_ERR_ARG, "too many sequences and heads for a step");
   } else if (s->n_tokens / 64 + (s->cu_seqlens != nullptr ? s->n_seqs + 2 : s->n_tokens / s->seq_len) >=
-             kMaxWorkgroups) {
+             (use == Use::kSaved ? kMaxSavedChunks : kMaxWorkgroups)) {
     return fail(MOC_ERR_ARG, "too many chunks of 64 tokens");
   }
   return MOC_OK;
@@ -228,18 +231,20 @@ int moc_conv_update(const void* x, const void* weight, const void* bias, void* c
 
 size_t moc_scan_saved_bytes(const MocScan* s) {
   clear_error();
-  return check_scan(s, false) != MOC_OK ? 0 : moc::scan_saved_bytes(problem(s));
+  return check_scan(s, Use::kSaved) != MOC_OK ? 0 : moc::scan_saved_bytes(problem(s));
 }
 
 size_t moc_scan_forward_workspace_bytes(const MocScan* s, int with_saved) {
   clear_error();
-  return check_scan(s, false) != MOC_OK ? 0 : moc::scan_forward_workspace(problem(s), with_saved != 0);
+  return check_scan(s, with_saved != 0 ? Use::kSaved : Use::kForward) != MOC_OK
+             ? 0
+             : moc::scan_forward_workspace(problem(s), with_saved != 0);
 }
 
 int moc_scan_forward(const MocScan* s, void* y, const float* initial_state, float* final_state, void* saved,
                      size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
-  if (int rc = check_scan(s, false)) return rc;
+  if (int rc = check_scan(s, saved != nullptr ? Use::kSaved : Use::kForward)) return rc;
   if (!y) return fail(MOC_ERR_ARG, "null tensor pointer");
   if (int rc = check_states(s, initial_state, final_state)) return rc;
   const moc::Scan p = problem(s);
@@ -252,14 +257,14 @@ int moc_scan_forward(const MocScan* s, void* y, const float* initial_state, floa
 
 size_t moc_scan_backward_workspace_bytes(const MocScan* s) {
   clear_error();
-  return check_scan(s, false) != MOC_OK ? 0 : moc::scan_backward_workspace(problem(s));
+  return check_scan(s, Use::kSaved) != MOC_OK ? 0 : moc::scan_backward_workspace(problem(s));
 }
 
 int moc_scan_backward(const MocScan* s, const void* dy, int has_initial_state, const float* dfinal_state,
                       const void* saved, size_t saved_bytes, const MocScanGrads* grads, void* workspace,
                       size_t workspace_bytes, void* stream) {
   clear_error();
-  if (int rc = check_scan(s, false)) return rc;
+  if (int rc = check_scan(s, Use::kSaved)) return rc;
   if (!dy || !saved || !grads || !grads->dx || !grads->ddt || !grads->da || !grads->db || !grads->dc)
     return fail(MOC_ERR_ARG, "null tensor pointer");
   if (int rc = check_states(s, dfinal_state, grads->dinitial_state)) return rc;
@@ -277,7 +282,7 @@ int moc_scan_backward(const MocScan* s, const void* dy, int has_initial_state, c
 
 int moc_scan_update(const MocScan* s, float* state, void* y, void* stream) {
   clear_error();
-  if (int rc = check_scan(s, true)) return rc;
+  if (int rc = check_scan(s, Use::kStep)) return rc;
   if (!state || !y) return fail(MOC_ERR_ARG, "null tensor pointer");
   moc::scan_update(problem(s), state, y, s->n_tokens, static_cast<hipStream_t>(stream));
   return launched("moc_scan_update launch");

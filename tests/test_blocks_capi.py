@@ -15,3 +15,24 @@ def test_a_packed_scan_has_no_initial_state():
     grads = _lib.MocScanGrads(*[FAKE] * 7, None)
     assert L.moc_scan_backward(ref, FAKE, 1, None, FAKE, 1 << 40, ctypes.byref(grads), FAKE, 0, None) == ERR_ARG
     assert b"fixed-length" in L.moc_last_error()
+
+
+def test_chunks_of_a_differentiated_scan_fit_a_grid():
+    """The backward's workgroups have 512 threads, and a grid counts threads in 32 bits: 2^23 chunks are
+    refused before anything is launched, by the forward that would keep states for it too."""
+    L = _lib.lib()
+    small = dict(heads=1, head_dim=1, groups=1, state_dim=1, x_stride=1, dt_stride=1, b_stride=1, c_stride=1)
+    fits = ctypes.byref(_table(**small, n_tokens=64, seq_len=64))
+    grads = _lib.MocScanGrads(*[FAKE] * 7, None)
+    ERR_WORKSPACE = -3
+    for kw in (dict(n_tokens=(1 << 22) + (1 << 23), seq_len=1),              # a chunk a token
+               dict(n_tokens=1 << 29, seq_len=1 << 29),                      # 2^23 chunks of 64
+               dict(n_tokens=1 << 20, cu_seqlens=FAKE, n_seqs=1 << 23, seq_len=0)):
+        ref = ctypes.byref(_table(**small, **kw))
+        assert L.moc_scan_saved_bytes(ref) == 0 and L.moc_scan_backward_workspace_bytes(ref) == 0
+        assert L.moc_scan_forward_workspace_bytes(ref, 1) == 0 and L.moc_scan_forward_workspace_bytes(ref, 0) > 0
+        assert L.moc_scan_forward(ref, FAKE, None, None, FAKE, 1 << 50, FAKE, 0, None) == ERR_ARG
+        assert L.moc_scan_backward(ref, FAKE, 0, None, FAKE, 1 << 50, ctypes.byref(grads), FAKE, 0, None) == ERR_ARG
+        assert b"too many chunks" in L.moc_last_error()
+        assert L.moc_scan_forward(ref, FAKE, None, None, None, 0, FAKE, 0, None) == ERR_WORKSPACE  # (past the checks)
+    assert L.moc_scan_backward(fits, FAKE, 0, None, FAKE, 1 << 50, ctypes.byref(grads), FAKE, 0, None) == ERR_WORKSPACE
