@@ -347,26 +347,30 @@ int64_t parts(int64_t rows) { return rows < kParts ? rows : kParts; }
 __global__ __launch_bounds__(1024) void column_sums(ColumnSums a) {
   __shared__ float s[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
-  const int64_t cols = a.n0 + a.n1 + a.n2, c = int64_t(blockIdx.x) * 32 + cx;
-  float v = 0.f;
-  if (c < cols) {
+  const int64_t cols = a.n0 + a.n1 + a.n2;
+  for (int64_t c0 = int64_t(blockIdx.x) * 32; c0 < cols; c0 += int64_t(gridDim.x) * 32) {
+    const int64_t c = c0 + cx;
+    float v = 0.f;
+    if (c < cols) {
 #pragma unroll 4
-    for (int64_t r = ry; r < a.n; r += 32) v += a.part[r * cols + c];
-  }
-  s[ry][cx] = v;
-  __syncthreads();
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    if (ry < m) s[ry][cx] += s[ry + m][cx];
+      for (int64_t r = ry; r < a.n; r += 32) v += a.part[r * cols + c];
+    }
+    __syncthreads();  // (the last columns have been read)
+    s[ry][cx] = v;
     __syncthreads();
-  }
-  if (ry != 0 || c >= cols) return;
-  if (c < a.n0) {
-    if (a.out0 != nullptr) store_any(a.out0, a.dt0, c, s[0][cx]);
-  } else if (c < a.n0 + a.n1) {
-    if (a.out1 != nullptr) store_any(a.out1, a.dt1, c - a.n0, s[0][cx]);
-  } else if (a.out2 != nullptr) {
-    store_any(a.out2, a.dt2, c - a.n0 - a.n1, s[0][cx]);
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+      if (ry < m) s[ry][cx] += s[ry + m][cx];
+      __syncthreads();
+    }
+    if (ry != 0 || c >= cols) continue;
+    if (c < a.n0) {
+      if (a.out0 != nullptr) store_any(a.out0, a.dt0, c, s[0][cx]);
+    } else if (c < a.n0 + a.n1) {
+      if (a.out1 != nullptr) store_any(a.out1, a.dt1, c - a.n0, s[0][cx]);
+    } else if (a.out2 != nullptr) {
+      store_any(a.out2, a.dt2, c - a.n0 - a.n1, s[0][cx]);
+    }
   }
 }
 
@@ -374,7 +378,8 @@ __global__ __launch_bounds__(1024) void column_sums(ColumnSums a) {
 
 void launch_column_sums(const ColumnSums& c, hipStream_t st) {
   const int64_t cols = c.n0 + c.n1 + c.n2;
-  hipLaunchKernelGGL(column_sums, dim3(static_cast<unsigned>((cols + 31) / 32)), dim3(1024), 0, st, c);
+  // (a grid counts threads in 32 bits: 2^27 columns would pass it)
+  hipLaunchKernelGGL(column_sums, dim3(grid((cols + 31) / 32, 1 << 16)), dim3(1024), 0, st, c);
 }
 
 size_t norm_backward_workspace(int64_t rows, int64_t D) { return size_t(parts(rows)) * 2 * D * sizeof(float); }
