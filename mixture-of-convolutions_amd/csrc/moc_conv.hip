@@ -131,11 +131,8 @@ __global__ __launch_bounds__(64 * kWaves) void conv_fwd(ConvArgs a) {
   }
 }
 
-template <int DT, int S, int V>
+template <int DT, int S, int V, int AHEAD>
 __global__ __launch_bounds__(64 * kWaves) void conv_bwd(ConvArgs a) {
-  // rows loaded together: S of them bring the windows' registers round without a move (4
-  // taps: 62 us with two rows, 56 with four; 3 taps: 24 with two, 29 with four)
-  constexpr int kAheadBack = S == 3 || S == 4 ? S : 2;
   __shared__ float lds[kWaves - 1][64 * V];
   const int64_t c = (int64_t(blockIdx.x) * 64 + (threadIdx.x & 63)) * V;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -226,15 +223,15 @@ __global__ __launch_bounds__(64 * kWaves) void conv_bwd(ConvArgs a) {
         continue;
       }
       const int64_t end = hi < r1 ? hi : r1;
-      for (; u + kAheadBack <= end; u += kAheadBack) {
-        RawVec<DT, V> x[kAheadBack], dy[kAheadBack];
+      for (; u + AHEAD <= end; u += AHEAD) {
+        RawVec<DT, V> x[AHEAD], dy[AHEAD];
 #pragma unroll
-        for (int k = 0; k < kAheadBack; ++k) {
+        for (int k = 0; k < AHEAD; ++k) {
           x[k].load(a.x, (u + k) * a.D + c, left);
           dy[k].load(a.dy, (u + k) * a.D + c, left);
         }
 #pragma unroll
-        for (int k = 0; k < kAheadBack; ++k) {
+        for (int k = 0; k < AHEAD; ++k) {
           float g[V];
           x[k].get(win[S - 1]);
           dy[k].get(g);
@@ -323,6 +320,16 @@ constexpr int vec(int dt, int64_t S, bool backward) {
   return v < most ? v : most;
 }
 
+// Rows that the backward loads together: four, so that more loads are in flight and the windows
+// move less often, or two where up to 6 taps' rows end within a lane's vector, whose loads one
+// by one are too much code four times over.  Us with two / four, at 2, 3, 4, 6 and 8 taps: bf16
+// 16384 x 2048 54/52, 47/45, 53/50, 66/60, 77/74 (12 taps 117/108), 8192 x 2048 34/34, 30/29,
+// 33/32, 41/40, 50/49, fp32 16384 x 2048 103/93, 106/93, 111/98, 117/104, 128/111; odd rows:
+// bf16 6000 x 1130 26/36, 25/31, 29/36, 48/55, 69/69, 24000 x 1130 67/97, 61/71, 65/77, 96/113,
+// 134/130, fp32 6000 x 1130 23/24, 25/29, 28/33, 42/42, 53/52.  Four loses at 16384 x 4096 with
+// 3 and 4 taps: 91/111, 96/117 (2, 6 and 8 taps: 142/136, 147/129, 166/151).
+constexpr int ahead(int64_t S, bool odd) { return odd && S <= 6 ? 2 : 4; }
+
 // Rows of a strip: as many as still leave about 2048 waves (two a SIMD), 4 to 64.
 int strip(int64_t tokens, int64_t D, int v) {
   const int64_t across = (D + 64 * v - 1) / (64 * v);
@@ -381,8 +388,11 @@ void conv_backward(const Conv& p, const void* x, const void* w, const void* bias
   a.rows = strip(p.seq.n_tokens, p.D, v);
   const int64_t groups = strip_groups(p.seq.n_tokens, a.rows);
   const dim3 grid(static_cast<unsigned>((p.D + 64 * v - 1) / (64 * v)), static_cast<unsigned>(groups));
+  const bool odd = p.D % v != 0;
   with_shape(p.x_dt, p.S, [&](auto DT, auto S) {
-    hipLaunchKernelGGL((conv_bwd<DT.value, S.value, vec(DT.value, S.value, true)>), grid, dim3(64 * kWaves), 0, st, a);
+    constexpr int V = vec(DT.value, S.value, true);
+    auto* k = odd ? conv_bwd<DT.value, S.value, V, ahead(S.value, true)> : conv_bwd<DT.value, S.value, V, ahead(S.value, false)>;
+    hipLaunchKernelGGL(k, grid, dim3(64 * kWaves), 0, st, a);
   });
   if (sums) launch_column_sums({a.part, groups, p.S * p.D, p.D, 0, dw, dbias, nullptr, p.w_dt, p.b_dt, 0}, st);
 }
