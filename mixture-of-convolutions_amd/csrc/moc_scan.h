@@ -84,7 +84,9 @@ __device__ __forceinline__ f32x4 mm2(const Frag<3>& a0, const Frag<3>& a1, const
 }
 
 // Wait states between products made in a branch and the first use of their results behind
-// it: the compiler has been seen to leave them out on a path around a branch's body.
+// it: the compiler has been seen to leave them out on a path around a branch's body.  Which
+// places need it shows tests/test_wait_states.py, which follows every path of the assembly (as
+// the code stands it finds none without these calls either; with other code around it may).
 __device__ __forceinline__ void settle() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 7");
