@@ -339,10 +339,13 @@ constexpr int64_t kWalkers = 1024;
 unsigned grid(int64_t n, int64_t most) { return static_cast<unsigned>(n < most ? n : most); }
 
 // Workgroups of the backward, and rows of partial sums: two a CU, or what the rows
-// give.
-constexpr int64_t kParts = 512;
+// give; of the long kernels 64 (a column a lane, so that the columns fill the card).
+constexpr int64_t kParts = 512, kPartsLong = 64;
 
-int64_t parts(int64_t rows) { return rows < kParts ? rows : kParts; }
+int64_t parts(int64_t rows, int64_t D, int dt) {
+  const int64_t most = plan(D, dt).nv == 0 ? kPartsLong : kParts;
+  return rows < most ? rows : most;
+}
 
 __global__ __launch_bounds__(1024) void column_sums(ColumnSums a) {
   __shared__ float s[32][33];
@@ -382,7 +385,10 @@ void launch_column_sums(const ColumnSums& c, hipStream_t st) {
   hipLaunchKernelGGL(column_sums, dim3(grid((cols + 31) / 32, 1 << 16)), dim3(1024), 0, st, c);
 }
 
-size_t norm_backward_workspace(int64_t rows, int64_t D) { return size_t(parts(rows)) * 2 * D * sizeof(float); }
+size_t norm_backward_workspace(int64_t rows, int64_t D) {
+  // (for either type: fp32's rows end in the long kernels first)
+  return size_t(parts(rows, D, DT_BF16)) * 2 * D * sizeof(float);
+}
 
 void norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows,
                   int64_t D, int dt, int w_dt, int b_dt, float eps, hipStream_t st) {
@@ -406,14 +412,13 @@ void norm_backward(const void* x, const void* w, const void* dy, const float* me
   const Plan p = plan(D, dt);
   float* part = static_cast<float*>(workspace);
   const bool sums = dw != nullptr || db != nullptr;
-  int64_t n = parts(rows);
+  int64_t n = parts(rows, D, dt);
   if (p.nv == 0) {
     if (dx != nullptr) {
       auto* k = dt == DT_BF16 ? norm_dx_long<DT_BF16> : norm_dx_long<DT_F32>;
       hipLaunchKernelGGL(k, dim3(grid(rows, 1 << 22)), dim3(kThreads), 0, st, x, w, dy, mean, rstd, dx, rows, D, w_dt);
     }
     if (sums) {
-      if (n > 64) n = 64;
       auto* k = dt == DT_BF16 ? norm_sums_long<DT_BF16> : norm_sums_long<DT_F32>;
       hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((D + kThreads - 1) / kThreads), static_cast<unsigned>(n)),
                          dim3(kThreads), 0, st, x, dy, mean, rstd, part, rows, D);

@@ -36,3 +36,12 @@ def test_chunks_of_a_differentiated_scan_fit_a_grid():
         assert b"too many chunks" in L.moc_last_error()
         assert L.moc_scan_forward(ref, FAKE, None, None, None, 0, FAKE, 0, None) == ERR_WORKSPACE  # (past the checks)
     assert L.moc_scan_backward(fits, FAKE, 0, None, FAKE, 1 << 50, ctypes.byref(grads), FAKE, 0, None) == ERR_WORKSPACE
+
+
+def test_norm_workspace_of_long_rows():
+    """Rows past what a workgroup's registers hold are summed in 64 parts: no more is asked for."""
+    L = _lib.lib()
+    assert L.moc_norm_backward_workspace_bytes(4096, 1 << 20) == 64 * 2 * (1 << 20) * 4
+    assert L.moc_norm_backward_workspace_bytes(3, 1 << 20) == 3 * 2 * (1 << 20) * 4
+    assert L.moc_norm_backward_workspace_bytes(4096, 16384) == 512 * 2 * 16384 * 4
+    assert L.moc_norm_backward_workspace_bytes(4096, 16385) == 64 * 2 * 16385 * 4
