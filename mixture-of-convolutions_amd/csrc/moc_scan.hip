@@ -298,7 +298,8 @@ __global__ __launch_bounds__(kThreads) void join_segments(Args a, Walk w) {
 }
 
 // ---------------------------------------------------------------------------
-template <int DT, int NT, int VEC>
+// KEEP: w.kept is filled (a form of its own: the others would spill more for code they skip)
+template <int DT, int NT, int VEC, bool KEEP>
 __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void forward_walk(Args a, Walk w, void* y) {
   constexpr int NP = kPlanes<DT>, MP = kFormed<NP>, NB = 4 * NT, W = 64 * NT;
   constexpr bool kCInLds = DT == DT_BF16;  // (three planes of it beside B's would not fit)
@@ -407,8 +408,9 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
     else if (wave == 1) m_blocks(Int<4>{}, Int<5>{});
     else if (wave == 2) m_blocks(Int<8>{}, Int<9>{}, Int<10>{});
     else m_blocks(Int<13>{}, Int<14>{}, Int<15>{});
-    if (w.kept != nullptr && !(k == 0 && from == nullptr))
-      keep_state<NB>(kept_rows<DT, VEC>(a, w.kept, s.kept + k, h, p0, cols, NK), row, NK, acc);
+    const bool keep = KEEP && !(k == 0 && from == nullptr);
+    const Rows<DT, VEC> kept = kept_rows<DT, VEC>(a, w.kept, s.kept + k, h, p0, cols, NK);
+    if (DT == DT_F32 && keep) keep_state<NB>(kept, row, NK, acc);
     if (k + 1 < s.chunks) fetch(k + 1);
     f32x4 ya[4];
 #pragma unroll
@@ -422,6 +424,10 @@ __global__ __launch_bounds__(kThreads, waves_for(kForwardLds<DT, NT>, 3)) void f
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = acc[2 * ks + e / 4][e % 4];
         const Frag<MP> hf = split<MP>(f);
+        if (DT == DT_BF16 && keep && 32 * ks < NK) {
+          kept.put8(row, 32 * ks + 8 * g, hf.v[0]);
+          kept.put8(row, NK + 32 * ks + 8 * g, hf.v[1]);
+        }
 #pragma unroll
         for (int ib = 0; ib < 4; ++ib) {
           Frag<NP> cf;
@@ -724,7 +730,8 @@ void scan_forward(const Scan& p, void* y, const float* init, float* fin, void* s
   launch_segments(a, w, false, st);
   with_types(a, [&](auto DT, auto NT, auto VEC) {
     constexpr size_t lds = kForwardLds<DT.value, NT.value>;
-    auto* k = forward_walk<DT.value, NT.value, VEC.value>;
+    auto* k = w.kept != nullptr ? forward_walk<DT.value, NT.value, VEC.value, true>
+                                : forward_walk<DT.value, NT.value, VEC.value, false>;
     allow_lds(k, lds);
     const dim3 grid(static_cast<unsigned>(pieces(a.seqs, a.seg)),
                     static_cast<unsigned>(p.H * ((p.P + kTile - 1) / kTile)));
