@@ -460,7 +460,9 @@ int moc_conv_update(const void* x, const void* weight, const void* bias, void* c
  * state_dim] in x_dtype (bf16 or f32), tokens *_stride elements apart (below 2^31; not
  * read for a single token), a token's own values contiguous; heads h of group h / (heads / groups) share b and c.  a, d (or NULL),
  * dt_bias (or NULL) [heads] in any dtype.  head_dim <= 128, state_dim <= 256.  States
- * [n_seqs, heads, head_dim, state_dim] f32, fixed length only.
+ * [n_seqs, heads, head_dim, state_dim] f32, fixed length only.  Fewer than 2^24 chunks of 64
+ * tokens of a sequence, 2^23 where `saved` is asked for.  exp of u a summed over up to 64
+ * neighbouring tokens must be finite in f32 (it is where u a <= 0).
  */
 typedef struct MocScan {
   const void* x;
@@ -492,7 +494,9 @@ typedef struct MocScanGrads {
   float* dinitial_state;
 } MocScanGrads;
 
-/* Bytes of `saved` (0: the problem is not one the entry takes). */
+/* Bytes of `saved` (0: the problem is not one the entry takes): a state of 4 bytes an element for
+ * every 64 packed tokens, or for every 64 tokens or fewer of each fixed-length sequence, and 12
+ * bytes a head and token place. */
 size_t moc_scan_saved_bytes(const MocScan* scan);
 
 /* Workspace bytes of moc_scan_forward with or without `saved`. */
@@ -506,7 +510,7 @@ int moc_scan_forward(const MocScan* scan, void* y, const float* initial_state, f
 size_t moc_scan_backward_workspace_bytes(const MocScan* scan);
 
 /* Gradients for dy (contiguous, x dtype) and dfinal_state (or NULL) on the inputs and the
- * `saved` of moc_scan_forward; has_initial_state: whether that call had one.
+ * `saved` of moc_scan_forward; has_initial_state: whether that call had one (fixed length only).
  * dinitial_state may not be dfinal_state.  Sums over tokens and heads are formed in a fixed
  * order. */
 int moc_scan_backward(const MocScan* scan, const void* dy, int has_initial_state, const float* dfinal_state,

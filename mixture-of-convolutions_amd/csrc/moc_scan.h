@@ -405,7 +405,9 @@ struct Span {
 
 // An LDS tile of bf16 planes, W = 64, 128 or 256 columns.  Blocks of 8 columns (16 bytes)
 // of a row are permuted by an exclusive or with f(row), so that both kinds of operand
-// reads meet every bank once.  A 16-byte read serves 16 lanes at a time: rows 0-3 and 12-15
+// reads meet every bank once (state_walk, which has no others, counts no conflicts; with the
+// other accesses forward_walk counts 6.7 million cycles of them and backward_chunk 5.3, beside
+// 3.8 and 10.9 million LDS instructions at 16384 bf16 tokens, 32 heads of 64 x 128).  A 16-byte read serves 16 lanes at a time: rows 0-3 and 12-15
 // at block g with rows 4-11 at block g + 1, or the other way about (lanes 0-3, 12-15, 20-27,
 // then the rest of 32), and their blocks must all differ (for W = 64, where two rows share
 // the banks, those of rows of one parity).  A transposed read meets rows {0-3, 8-11} or

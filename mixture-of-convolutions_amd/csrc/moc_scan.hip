@@ -8,12 +8,13 @@
 // the waves of a workgroup share the chunk's (C B^T o decays) tile in LDS, its blocks on and
 // below the diagonal dealt out 2, 2, 3 and 3.
 //
-// 16384 bf16 tokens, 32 heads of 64 x 128, in 24 segments: forward_walk 79 us, 103 with the
-// states kept for the backward (134 MB); state_walk 38, join 13, prep 7.  x and y alone would
-// take memory 27 us: what bounds the walk is LDS (its reads fill about half of the time) and
+// 16384 bf16 tokens, 32 heads of 64 x 128, in 24 segments: forward_walk 89 us, 133 with the
+// states kept for the backward (268 MB, which alone take memory 53); state_walk 39 (the reverse
+// one, which keeps as much, 99), join 12, prep 7.  x and y alone would take memory 27 us: what
+// bounds the walk without kept states is LDS (its reads fill about half of the time) and
 // vector instructions (a third), which the barriers of a chunk keep apart.  An address kept
 // in a register over a walk is dear: one that spills is reloaded behind the next chunk's
-// loads and waits for them (138 -> 114 us without).
+// loads and waits for them (138 -> 114 us without, when that was changed).
 //
 // A batch of few heads and sequences would leave most CUs idle, so sequences are
 // cut into segments: every segment's own state is formed first (state_walk, no output),
@@ -603,15 +604,18 @@ size_t prep_bytes(const Scan& p) {
 // Segments: a walk's workgroups are heads x segments, and 768 of them are on the card at
 // a time (three a CU, what registers and LDS allow): at most one round of them where
 // sequences are cut, as a second one would run with the card part empty (16384 tokens, 32
-// heads of 64 x 128, forward and backward: 496 us with 768, 523 with 512, 538 with 1024).
+// heads of 64 x 128, forward: 133 us with 768, 142 with 512, 138 with 1024, with the backward
+// 585, 590, 624).
 //
 // Cutting halves a walk's length at the price of a second walk, without output, and the
 // joining.  In units of one workgroup's time for a chunk, alone on its CU (3 us for bf16, 7
 // to 11 for fp32), a walk of q chunks takes q f, f = 1/4 + 3/4 of the workgroups a CU (at
 // least 1), the first walk half of that, and launches and joining 4 (bf16) or 1.3 (fp32).
 // The least of whole sequences, segments from 256 and segments from 128 tokens on is taken
-// (us, whole / 256 / 128: bf16 8 x 777 tokens, 24 heads of 64 x 64: 41 / 50 / 50; 16 x 1000, 8
-// heads of 64 x 128: 60 / 52 / 54; fp32 8 x 600, 12 heads of 64 x 64: 77 / 64 / 46).
+// (us, forward, whole / 256 / 128: bf16 8 x 777 tokens, 24 heads of 64 x 64: 44 / 51 / 50; 2 x
+// 2000, 16 heads of 64 x 128: 121 / 46 / 48; 16 x 1000, 8 heads of 64 x 128: 66 / 56 / 57; fp32 8
+// x 600, 12 heads of 64 x 64: 79 / 68 / 49).  A packed axis counts as one sequence, whatever
+// its longest: 16384 tokens in 256 sequences take 355 us forward where 64 take 160.
 int64_t segment(const Scan& p) {
   const int64_t n = p.seq.n_tokens, heads = p.H * ((p.P + kTile - 1) / kTile);
   const bool packed = p.seq.cu != nullptr;

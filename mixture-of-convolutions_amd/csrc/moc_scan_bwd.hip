@@ -22,10 +22,10 @@
 // eight times a bf16 x), for bf16 in two planes: in one they would move half as much, but each
 // pair's product in dA, a sum over all tokens, would be off by 0.001 and more.
 //
-// 16384 bf16 tokens, 32 heads of 64 x 128: 214 us for 470 MB (2.2 TB/s; 67 us more where the next
-// head's loads were waited for early, by reloads of spilled addresses, by loads of A, C and
-// D behind them and by moves of their registers).  One workgroup of 8 waves fits a CU (230
-// registers, 93 KB), and the phases of a head, parted by three barriers, overlap little:
+// 16384 bf16 tokens, 32 heads of 64 x 128: 255 us back to back for 740 MB (2.9 TB/s; 67 us more
+// where the next head's loads were waited for early, by reloads of spilled addresses, by loads of
+// A, C and D behind them and by moves of their registers).  One workgroup of 8 waves fits a CU
+// (254 registers, 134 KB), and the phases of a head, parted by three barriers, overlap little:
 // vector instructions issue for a third of the time, LDS reads take as much.
 #include <type_traits>
 
@@ -494,11 +494,15 @@ __global__ __launch_bounds__(kThreads) void sum_subs(const float* __restrict__ p
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
 // Parts of a group's heads.  A CU holds one workgroup, so that the time goes with the rounds
-// of 256 of them: each takes a part's heads and, measured in heads (6.4 us for bf16 at 64 x
+// of 256 of them: each takes a part's heads and, measured in heads (8 us for bf16 at 64 x
 // 128, more for fp32), 1.25 (fp32: 0.75) for what is done once a workgroup.  More than one
-// part also costs the launch that adds them and their way through memory.  16384 bf16 tokens,
-// 32 heads of one group: 1 part 213 us, 2 parts 222 + 9, 4 parts 236 + 15; forward and
-// backward of 8000 bf16 tokens, 40 heads of 4 groups, 1 part 323 us, 2 parts 391.
+// part also costs the launch that adds them and their way through memory.  The whole backward
+// in us with 1 / 2 / 4 / 8 parts: bf16 16384 tokens, 32 heads of 64 x 128, one group 378 / 405 /
+// 434 / 485 (1 is taken); 8000 tokens, 40 heads, 4 groups 266 / 312 / 362 / 397 (1); 2 x 2048, 16
+// heads 142 / 101 / 81 / 94 (4); 300 tokens, 32 heads 217 / 124 / 78 / 56 (32: 48); fp32 2 x 2048,
+// 16 heads 337 / 217 / 157 / 173 (4).  Costs are those of heads of 64 x 128: with small heads the
+// rule can miss the best, 3 x 3000 tokens, 10 heads of 40 x 24, 2 groups by 12% (fp32 135 / 120 /
+// 119 / 133, 5 parts are taken: 133) and 9% (bf16 86 / 79 / 79 / 89, 1 is taken).
 int64_t subs_of(const Args& a) {
   const int64_t wgs = a.chunks * a.p.G, hpg = a.p.H / a.p.G;
   const bool bf = a.p.x_dt == DT_BF16;
