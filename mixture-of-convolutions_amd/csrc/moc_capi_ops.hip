@@ -66,7 +66,9 @@ moc::SeqLayout layout(const void* cu, int cu64, int64_t n_seqs, int64_t n_tokens
 }
 
 int check_conv(int64_t dim, int64_t ks, int x_dt, int w_dt, int b_dt, int activation) {
-  if (dim <= 0 || dim >= kMaxTokens) return fail(MOC_ERR_ARG, "dim must be positive, got %lld", (long long)dim);
+  // (a lane has two channels at least, so that 2^31 of them would take a grid of 2^32 threads)
+  if (dim <= 0 || dim >= kMaxTokens / 2)
+    return fail(MOC_ERR_ARG, "dim must be in [1, 2^30), got %lld", (long long)dim);
   if (ks < 1 || ks > moc::kConvMaxS)
     return fail(MOC_ERR_ARG, "kernel_size must be in [1, %d], got %lld", moc::kConvMaxS, (long long)ks);
   if (!x_dt_ok(x_dt)) return fail(MOC_ERR_DTYPE, "unsupported x dtype code %d (bf16 or f32 only)", x_dt);

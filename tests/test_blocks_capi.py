@@ -45,3 +45,14 @@ def test_norm_workspace_of_long_rows():
     assert L.moc_norm_backward_workspace_bytes(3, 1 << 20) == 3 * 2 * (1 << 20) * 4
     assert L.moc_norm_backward_workspace_bytes(4096, 16384) == 512 * 2 * 16384 * 4
     assert L.moc_norm_backward_workspace_bytes(4096, 16385) == 64 * 2 * 16385 * 4
+
+
+def test_conv_channels_fit_a_grid():
+    """2^31 - 1 channels, two a lane, would be a grid of 2^32 threads, which runs none of them."""
+    L = _lib.lib()
+    for dim in ((1 << 31) - 1, 1 << 30, 0):
+        assert L.moc_conv_forward(FAKE, FAKE, None, None, FAKE, None, None, 0, 0, 1, 1, dim, 16, 0, 0, 0, 0, None) == ERR_ARG
+        assert L.moc_conv_backward(FAKE, FAKE, None, FAKE, FAKE, FAKE, None, None, 0, 0, 1, 1, dim, 16, 0, 0, 0, 0, FAKE,
+                                   1 << 60, None) == ERR_ARG
+        assert L.moc_conv_update(FAKE, FAKE, None, FAKE, 1, 1, 1, FAKE, 1, dim, 16, 0, 0, 0, 0, None) == ERR_ARG
+        assert b"dim must be" in L.moc_last_error()
